@@ -4,7 +4,7 @@ A cache keeps the keys and values of every sequence and head as int8, with the l
 integer q of a block with the magnitude a stands for q * a / 127.  Three operators work on it:
 
     write   tokens enter at a position of their sequence; a block that holds older tokens already grows to the larger magnitude, and the older
-            integers are rounded again to it:  q = rint(127 x / a),  q' = rint(q a / a')
+            integers are rounded again to it:  q = round(127 x / a),  q' = round(q a / a'), both to the nearest integer, halves away from zero
     read    a range of tokens comes back as fp16
     attend  softmax(scale q k^T + position bias, over the keys that length, causality and mask leave) v, straight from the integers: the decode
             step's single query, a few drafted tokens, whole chunks of a prompt
@@ -133,13 +133,18 @@ class _Source:
         return x.view(batch, heads, dim, tokens).transpose(2, 3) if layout == "columns" else x.view(batch, tokens, heads, dim).transpose(1, 2)
 
 
+def _nearest(x):
+    """The nearest integer, halves away from zero."""
+    return torch.sign(x) * torch.floor(x.abs() + 0.5)
+
+
 def _cache(src, batch, heads, length, dim, block):
     """Keys or values (batch, heads, length, dim) as integers, and the blocks' magnitudes."""
     x = src.normal(batch, heads, length, dim)
     x *= torch.exp(0.5 * torch.randn((heads, 1, dim), generator=src.gen, device="cuda")).half()
     blocks = x.view(batch, heads, length // block, block, dim)
     top = blocks.abs().amax((3, 4))
-    ints = torch.round(127 * blocks.float() / top[..., None, None].float().clamp(min=1e-30)).to(torch.int8)
+    ints = _nearest(127 * blocks.float() / top[..., None, None].float().clamp(min=1e-30)).to(torch.int8)
     return ints.view(batch, heads, length, dim), top
 
 
@@ -255,8 +260,8 @@ def _write(s, ints, top, x, values):
     else:
         held = ints.transpose(1, 2)[batches, at].float()
     div = torch.where(after > 0, after, torch.ones_like(after)).repeat_interleave(block, 1)[..., None]
-    again = torch.round(held * before.repeat_interleave(block, 1)[..., None] / div)
-    fresh = torch.round(127 * picked / div)
+    again = _nearest(held * before.repeat_interleave(block, 1)[..., None] / div)
+    fresh = _nearest(127 * picked / div)
     moved = old & touched.view(b, blocks).repeat_interleave(block, 1)
     result = torch.where(new[:, :, None, None], fresh, torch.where(moved[:, :, None, None], again, held)).to(torch.int8)
     if values:
@@ -322,8 +327,10 @@ def _exact_write(ints, top, x, pos, count, block):
         a = fresh.abs().amax((1, 2))
         if t > blk * block:
             a = torch.maximum(a, top[:, blk])
-            ints[:, blk * block:t] = torch.round(ints[:, blk * block:t] * top[:, blk, None, None] / a.clamp(min=1e-300)[:, None, None])
-        ints[:, t:end] = torch.round(127 * fresh / a.clamp(min=1e-300)[:, None, None])
+            again = ints[:, blk * block:t] * top[:, blk, None, None] / a.clamp(min=1e-300)[:, None, None]
+            ints[:, blk * block:t] = torch.where(again < 0, torch.ceil(again - 0.5), torch.floor(again + 0.5))
+        parts = 127 * fresh / a.clamp(min=1e-300)[:, None, None]
+        ints[:, t:end] = torch.where(parts < 0, torch.ceil(parts - 0.5), torch.floor(parts + 0.5))
         top[:, blk] = a
         t = end
 
