@@ -10,7 +10,7 @@ import sys
 
 from cpm_kernels_amd.torch import *  # noqa: F401,F403
 
-SUBMODULES = ("arith", "embedding", "gelu", "gemm", "layernorm", "mask", "position_embedding",
+SUBMODULES = ("arith", "embedding", "gelu", "gemm", "kv_cache", "layernorm", "mask", "position_embedding",
               "softmax", "transpose", "utils")
 
 for _name in SUBMODULES:

@@ -3,7 +3,7 @@ launchers this build adds (gemm_int8_scale, gemm_quantize, gemm_quantize_cols, g
 their `_ld` forms with padded rows, gemm_int8_scale_one, gemm_int8_scale_sum, gemm_fp16_sum, gemm_int8_scale_parts, gemm_fp16_parts,
 gemm_add_parts, gemm_int8_scale_split, gemm_fp16_split, gemm_quantize_cols_rows, gemm_backward_quantize_both, layernorm_affine_forward,
 layernorm_affine_forward_stats, layernorm_affine_backward, embedding_order_ids, embedding_backward_rows,
-embedding_backward_prepare)."""
+embedding_backward_prepare) and the key/value cache in 8 bits (kv_write_int8, kv_read_int8, kv_attention_int8)."""
 from .embedding import embedding_forward, embedding_backward_stage1, embedding_backward_stage2, embedding_step, \
     embedding_order_ids, embedding_backward_rows, embedding_backward_prepare
 from .gelu import gelu_forward, gelu_backward, gelu_inplace_forward
@@ -15,6 +15,7 @@ from .gemm import gemm_calc_scale, gemm_calc_scale_transpose, gemm_round, gemm_r
     gemm_depth_parts, gemm_fp16_copy_pays, gemm_int8_scale_split, gemm_fp16_split, gemm_quantize_cols_rows, gemm_backward_quantize_both
 from .gemv import gemv_fp16, gemv_broadcast_mat_int8, gemv_fp16_transpose, gemv_broadcast_mat_fp16, \
     gemv_calc_scale, gemv_round, gemv_broadcast_mat_fp16_light, gemv_fp16_light, gemv_fp16_transpose_light
+from .kv_cache import kv_write_int8, kv_read_int8, kv_attention_int8, kv_attention_int8_workspace
 from .mask import mask
 from .arith import arith_batch_add_backward, arith_batch_add_forward, arith_element_add, arith_ln_add_backward, \
     arith_ln_div, arith_ln_mul, arith_ln_mul_add, arith_ln_mul_backward, arith_ln_sub_div, arith_element_mul, \

@@ -40,7 +40,9 @@ _LAUNCHERS = {
     "position_embedding_backward": "iiiiipppip", "embedding_backward_stage1": "iiippppppp",
     "embedding_backward_stage2": "iipppp", "embedding_order_ids": "ipppp", "embedding_backward_rows": "iipppppp", "embedding_backward_prepare": "iiiippppppp",
     "transpose": "iiippp", "transpose_i8": "iiippp", "array_add": "piip", "adjustify_logits": "iipfffpp",
-    "copy_extend_buffer": "iiippp", "has_nan_inf": "lppp", "copy_pos_hidden": "iiiippp", "async_status": "",
+    "copy_extend_buffer": "iiippp",
+    "kv_write_int8": "iiiiiipllllpllllpipppppp", "kv_read_int8": "iiiiiipppppippllllp", "kv_attention_int8": "iiiiiiipllllpppppipiifppiiipllpllllpp",
+    "has_nan_inf": "lppp", "copy_pos_hidden": "iiiippp", "async_status": "",
     "selftest_exchange_timeout": "ip",
 }
 _CTYPES = {"i": ctypes.c_int32, "l": ctypes.c_int64, "f": ctypes.c_float, "p": ctypes.c_void_p}
@@ -48,7 +50,7 @@ _CTYPES = {"i": ctypes.c_int32, "l": ctypes.c_int64, "f": ctypes.c_float, "p": c
 EXPORTED_SYMBOLS = sorted(["cpmk_" + n for n in _LAUNCHERS] + [
     "cpmk_version", "cpmk_error_string", "cpmk_device_count", "cpmk_get_device",
     "cpmk_set_device", "cpmk_device_props", "cpmk_exchange_capture_slots_left", "cpmk_gemm_sum_groups", "cpmk_gemm_sum_groups_for", "cpmk_gemm_sum_krows_groups",
-    "cpmk_gemm_sum_groups_timed",
+    "cpmk_gemm_sum_groups_timed", "cpmk_kv_attention_int8_workspace",
     "cpmk_gemm_depth_parts", "cpmk_gemm_fp16_copy_pays",
 ])
 
@@ -148,6 +150,11 @@ def gemm_depth_parts(f16: int, m: int, k: int, n: int, batchA: int, batchB: int,
 @lib.bind("cpmk_gemm_fp16_copy_pays", [ctypes.c_int32] * 4 + [ctypes.c_int], ctypes.c_int)
 def gemm_fp16_copy_pays(m: int, k: int, n: int, batch: int, bT: int) -> int:
     return lib.cpmk_gemm_fp16_copy_pays(m, k, n, batch, bT)
+
+
+@lib.bind("cpmk_kv_attention_int8_workspace", [ctypes.c_int32] * 6, ctypes.c_int64)
+def kv_attention_int8_workspace(batch: int, heads: int, kv_heads: int, tokens: int, dim: int, length: int) -> int:
+    return lib.cpmk_kv_attention_int8_workspace(batch, heads, kv_heads, tokens, dim, length)
 
 
 @lib.bind("cpmk_device_count", [ctypes.POINTER(ctypes.c_int)], ctypes.c_int)

@@ -141,6 +141,9 @@ PyMethodDef g_launchers[] = {
     CPMK_ENTRY(cpmk_embedding_forward)
     CPMK_ENTRY(cpmk_embedding_step)
     CPMK_ENTRY(cpmk_copy_data_to_kv)
+    CPMK_ENTRY(cpmk_kv_write_int8)
+    CPMK_ENTRY(cpmk_kv_read_int8)
+    CPMK_ENTRY(cpmk_kv_attention_int8)
     CPMK_ENTRY(cpmk_gemv_calc_scale)
     CPMK_ENTRY(cpmk_gemv_round)
     CPMK_ENTRY(cpmk_gemv_broadcast_mat_int8)

@@ -15,6 +15,7 @@ from .arith import (
 from .embedding import Embedding, EmbeddingTH, OpEmbedding
 from .gelu import gelu, gelu_inplace, geluTH
 from .gemm import bmm
+from .kv_cache import QuantizedKV
 from .layernorm import LayerNorm, LayerNormTH, normalize_inplace, normalizeTH
 from .mask import mask, mask_inplace, maskTH
 from .position_embedding import PositionEmbedding, PositionEmbeddingTH

@@ -479,6 +479,43 @@ int cpmk_has_nan_inf(int64_t n, const void* inp, void* out, void* stream);
 int cpmk_copy_pos_hidden(int32_t batch, int32_t hidden_size, int32_t seq_len, int32_t pos, const void* inp,
                          void* out, void* stream);
 
+/* ---- key/value cache in 8 bits (beside cpmk_copy_data_to_kv, which keeps fp16; no counterpart in the reference) ----
+ * keys (batch, heads, length, dim) int8, values (batch, heads, length / 16, dim, 16) int8 (sixteen tokens of one unit side by side), and for each of
+ * them absmax (batch, heads, length / block) fp16, the largest magnitude of a block of tokens: an integer q of a block stands for q * absmax / 127.
+ * dim a multiple of 16, at most 256; block 16, 32, 64 or 128; length a multiple of block; length * dim below 2^31; keys and values 16-byte aligned.
+ * The fp16 tensors (batch, heads, tokens, dim) come with the strides of their axes, in elements. */
+
+/* Tokens into the cache: token i of sequence b to position pos_each[b] + i (pos + i if pos_each is NULL), for i < count_each[b] (all `tokens` if it is
+ * NULL).  q = round(127 x / absmax), halves away from zero, infinities as +-65504 and NaN as 0; a block that holds older tokens of the sequence (positions
+ * below the first one written) keeps the larger of both magnitudes, its older integers rounded again to it.  What lies behind the last token written is
+ * left as it is.  Positions on the device: a sequence whose position is negative is left alone, tokens that would come to lie behind the cache are dropped. */
+int cpmk_kv_write_int8(int32_t batch, int32_t heads, int32_t tokens, int32_t dim, int32_t length, int32_t block,
+                       const void* k /* fp16 */, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit,
+                       const void* v /* fp16 */, int64_t v_batch, int64_t v_head, int64_t v_token, int64_t v_unit,
+                       const void* pos_each /* (batch) int32 or NULL */, int32_t pos, const void* count_each /* (batch) int32 or NULL */,
+                       void* keys, void* values, void* key_absmax, void* value_absmax, void* stream);
+/* Positions from_each[b] (or from) .. + tokens - 1 of every sequence as fp16; zeros where a position lies outside of the cache.  k and v have the same strides. */
+int cpmk_kv_read_int8(int32_t batch, int32_t heads, int32_t tokens, int32_t dim, int32_t length, int32_t block,
+                      const void* keys, const void* values, const void* key_absmax, const void* value_absmax,
+                      const void* from_each /* (batch) int32 or NULL */, int32_t from, void* k /* fp16 */, void* v /* fp16 */,
+                      int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit, void* stream);
+/* out[b,h,i,:] = sum_j p_j v_j, p = softmax over j of scale * q[b,h,i,:] . k_j + bias[h, bucket(at - j)], query head h on cache head
+ * h / (heads / kv_heads), at = the query's position: pos_each[b] + i, or pos + i, or, with a negative pos, lens[b] - tokens + i.  Key j counts where
+ * j < lens_each[b] (or len), j <= at if causal, and mask[b * mask_batch + i * mask_token + j] != 0 if there is a mask (rows of `length` bytes; a
+ * mask_token of 0 for one row a sequence).  A query that no key is left for gives zeros.  bias: the table of cpmk_position_embedding_forward, buckets
+ * as there (mapping of cpmk_position_embedding_init), at most 1024 distances (both signs counted if bidirectional); NULL for none.
+ * workspace: cpmk_kv_attention_int8_workspace() bytes on the device, 4-byte aligned, the call's own until it has finished; NULL if that is 0. */
+int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length, int32_t block,
+                           const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
+                           const void* keys, const void* values, const void* key_absmax, const void* value_absmax,
+                           const void* lens_each /* (batch) int32 or NULL */, int32_t len, const void* pos_each /* (batch) int32 or NULL */, int32_t pos,
+                           int causal, float scale, const void* bias /* (heads, num_buckets) fp16 or NULL */, const void* mapping /* (max_distance) int32 */,
+                           int32_t num_buckets, int32_t max_distance, int bidirectional,
+                           const void* mask /* bool or NULL */, int64_t mask_batch, int64_t mask_token,
+                           void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit,
+                           void* workspace, void* stream);
+int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length);
+
 #ifdef __cplusplus
 }
 #endif
