@@ -1,0 +1,82 @@
+// What the kernels of the attention over the 8-bit key/value cache share (kv_attention.hip: few queries, kv_chunk.hip: many).
+#pragma once
+#include "common.h"
+
+namespace cpmk {
+
+struct KvAttention {
+    const half_t* q;
+    int64_t q_batch, q_head, q_token, q_unit;
+    const int8_t *keys, *values;
+    const half_t *key_top, *value_top;
+    const int32_t *lens_each, *pos_each;
+    const half_t* table;            // (heads, buckets) or null
+    const int32_t* mapping;
+    const uint8_t* mask;
+    int64_t mask_batch, mask_token;
+    half_t* out;
+    int64_t out_batch, out_head, out_token, out_unit;
+    float* parts;
+    float scale;                    // with log2(e)
+    int32_t len, pos;               // pos < 0: the queries are the last of the keys
+    int32_t heads, held, group, tokens, dim, length, block_shift, buckets, distances, first_distance;
+    int32_t causal;
+    int32_t row_tiles, splits;
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kTile = 64;           // keys a wave takes at a time
+constexpr int32_t kFar = 1 << 30;   // positions and rows stay below
+constexpr int kChunkLeast = 4;       // tiles of a part, at least (kv_chunk.hip)
+constexpr int kChunkPad = 96;        // distances beyond the table's ends that a tile of 32 queries and 64 keys can reach into
+
+// sixteen bytes as integers -> halves, exactly: 1024 + 128 + q has q in its last bits
+__device__ __forceinline__ void halves_of(uint4_t p, half8_t& lo, half8_t& hi) {
+    uint32_t h[8];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t u = p[d] ^ 0x80808080u;
+        h[2 * d] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+        h[2 * d + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    }
+    const half2_t off = {(half_t)1152.0f, (half_t)1152.0f};
+    uint4_t a, b;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        a[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[d]) - off);
+        b[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[4 + d]) - off);
+    }
+    lo = __builtin_bit_cast(half8_t, a);
+    hi = __builtin_bit_cast(half8_t, b);
+}
+
+__device__ __forceinline__ float kv_scale(half_t top) { return fmaxf((float)top * (1.0f / 127.0f), 0x1p-34f); }
+
+// The keys that a tile of rows looks at: how many, and the parts they are cut into (the same here and where the parts are joined).
+struct KvRange {
+    int32_t len, pos, keys, tiles, per_part, parts;
+};
+__device__ __forceinline__ KvRange kv_range(const KvAttention& a, int64_t b, int32_t last_query, int least) {
+    KvRange r;
+    r.len = max(0, min(a.lens_each ? a.lens_each[b] : a.len, a.length));
+    r.pos = a.pos_each ? max(-kFar, min(a.pos_each[b], kFar - 1)) : a.pos < 0 ? r.len - a.tokens : min(a.pos, kFar - 1);
+    r.keys = a.causal ? max(0, min(r.len, r.pos + last_query + 1)) : r.len;
+    r.tiles = (r.keys + kTile - 1) / kTile;
+    r.per_part = max((r.tiles + a.splits - 1) / a.splits, min(least, max(r.tiles, 1)));
+    r.parts = max(1, (r.tiles + r.per_part - 1) / r.per_part);
+    return r;
+}
+
+// The biases of a head over the distances first .. first + count - 1, in units of log2, to LDS: entry i is that of distance first + i, those off the table's ends
+// at its ends.
+__device__ __forceinline__ float kv_bias(const KvAttention& a, int32_t head, int32_t rel) {
+    rel = max(a.first_distance, min(rel, a.distances - 1));
+    const int32_t bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
+    return (float)a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))] * kLog2e;
+}
+
+// Many queries (kv_chunk.hip).  How many rows a part of one query tile has, and the launch (0 or an error code).
+int kv_chunk_rows(int32_t tokens, int32_t dim);
+int kv_chunk_launch(const KvAttention& a, int32_t batch, hipStream_t st);
+
+}  // namespace cpmk

@@ -11,70 +11,11 @@
 //
 // Work is divided over the keys too where rows are few: a workgroup takes every tile of 64 keys of its part, wave by wave, and its waves join their sums
 // through LDS; parts leave theirs in the workspace and a second kernel joins them.
-#include "common.h"
+#include "kv_attention.h"
 
 namespace cpmk {
 
-struct KvAttention {
-    const half_t* q;
-    int64_t q_batch, q_head, q_token, q_unit;
-    const int8_t *keys, *values;
-    const half_t *key_top, *value_top;
-    const int32_t *lens_each, *pos_each;
-    const half_t* table;            // (heads, buckets) or null
-    const int32_t* mapping;
-    const uint8_t* mask;
-    int64_t mask_batch, mask_token;
-    half_t* out;
-    int64_t out_batch, out_head, out_token, out_unit;
-    float* parts;
-    float scale;                    // with log2(e)
-    int32_t len, pos;               // pos < 0: the queries are the last of the keys
-    int32_t heads, held, group, tokens, dim, length, block_shift, buckets, distances, first_distance;
-    int32_t causal;
-    int32_t row_tiles, splits;
-};
-
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kTile = 64;           // keys a wave takes at a time
-constexpr int32_t kFar = 1 << 30;   // positions and rows stay below
-
-// sixteen bytes as integers -> halves, exactly: 1024 + 128 + q has q in its last bits
-__device__ __forceinline__ void halves_of(uint4_t p, half8_t& lo, half8_t& hi) {
-    uint32_t h[8];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        const uint32_t u = p[d] ^ 0x80808080u;
-        h[2 * d] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-        h[2 * d + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    }
-    const half2_t off = {(half_t)1152.0f, (half_t)1152.0f};
-    uint4_t a, b;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        a[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[d]) - off);
-        b[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[4 + d]) - off);
-    }
-    lo = __builtin_bit_cast(half8_t, a);
-    hi = __builtin_bit_cast(half8_t, b);
-}
-
-__device__ __forceinline__ float kv_scale(half_t top) { return fmaxf((float)top * (1.0f / 127.0f), 0x1p-34f); }
-
-// The keys that a tile of rows looks at: how many, and the parts they are cut into (the same here and where the parts are joined).
-struct KvRange {
-    int32_t len, pos, keys, tiles, per_part, parts;
-};
-__device__ __forceinline__ KvRange kv_range(const KvAttention& a, int64_t b, int32_t last_query, int waves) {
-    KvRange r;
-    r.len = max(0, min(a.lens_each ? a.lens_each[b] : a.len, a.length));
-    r.pos = a.pos_each ? max(-kFar, min(a.pos_each[b], kFar - 1)) : a.pos < 0 ? r.len - a.tokens : min(a.pos, kFar - 1);
-    r.keys = a.causal ? max(0, min(r.len, r.pos + last_query + 1)) : r.len;
-    r.tiles = (r.keys + kTile - 1) / kTile;
-    r.per_part = max((r.tiles + a.splits - 1) / a.splits, min(waves, max(r.tiles, 1)));
-    r.parts = max(1, (r.tiles + r.per_part - 1) / r.per_part);
-    return r;
-}
+constexpr int kWaves = 4;
 
 // DS: 64-unit steps of a head.
 template <int DS, int WAVES, bool BIAS, bool MASK>
@@ -251,38 +192,53 @@ __global__ __launch_bounds__(WAVES * 64) void k_kv_attend(KvAttention a) {
     }
 }
 
-// One row a workgroup of 256: parts joined under the largest of their maxima.
-__global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int waves) {
-    const int32_t rows = a.tokens * a.group;
-    uint32_t w = blockIdx.x;
-    const int32_t r = w % (uint32_t)rows;
-    w /= (uint32_t)rows;
-    const int32_t kvh = w % (uint32_t)a.held;
-    const int64_t b = w / (uint32_t)a.held;
-    const int32_t rt = r >> 4, query = r / a.group, g = r - query * a.group;
-    const KvRange range = kv_range(a, b, min(rt * 16 + 15, rows - 1) / a.group, waves);
-    const int64_t size = 16 * (int64_t)(a.dim + 2);
-    const float* const part = a.parts + ((b * a.held + kvh) * a.row_tiles + rt) * a.splits * size;
-    const float* const tops = part + 16 * a.dim + (r & 15);
+// Parts joined under the largest of their maxima: a wave a row, its lanes along the units.  `rows` of them lie together (sixteen rows of a head of the cache, or queries of a query head).
+__global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int chunks, uint32_t total_rows) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= total_rows) return;
+    const int32_t group = chunks ? 1 : a.group, heads = chunks ? a.heads : a.held, of_head = a.tokens * group;
+    const int32_t r = id % (uint32_t)of_head;
+    const uint32_t w = id / (uint32_t)of_head;
+    const int32_t h = w % (uint32_t)heads;
+    const int64_t b = w / (uint32_t)heads;
+    const int32_t rt = r / rows, in_tile = r - rt * rows, query = r / group, g = r - query * group;
+    const KvRange range = kv_range(a, b, min(rt * rows + rows - 1, of_head - 1) / group, chunks ? kChunkLeast : kWaves);
+    const int64_t size = (int64_t)rows * (a.dim + 2);
+    const float* const part = a.parts + ((b * heads + h) * a.row_tiles + rt) * a.splits * size;
+    const float* const tops = part + rows * a.dim + in_tile;
     float m = -__builtin_inff();
-    for (int i = 0; i < range.parts; ++i) m = fmaxf(m, tops[i * size]);
+    for (int i = lane; i < range.parts; i += 64) m = fmaxf(m, tops[i * size]);
+    m = wave_max(m);
     const float base = m == -__builtin_inff() ? 0.0f : m;
-    float total = 0.0f;
-    for (int i = 0; i < range.parts; ++i) total = __builtin_fmaf(tops[i * size + 16], __builtin_amdgcn_exp2f(tops[i * size] - base), total);
-    for (int u = threadIdx.x; u < a.dim; u += 256) {
-        float value = 0.0f;
-        for (int i = 0; i < range.parts; ++i) value = __builtin_fmaf(part[i * size + (r & 15) * a.dim + u], __builtin_amdgcn_exp2f(tops[i * size] - base), value);
-        a.out[b * a.out_batch + (int64_t)(kvh * a.group + g) * a.out_head + (int64_t)query * a.out_token + (int64_t)u * a.out_unit] =
-            (half_t)(total == 0.0f ? 0.0f : value / total);
+    float total = 0.0f, value[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < range.parts; ++i) {
+        const float f = __builtin_amdgcn_exp2f(tops[i * size] - base);
+        total = __builtin_fmaf(tops[i * size + rows], f, total);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c * 64 + lane < a.dim) value[c] = __builtin_fmaf(part[i * size + in_tile * a.dim + c * 64 + lane], f, value[c]);
     }
+    half_t* const out = a.out + b * a.out_batch + (int64_t)(h * group + g) * a.out_head + (int64_t)query * a.out_token;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c * 64 + lane < a.dim) out[(int64_t)(c * 64 + lane) * a.out_unit] = (half_t)(total == 0.0f ? 0.0f : value[c] / total);
 }
 
-constexpr int kWaves = 4;
-
-static int kv_splits(int64_t batch, int64_t held, int64_t row_tiles, int64_t length) {
-    const int64_t base = batch * held * row_tiles, most = ceil_div(length, kTile * kWaves);
-    const int64_t s = ceil_div(4 * (int64_t)compute_units(), base);
-    return (int)(s < 1 ? 1 : s > most ? most : s);
+// Which kernel a call takes, and into how many parts its keys are cut.
+struct KvPlan {
+    int rows, row_tiles, splits;
+    bool chunks;
+};
+static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length) {
+    KvPlan p;
+    p.chunks = tokens > 32;
+    p.rows = p.chunks ? kv_chunk_rows((int32_t)tokens, dim) : 16;
+    p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
+    const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, most = ceil_div(length, kTile * (p.chunks ? kChunkLeast : kWaves));
+    const int64_t want = ceil_div((p.chunks ? 1 : 4) * (int64_t)compute_units(), base);
+    p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+    return p;
 }
 
 template <int DS>
@@ -303,9 +259,9 @@ extern "C" {
 
 int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length) {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || dim <= 0 || length <= 0 || heads % kv_heads) return 0;
-    const int64_t row_tiles = ceil_div((int64_t)tokens * (heads / kv_heads), 16);
-    const int splits = kv_splits(batch, kv_heads, row_tiles, length);
-    return splits > 1 ? (int64_t)batch * kv_heads * row_tiles * splits * 16 * (dim + 2) * (int64_t)sizeof(float) : 0;
+    if ((int64_t)tokens * (heads / kv_heads) > kFar) return 0;
+    const KvPlan p = kv_plan(batch, heads, kv_heads, tokens, dim, length);
+    return p.splits > 1 ? (int64_t)batch * (p.chunks ? heads : kv_heads) * p.row_tiles * p.splits * p.rows * (dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
 int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length, int32_t block, const void* q,
@@ -337,17 +293,20 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     a.parts = (float*)workspace, a.scale = scale * kLog2e, a.causal = causal != 0;
     a.heads = heads, a.held = kv_heads, a.group = heads / kv_heads, a.tokens = tokens, a.dim = dim, a.length = length;
     a.block_shift = __builtin_ctz((unsigned)block);
-    a.row_tiles = (int32_t)ceil_div((int64_t)tokens * a.group, 16);
-    a.splits = kv_splits(batch, kv_heads, a.row_tiles, length);
+    const KvPlan plan = kv_plan(batch, heads, kv_heads, tokens, dim, length);
+    a.row_tiles = plan.row_tiles, a.splits = plan.splits;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;
     const int64_t grid = (int64_t)batch * kv_heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
     if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
     hipStream_t st = (hipStream_t)stream;
-    if (dim <= 64) kv_launch<1>(a, (unsigned)grid, st);
+    if (plan.chunks) {
+        if (int e = kv_chunk_launch(a, batch, st)) return e;
+    } else if (dim <= 64) kv_launch<1>(a, (unsigned)grid, st);
     else if (dim <= 128) kv_launch<2>(a, (unsigned)grid, st);
     else if (dim <= 192) kv_launch<3>(a, (unsigned)grid, st);
     else kv_launch<4>(a, (unsigned)grid, st);
-    if (a.splits > 1) hipLaunchKernelGGL(k_kv_join, dim3((unsigned)rows), dim3(256), 0, st, a, kWaves);
+    if (a.splits > 1)
+        hipLaunchKernelGGL(k_kv_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan.rows, (int)plan.chunks, (uint32_t)rows);
     return launch_status();
 }
 

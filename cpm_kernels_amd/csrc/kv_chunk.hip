@@ -1,0 +1,299 @@
+// Attention over the 8-bit key/value cache for chunks of queries (the mathematics: kv_attention.hip).
+//
+// A workgroup has 32 queries a wave of one head and goes over its keys in tiles of 64.  It turns a tile's integers into fp16 once, for all its waves, into LDS, two tiles in turn:
+// while one is multiplied the next is converted and the one behind it is on its way from memory.  Scores are formed transposed with v_mfma_f32_32x32x16_f16, keys as
+// the rows in an order that leaves each lane sixteen neighbouring keys (one block of magnitudes) of one query twice, so the probabilities go from the lane's registers
+// straight into the second product.  The running maximum follows the true one at a distance of up to 2^8: fp16 keeps the probabilities' bits either way, and the sums are rescaled
+// in the first tiles only.
+//
+// LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at (2 u + h) 64 + (r ^ (u & 7)), read along r; the exclusive or spreads the eight unit steps that
+// neighbouring lanes write over the banks.  Values (group of sixteen keys g, half s, unit) at (2 g + s) D + unit.
+#include "kv_attention.h"
+
+namespace cpmk {
+
+constexpr int kLazy = 8;
+
+// NT: 32-unit steps of a head, NW: waves
+template <int NT, int NW, bool BIAS, bool MASK>
+__global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
+    constexpr int D = NT * 32, KS = NT * 2, NTHR = NW * 64, PIECES = (8 * D + NTHR - 1) / NTHR, ROWS = NW * 32;
+    constexpr int kKeyBytes = 64 * D * 2, kBuffer = 2 * kKeyBytes;
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+    float* const biases = reinterpret_cast<float*>(lds + 2 * kBuffer);
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+    const int32_t split = w % (uint32_t)a.splits;
+    w /= (uint32_t)a.splits;
+    const int64_t tile_of = w;
+    const int32_t qt = w % (uint32_t)a.row_tiles;
+    w /= (uint32_t)a.row_tiles;
+    const int32_t h = w % (uint32_t)a.heads;
+    const int64_t b = w / (uint32_t)a.heads;
+    const KvRange range = kv_range(a, b, min(qt * ROWS + ROWS - 1, a.tokens - 1), kChunkLeast);
+    if (split >= range.parts) return;
+
+    const int32_t q_first = qt * ROWS + wave * 32;
+    const int32_t query = min(q_first + col, a.tokens - 1);         // (queries past the end repeat the last one)
+    const int32_t where = range.pos + query, limit = a.causal ? min(range.len, where + 1) : range.len;
+    // what all and what any of the wave's queries see
+    const int32_t last = min(q_first + 31, a.tokens - 1);
+    const int32_t all_see = a.causal ? min(range.len, range.pos + min(q_first, a.tokens - 1) + 1) : range.len;
+    const int32_t any_sees = q_first >= a.tokens ? 0 : a.causal ? min(range.len, range.pos + last + 1) : range.len;
+    const bool flip = a.scale < 0.0f;           // (so that the largest score is the largest product)
+    const float scale = flip ? -a.scale : a.scale;
+
+    half8_t q[KS];
+    {
+        const half_t* p = a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int u = s * 16 + half * 8;
+            q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            if (u < a.dim) {
+                if (a.q_unit == 1) q[s] = load_half8_any(p + u);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[s][e] = p[(u + e) * a.q_unit];
+            }
+            if (flip) q[s] = -q[s];
+        }
+    }
+    const int32_t lo_rel = a.first_distance - kChunkPad;
+    if (BIAS)
+        for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
+
+    const int64_t head = b * a.held + h / a.group;
+    const int8_t* const keys = a.keys + head * a.length * a.dim;
+    const int8_t* const values = a.values + head * a.length * a.dim;
+    const half_t* const key_top = a.key_top + (head * a.length >> a.block_shift);
+    const half_t* const value_top = a.value_top + (head * a.length >> a.block_shift);
+    const uint8_t* const mask = MASK ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
+
+    // the pieces of a tile that this thread brings: keys first, a token's units side by side, then values as they lie
+    const int runs = a.dim >> 4;
+    int32_t at_lds[PIECES], row[PIECES], offset[PIECES];
+    bool is_key[PIECES], real[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = tid + i * NTHR;
+        real[i] = p < 8 * a.dim;
+        is_key[i] = p < 4 * a.dim;
+        if (is_key[i]) {
+            const int key = p / runs, u = p - key * runs;
+            const int r = (key & 32) | ((key >> 2) & 3) << 3 | ((key >> 4) & 1) << 2 | (key & 3);
+            row[i] = key;
+            offset[i] = u * 16;
+            at_lds[i] = (u * 128 + (r ^ (u & 7))) * 16;
+        } else {
+            const int v = p - 4 * a.dim, g = min(v / a.dim, 3), unit = v - g * a.dim;
+            row[i] = g * 16;
+            offset[i] = unit * 16;
+            at_lds[i] = kKeyBytes + (g * 2 * D + unit) * 16;
+        }
+    }
+    uint4_t raw[PIECES];
+    auto fetch = [&](int32_t tile) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int32_t k = min(tile * kTile + row[i], is_key[i] ? a.length - 1 : a.length - 16);
+            if (real[i]) raw[i] = *reinterpret_cast<const uint4_t*>((is_key[i] ? keys : values) + k * a.dim + offset[i]);
+        }
+    };
+    auto convert = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            if (real[i]) {
+                half8_t lo, hi;
+                halves_of(raw[i], lo, hi);
+                int8_t* const p = lds + buffer * kBuffer + at_lds[i];
+                *reinterpret_cast<half8_t*>(p) = lo;
+                *reinterpret_cast<half8_t*>(p + (is_key[i] ? 64 : D) * 16) = hi;
+            }
+    };
+    const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
+    if (t_begin < t_end) fetch(t_begin);
+    if (a.dim < D) {        // (units past the head's: zeros)
+        for (int i = tid; i < 2 * kBuffer / 16; i += NTHR) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
+        __syncthreads();
+    }
+    if (t_begin < t_end) convert(0);
+    if (t_begin + 1 < t_end) fetch(t_begin + 1);
+    __syncthreads();
+
+    float16_tv acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (int32_t t = t_begin; t < t_end; ++t) {
+        const int buffer = (t - t_begin) & 1;
+        const int32_t k0 = t * kTile;
+        const int8_t* const kl = lds + buffer * kBuffer;
+        const int8_t* const vl = kl + kKeyBytes;
+        const bool active = k0 < any_sees;
+        half8_t p[2][2];
+        if (active) {
+            float16_tv s[2];
+#pragma unroll
+            for (int su = 0; su < 2; ++su) {
+                s[su] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < KS; ++u) {
+                    const half8_t k = *reinterpret_cast<const half8_t*>(kl + ((2 * u + half) * 64 + ((su * 32 + col) ^ (u & 7))) * 16);
+                    s[su] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[u], s[su], 0, 0, 0);
+                }
+            }
+            float factor[2], add[2], inverse[2];
+#pragma unroll
+            for (int su = 0; su < 2; ++su) {
+                const int32_t at = min(k0 + su * 32 + half * 16, a.length - 16) >> a.block_shift;
+                factor[su] = (float)key_top[at] * (1.0f / 127.0f) * scale;
+                const float vs = kv_scale(value_top[at]);
+                add[su] = __builtin_log2f(vs);
+                inverse[su] = 1.0f / vs;
+            }
+            // one bias for the whole tile where all its distances lie beyond the table's end
+            const int32_t rel_min = range.pos + q_first - (k0 + kTile - 1), rel_max = range.pos + last - k0;
+            const bool near = BIAS && rel_min < a.distances - 1 && rel_max > a.first_distance;
+            if (BIAS && !near) {
+                const float one = biases[(rel_min >= a.distances - 1 ? a.distances - 1 : a.first_distance) - lo_rel];
+                add[0] += one;
+                add[1] += one;
+            }
+            float m;
+            if (!MASK && !near && k0 + kTile <= all_see) {
+                m = -__builtin_inff();
+#pragma unroll
+                for (int su = 0; su < 2; ++su) {
+                    float g = s[su][0];
+#pragma unroll
+                    for (int j = 1; j < 16; ++j) g = fmaxf(g, s[su][j]);
+                    m = fmaxf(m, __builtin_fmaf(g, factor[su], add[su]));
+                }
+            } else {
+#pragma unroll
+                for (int su = 0; su < 2; ++su) {
+                    const int32_t mine = k0 + su * 32 + half * 16;
+                    const float* const bp = biases + (near ? where - mine - lo_rel : 15);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float bias = near ? add[su] + bp[-j] : add[su];
+                        s[su][j] = __builtin_fmaf(s[su][j], factor[su], bias);
+                        if (mine + j >= limit) s[su][j] = -__builtin_inff();
+                    }
+                    if (MASK) {
+                        struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
+                        const Byte16Any keep = *reinterpret_cast<const Byte16Any*>(mask + min(mine, a.length - 16));
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (!(keep.w[j >> 2] >> ((j & 3) * 8) & 0xffu)) s[su][j] = -__builtin_inff();
+                    }
+                    factor[su] = 1.0f;
+                    add[su] = 0.0f;
+                }
+                m = s[0][0];
+#pragma unroll
+                for (int su = 0; su < 2; ++su)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) m = fmaxf(m, s[su][j]);
+            }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            if (__builtin_amdgcn_ballot_w64(m > top + kLazy)) {
+                const float now = fmaxf(m, top), f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+                top = now;
+                sum *= f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n] *= f;
+            }
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+            for (int su = 0; su < 2; ++su) {
+                const float shift = add[su] - base;
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[su][j], factor[su], shift));
+                    part += e;
+                    p[su][j >> 3][j & 7] = (half_t)e;
+                }
+                sum = __builtin_fmaf(part, inverse[su], sum);
+            }
+        }
+        if (t + 1 < t_end) convert(buffer ^ 1);
+        if (t + 2 < t_end) fetch(t + 2);
+        if (active) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int su = 0; su < 2; ++su)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const half8_t v = *reinterpret_cast<const half8_t*>(vl + (((su * 2 + half) * 2 + e) * D + n * 32 + col) * 16);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[su][e], acc[n], 0, 0, 0);
+                    }
+        }
+        __syncthreads();
+    }
+    sum += __shfl_xor(sum, 32);
+    if (q_first + col >= a.tokens) return;
+    if (a.splits > 1) {
+        float* const part = a.parts + (tile_of * a.splits + split) * ROWS * (a.dim + 2);
+        const int r = wave * 32 + col;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int u = n * 32 + c * 8 + half * 4;
+                if (u < a.dim) *reinterpret_cast<float4_t*>(part + r * a.dim + u) = float4_t{acc[n][c * 4], acc[n][c * 4 + 1], acc[n][c * 4 + 2], acc[n][c * 4 + 3]};
+            }
+        if (half == 0) {
+            part[ROWS * a.dim + r] = top;
+            part[ROWS * a.dim + ROWS + r] = sum;
+        }
+        return;
+    }
+    half_t* const out = a.out + b * a.out_batch + (int64_t)h * a.out_head + (int64_t)query * a.out_token;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int u = n * 32 + c * 8 + half * 4;
+            if (u >= a.dim) continue;
+            half4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (half_t)(acc[n][c * 4 + e] * inv);
+            if (a.out_unit == 1) *reinterpret_cast<Half4Any*>(out + u) = __builtin_bit_cast(Half4Any, v);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[(u + e) * a.out_unit] = v[e];
+        }
+}
+
+template <int NT, int NW, bool BIAS, bool MASK>
+static int chunk_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
+    const int lds = 2 * 2 * 64 * NT * 32 * 2 + (BIAS ? (a.distances - a.first_distance + 2 * kChunkPad) * 4 : 0);
+    static std::atomic<bool> done[64];
+    if (int e = enable_dynamic_lds((const void*)k_kv_chunk<NT, NW, BIAS, MASK>, 160 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_kv_chunk<NT, NW, BIAS, MASK>), dim3(grid), dim3(NW * 64), lds, st, a);
+    return 0;
+}
+
+template <int NT, int NW>
+static int chunk_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
+    if (a.table) return a.mask ? chunk_launch<NT, NW, true, true>(a, grid, st) : chunk_launch<NT, NW, true, false>(a, grid, st);
+    return a.mask ? chunk_launch<NT, NW, false, true>(a, grid, st) : chunk_launch<NT, NW, false, false>(a, grid, st);
+}
+
+int kv_chunk_rows(int32_t tokens, int32_t dim) { return tokens > 128 && dim <= 128 ? 256 : 128; }
+
+int kv_chunk_launch(const KvAttention& a, int32_t batch, hipStream_t st) {
+    const int64_t grid = (int64_t)batch * a.heads * a.row_tiles * a.splits;
+    if (!grid_fits(grid)) return CPMK_ETOOBIG;
+    const unsigned g = (unsigned)grid;
+    if (kv_chunk_rows(a.tokens, a.dim) == 256) return a.dim <= 64 ? chunk_launch<2, 8>(a, g, st) : a.dim <= 96 ? chunk_launch<3, 8>(a, g, st) : chunk_launch<4, 8>(a, g, st);
+    return a.dim <= 64 ? chunk_launch<2, 4>(a, g, st) : a.dim <= 96 ? chunk_launch<3, 4>(a, g, st) : a.dim <= 128 ? chunk_launch<4, 4>(a, g, st) : chunk_launch<8, 4>(a, g, st);
+}
+
+}  // namespace cpmk
