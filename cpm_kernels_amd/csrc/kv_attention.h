@@ -75,6 +75,23 @@ __device__ __forceinline__ float kv_bias(const KvAttention& a, int32_t head, int
     return (float)a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))] * kLog2e;
 }
 
+// Eight units of a query from each of `first[]` on, zeros past the head's last one.  Every load is made, inside the row, so that none waits for another.
+template <int N, class First>
+__device__ __forceinline__ void load_query(half8_t (&q)[N], const half_t* p, int64_t stride, int dim, First first) {
+    if (stride == 1) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) q[s] = load_half8_any(p + min(first(s), dim - 8));
+    } else {
+#pragma unroll
+        for (int s = 0; s < N; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = p[(min(first(s), dim - 8) + e) * stride];
+    }
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+        if (first(s) >= dim) q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+}
+
 // Many queries (kv_chunk.hip).  How many rows a part of one query tile has, and the launch (0 or an error code).
 int kv_chunk_rows(int32_t tokens, int32_t dim);
 int kv_chunk_launch(const KvAttention& a, int32_t batch, hipStream_t st);

@@ -42,20 +42,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_kv_attend(KvAttention a) {
     const int32_t limit = a.causal ? min(range.len, where + 1) : range.len;
 
     half8_t q[2 * DS];
-    {
-        const half_t* p = a.q + b * a.q_batch + (int64_t)(kvh * a.group + g) * a.q_head + (int64_t)query * a.q_token;
-#pragma unroll
-        for (int s = 0; s < 2 * DS; ++s) {
-            const int u = (s >> 1) * 64 + quad * 16 + (s & 1) * 8;
-            q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-            if (u < a.dim) {
-                if (a.q_unit == 1) q[s] = load_half8_any(p + u);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[s][e] = p[(u + e) * a.q_unit];
-            }
-        }
-    }
+    load_query(q, a.q + b * a.q_batch + (int64_t)(kvh * a.group + g) * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim,
+               [&](int s) { return (s >> 1) * 64 + quad * 16 + (s & 1) * 8; });
     const int entries = a.distances - a.first_distance;
     if (BIAS) {
         // the bias of every distance from first_distance on, for each head of the tile

@@ -6,6 +6,10 @@
 // straight into the second product.  The running maximum follows the true one at a distance of up to 2^8: fp16 keeps the probabilities' bits either way, and the sums are rescaled
 // in the first tiles only.
 //
+// A wave does a tile in two phases with a barrier behind each: products (the values of the tile before, the scores of this one), then everything else (softmax, conversion, loads).
+// Of eight waves the second four are one phase behind the first four, so that each SIMD has one wave in either: with all in the same phase the matrix pipe
+// idled through the softmax.
+//
 // LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at (2 u + h) 64 + (r ^ (u & 7)), read along r; the exclusive or spreads the eight unit steps that
 // neighbouring lanes write over the banks.  Values (group of sixteen keys g, half s, unit) at (2 g + s) D + unit.
 #include "kv_attention.h"
@@ -14,12 +18,26 @@ namespace cpmk {
 
 constexpr int kLazy = 8;
 
+// N products whose operands come from LDS one each: so many reads ahead that a read's latency lies behind products (the compiler keeps two ahead).
+template <int N>
+__device__ __forceinline__ void products_in_step() {
+    constexpr int kAhead = 6;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
+}
+
 // NT: 32-unit steps of a head, NW: waves
 template <int NT, int NW, bool BIAS, bool MASK>
 __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     constexpr int D = NT * 32, KS = NT * 2, NTHR = NW * 64, PIECES = (8 * D + NTHR - 1) / NTHR, ROWS = NW * 32;
     constexpr int kKeyBytes = 64 * D * 2, kBuffer = 2 * kKeyBytes;
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+    __shared__ float4_t facts[2][4];            // of a tile's four groups of keys: factor of the scores, log2 and inverse of the values' scale
     float* const biases = reinterpret_cast<float*>(lds + 2 * kBuffer);
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -45,21 +63,10 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     const float scale = flip ? -a.scale : a.scale;
 
     half8_t q[KS];
-    {
-        const half_t* p = a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token;
+    load_query(q, a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim, [&](int s) { return s * 16 + half * 8; });
+    if (flip)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int u = s * 16 + half * 8;
-            q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-            if (u < a.dim) {
-                if (a.q_unit == 1) q[s] = load_half8_any(p + u);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[s][e] = p[(u + e) * a.q_unit];
-            }
-            if (flip) q[s] = -q[s];
-        }
-    }
+        for (int s = 0; s < KS; ++s) q[s] = -q[s];
     const int32_t lo_rel = a.first_distance - kChunkPad;
     if (BIAS)
         for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
@@ -71,88 +78,119 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     const half_t* const value_top = a.value_top + (head * a.length >> a.block_shift);
     const uint8_t* const mask = MASK ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
 
-    // the pieces of a tile that this thread brings: keys first, a token's units side by side, then values as they lie
+    // the pieces of a tile that this thread brings: keys first, a token's units side by side, then values as they lie (a wave has one kind)
     const int runs = a.dim >> 4;
-    int32_t at_lds[PIECES], row[PIECES], offset[PIECES];
+    uint32_t at_lds[PIECES], offset[PIECES], last_offset[PIECES];
     bool is_key[PIECES], real[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int p = tid + i * NTHR;
-        real[i] = p < 8 * a.dim;
-        is_key[i] = p < 4 * a.dim;
+        real[i] = wave * 64 + i * NTHR < 8 * a.dim;
+        is_key[i] = wave * 64 + i * NTHR < 4 * a.dim;
         if (is_key[i]) {
             const int key = p / runs, u = p - key * runs;
             const int r = (key & 32) | ((key >> 2) & 3) << 3 | ((key >> 4) & 1) << 2 | (key & 3);
-            row[i] = key;
-            offset[i] = u * 16;
+            offset[i] = key * a.dim + u * 16;
+            last_offset[i] = (a.length - 1) * a.dim + u * 16;
             at_lds[i] = (u * 128 + (r ^ (u & 7))) * 16;
         } else {
-            const int v = p - 4 * a.dim, g = min(v / a.dim, 3), unit = v - g * a.dim;
-            row[i] = g * 16;
-            offset[i] = unit * 16;
+            const int v = p - 4 * a.dim, g = min(v / a.dim, 3), unit = min(v - g * a.dim, a.dim - 1);
+            offset[i] = g * 16 * a.dim + unit * 16;
+            last_offset[i] = (a.length - 16) * a.dim + unit * 16;
             at_lds[i] = kKeyBytes + (g * 2 * D + unit) * 16;
         }
     }
+    const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
     uint4_t raw[PIECES];
-    auto fetch = [&](int32_t tile) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int32_t k = min(tile * kTile + row[i], is_key[i] ? a.length - 1 : a.length - 16);
-            if (real[i]) raw[i] = *reinterpret_cast<const uint4_t*>((is_key[i] ? keys : values) + k * a.dim + offset[i]);
-        }
-    };
-    auto convert = [&](int buffer) {
+    half_t key_raw = 0, value_raw = 0;
+    // Keys of tile t + 1 and values of tile t, and the magnitudes that go with tile t + 1.  (Tiles past the end: the last keys again, into buffers that nobody reads.)
+    auto fetch = [&](int32_t t) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
-            if (real[i]) {
+            if (PIECES * NTHR == 8 * D || real[i]) {
+                const uint32_t o = min(offset[i] + (uint32_t)max(t + is_key[i], 0) * (uint32_t)(kTile * a.dim), last_offset[i]);
+                raw[i] = *reinterpret_cast<const uint4_t*>((is_key[i] ? keys : values) + o);
+            }
+        if (wave == 0) {
+            const uint32_t at = (uint32_t)min((t + 1) * kTile + (lane & 3) * 16, a.length - 16) >> a.block_shift;
+            key_raw = key_top[at];
+            value_raw = value_top[at];
+        }
+    };
+    auto convert = [&](int32_t t) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            if (PIECES * NTHR == 8 * D || real[i]) {
                 half8_t lo, hi;
                 halves_of(raw[i], lo, hi);
-                int8_t* const p = lds + buffer * kBuffer + at_lds[i];
+                int8_t* const p = lds + ((t + is_key[i] - t_begin) & 1) * kBuffer + at_lds[i];
                 *reinterpret_cast<half8_t*>(p) = lo;
                 *reinterpret_cast<half8_t*>(p + (is_key[i] ? 64 : D) * 16) = hi;
             }
+        if (wave == 0) {
+            const float vs = kv_scale(value_raw);
+            facts[(t + 1 - t_begin) & 1][lane & 3] = float4_t{(float)key_raw * (1.0f / 127.0f) * scale, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
+        }
     };
-    const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
-    if (t_begin < t_end) fetch(t_begin);
-    if (a.dim < D) {        // (units past the head's: zeros)
-        for (int i = tid; i < 2 * kBuffer / 16; i += NTHR) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
+    const int late = NW == 8 ? wave >> 2 : 0;
+    if (t_begin < t_end) {
+        fetch(t_begin - 1);
+        if (a.dim < D) {        // (units past the head's: zeros)
+            for (int i = tid; i < 2 * kBuffer / 16; i += NTHR) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
+            __syncthreads();
+        }
+        convert(t_begin - 1);
+        fetch(t_begin);
         __syncthreads();
+        if (late) {
+            convert(t_begin);
+            fetch(t_begin + 1);
+            __syncthreads();
+        }
     }
-    if (t_begin < t_end) convert(0);
-    if (t_begin + 1 < t_end) fetch(t_begin + 1);
-    __syncthreads();
 
-    float16_tv acc[NT];
+    float16_tv acc[NT], s[2];
+    float4_t fact[2];
+    half8_t p[2][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     float top = -__builtin_inff(), sum = 0.0f;
-    for (int32_t t = t_begin; t < t_end; ++t) {
-        const int buffer = (t - t_begin) & 1;
-        const int32_t k0 = t * kTile;
-        const int8_t* const kl = lds + buffer * kBuffer;
-        const int8_t* const vl = kl + kKeyBytes;
-        const bool active = k0 < any_sees;
-        half8_t p[2][2];
-        if (active) {
-            float16_tv s[2];
+    auto values_of = [&](int32_t t) {       // the values of tile t by their probabilities
+        const int8_t* const vl = lds + ((t - t_begin) & 1) * kBuffer + kKeyBytes;
 #pragma unroll
-            for (int su = 0; su < 2; ++su) {
-                s[su] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        for (int su = 0; su < 2; ++su)
 #pragma unroll
-                for (int u = 0; u < KS; ++u) {
-                    const half8_t k = *reinterpret_cast<const half8_t*>(kl + ((2 * u + half) * 64 + ((su * 32 + col) ^ (u & 7))) * 16);
-                    s[su] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[u], s[su], 0, 0, 0);
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const half8_t v = *reinterpret_cast<const half8_t*>(vl + (((su * 2 + half) * 2 + e) * D + n * 32 + col) * 16);
+                    acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[su][e], acc[n], 0, 0, 0);
                 }
-            }
-            float factor[2], add[2], inverse[2];
+    };
+    auto scores_of = [&](int32_t t) {
+        const int8_t* const kl = lds + ((t - t_begin) & 1) * kBuffer;
+#pragma unroll
+        for (int su = 0; su < 2; ++su) {
+            fact[su] = facts[(t - t_begin) & 1][su * 2 + half];
+            s[su] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < KS; ++u)
 #pragma unroll
             for (int su = 0; su < 2; ++su) {
-                const int32_t at = min(k0 + su * 32 + half * 16, a.length - 16) >> a.block_shift;
-                factor[su] = (float)key_top[at] * (1.0f / 127.0f) * scale;
-                const float vs = kv_scale(value_top[at]);
-                add[su] = __builtin_log2f(vs);
-                inverse[su] = 1.0f / vs;
+                const half8_t k = *reinterpret_cast<const half8_t*>(kl + ((2 * u + half) * 64 + ((su * 32 + col) ^ (u & 7))) * 16);
+                s[su] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[u], s[su], 0, 0, 0);
             }
+    };
+    if (t_begin < t_end) {
+        if (t_begin * kTile < any_sees) scores_of(t_begin);
+        __syncthreads();
+    }
+    for (int32_t t = t_begin; t < t_end; ++t) {
+        const int32_t k0 = t * kTile;
+        const bool active = k0 < any_sees;
+        if (active) {
+            float factor[2] = {fact[0][0], fact[1][0]}, add[2] = {fact[0][1], fact[1][1]};
             // one bias for the whole tile where all its distances lie beyond the table's end
             const int32_t rel_min = range.pos + q_first - (k0 + kTile - 1), rel_max = range.pos + last - k0;
             const bool near = BIAS && rel_min < a.distances - 1 && rel_max > a.first_distance;
@@ -163,31 +201,35 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
             }
             float m;
             if (!MASK && !near && k0 + kTile <= all_see) {
-                m = -__builtin_inff();
+                float g[2];
 #pragma unroll
                 for (int su = 0; su < 2; ++su) {
-                    float g = s[su][0];
+                    g[su] = s[su][0];
 #pragma unroll
-                    for (int j = 1; j < 16; ++j) g = fmaxf(g, s[su][j]);
-                    m = fmaxf(m, __builtin_fmaf(g, factor[su], add[su]));
+                    for (int j = 1; j < 16; ++j) g[su] = fmaxf(g[su], s[su][j]);
                 }
+                m = fmaxf(__builtin_fmaf(g[0], factor[0], add[0]), __builtin_fmaf(g[1], factor[1], add[1]));
             } else {
 #pragma unroll
                 for (int su = 0; su < 2; ++su) {
                     const int32_t mine = k0 + su * 32 + half * 16;
-                    const float* const bp = biases + (near ? where - mine - lo_rel : 15);
+                    if (BIAS && near) {
+                        const float* const bp = biases + (where - mine - 15 - lo_rel);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float bias = near ? add[su] + bp[-j] : add[su];
-                        s[su][j] = __builtin_fmaf(s[su][j], factor[su], bias);
-                        if (mine + j >= limit) s[su][j] = -__builtin_inff();
+                        for (int j = 0; j < 16; ++j) s[su][j] = __builtin_fmaf(s[su][j], factor[su], add[su] + bp[15 - j]);
+                    } else
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[su][j] = __builtin_fmaf(s[su][j], factor[su], add[su]);
+                    if (k0 + kTile > all_see) {
+                        const int32_t left = limit - mine;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[su][j] = j < left ? s[su][j] : -__builtin_inff();
                     }
                     if (MASK) {
                         struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
                         const Byte16Any keep = *reinterpret_cast<const Byte16Any*>(mask + min(mine, a.length - 16));
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (!(keep.w[j >> 2] >> ((j & 3) * 8) & 0xffu)) s[su][j] = -__builtin_inff();
+                        for (int j = 0; j < 16; ++j) s[su][j] = (keep.w[j >> 2] >> ((j & 3) * 8) & 0xffu) ? s[su][j] : -__builtin_inff();
                     }
                     factor[su] = 1.0f;
                     add[su] = 0.0f;
@@ -198,7 +240,11 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) m = fmaxf(m, s[su][j]);
             }
-            m = fmaxf(m, __shfl_xor(m, 32));
+            {
+                const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+                const uint32_t low = both[0], high = both[1];       // (a bit cast of a vector's element itself takes the first one's)
+                m = fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+            }
             if (__builtin_amdgcn_ballot_w64(m > top + kLazy)) {
                 const float now = fmaxf(m, top), f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
                 top = now;
@@ -210,31 +256,27 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
 #pragma unroll
             for (int su = 0; su < 2; ++su) {
                 const float shift = add[su] - base;
-                float part = 0.0f;
+                float part = 0.0f;         // (of the unrounded ones: beside much larger values the rounded ones may have no bits left, and still be most of the sum)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[su][j], factor[su], shift));
                     part += e;
                     p[su][j >> 3][j & 7] = (half_t)e;
                 }
-                sum = __builtin_fmaf(part, inverse[su], sum);
+                sum = __builtin_fmaf(part, fact[su][2], sum);
             }
         }
-        if (t + 1 < t_end) convert(buffer ^ 1);
-        if (t + 2 < t_end) fetch(t + 2);
-        if (active) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int su = 0; su < 2; ++su)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const half8_t v = *reinterpret_cast<const half8_t*>(vl + (((su * 2 + half) * 2 + e) * D + n * 32 + col) * 16);
-                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[su][e], acc[n], 0, 0, 0);
-                    }
+        convert(t + late);
+        fetch(t + 1 + late);
+        __syncthreads();
+        if (active) {           // (behind the last tile: scores that nobody looks at)
+            values_of(t);
+            scores_of(t + 1);
+            products_in_step<4 * NT + 2 * KS>();
         }
         __syncthreads();
     }
+    if (!late && NW == 8 && t_begin < t_end) __syncthreads();
     sum += __shfl_xor(sum, 32);
     if (q_first + col >= a.tokens) return;
     if (a.splits > 1) {
@@ -275,7 +317,7 @@ template <int NT, int NW, bool BIAS, bool MASK>
 static int chunk_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
     const int lds = 2 * 2 * 64 * NT * 32 * 2 + (BIAS ? (a.distances - a.first_distance + 2 * kChunkPad) * 4 : 0);
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_kv_chunk<NT, NW, BIAS, MASK>, 160 * 1024, done)) return e;
+    if (int e = enable_dynamic_lds((const void*)k_kv_chunk<NT, NW, BIAS, MASK>, 160 * 1024 - 256, done)) return e;
     hipLaunchKernelGGL((k_kv_chunk<NT, NW, BIAS, MASK>), dim3(grid), dim3(NW * 64), lds, st, a);
     return 0;
 }
