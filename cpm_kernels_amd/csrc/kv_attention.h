@@ -27,6 +27,7 @@ struct KvAttention {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTile = 64;           // keys a wave takes at a time
 constexpr int32_t kFar = 1 << 30;   // positions and rows stay below
+constexpr int kChunkRows = 128;     // queries of a workgroup (kv_chunk.hip)
 constexpr int kChunkLeast = 4;       // tiles of a part, at least (kv_chunk.hip)
 constexpr int kChunkPad = 96;        // distances beyond the table's ends that a tile of 32 queries and 64 keys can reach into
 
@@ -92,8 +93,7 @@ __device__ __forceinline__ void load_query(half8_t (&q)[N], const half_t* p, int
         if (first(s) >= dim) q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
 }
 
-// Many queries (kv_chunk.hip).  How many rows a part of one query tile has, and the launch (0 or an error code).
-int kv_chunk_rows(int32_t tokens, int32_t dim);
+// Many queries (kv_chunk.hip): 0 or an error code.
 int kv_chunk_launch(const KvAttention& a, int32_t batch, hipStream_t st);
 
 }  // namespace cpmk

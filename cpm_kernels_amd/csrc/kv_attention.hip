@@ -221,7 +221,7 @@ struct KvPlan {
 static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length) {
     KvPlan p;
     p.chunks = tokens > 32;
-    p.rows = p.chunks ? kv_chunk_rows((int32_t)tokens, dim) : 16;
+    p.rows = p.chunks ? kChunkRows : 16;
     p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
     const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, most = ceil_div(length, kTile * (p.chunks ? kChunkLeast : kWaves));
     const int64_t want = ceil_div((p.chunks ? 1 : 4) * (int64_t)compute_units(), base);

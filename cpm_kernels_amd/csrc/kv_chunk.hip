@@ -6,17 +6,18 @@
 // straight into the second product.  The running maximum follows the true one at a distance of up to 2^8: fp16 keeps the probabilities' bits either way, and the sums are rescaled
 // in the first tiles only.
 //
-// A wave does a tile in two phases with a barrier behind each: products (the values of the tile before, the scores of this one), then everything else (softmax, conversion, loads).
-// Of eight waves the second four are one phase behind the first four, so that each SIMD has one wave in either: with all in the same phase the matrix pipe
-// idled through the softmax.
+// A workgroup of four waves meets at one barrier a tile, between the softmax (with the conversion and the loads) and the products (values of this tile, scores of the next); what fills the
+// matrix pipe meanwhile are the other workgroups of the compute unit, three of them for heads of up to 64 units, two up to 128.  One workgroup of eight waves, half of them a
+// phase behind the others, was 20 % slower with 64 units (8 x 64 heads of 512 queries over 1024 keys: 138 against 114 us) and between 3 % slower and 6 % faster with 128.
 //
-// LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at (2 u + h) 64 + (r ^ (u & 7)), read along r; the exclusive or spreads the eight unit steps that
+// LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at 129 u + 64 h + r, read along r; the odd distance spreads the eight unit steps that
 // neighbouring lanes write over the banks.  Values (group of sixteen keys g, half s, unit) at (2 g + s) D + unit.
 #include "kv_attention.h"
 
 namespace cpmk {
 
 constexpr int kLazy = 8;
+constexpr int kChunkWaves = kChunkRows / 32;
 
 // N products whose operands come from LDS one each: so many reads ahead that a read's latency lies behind products (the compiler keeps two ahead).
 template <int N>
@@ -31,13 +32,13 @@ __device__ __forceinline__ void products_in_step() {
     __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
 }
 
-// NT: 32-unit steps of a head, NW: waves
-template <int NT, int NW, bool BIAS, bool MASK>
-__global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
-    constexpr int D = NT * 32, KS = NT * 2, NTHR = NW * 64, PIECES = (8 * D + NTHR - 1) / NTHR, ROWS = NW * 32;
-    constexpr int kKeyBytes = 64 * D * 2, kBuffer = 2 * kKeyBytes;
+// NT: 32-unit steps of a head
+template <int NT, bool BIAS, bool MASK>
+__global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_kv_chunk(KvAttention a) {
+    constexpr int D = NT * 32, KS = NT * 2, NTHR = kChunkWaves * 64, PIECES = (8 * D + NTHR - 1) / NTHR, ROWS = kChunkRows;
+    constexpr int kKeyBytes = KS * 129 * 16, kBuffer = kKeyBytes + 64 * D * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];
-    __shared__ float4_t facts[2][4];            // of a tile's four groups of keys: factor of the scores, log2 and inverse of the values' scale
+    __shared__ float4_t facts[16][4];           // of the groups of keys of sixteen tiles, in a ring: factor of the scores, log2 and inverse of the values' scale
     float* const biases = reinterpret_cast<float*>(lds + 2 * kBuffer);
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -62,15 +63,6 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     const bool flip = a.scale < 0.0f;           // (so that the largest score is the largest product)
     const float scale = flip ? -a.scale : a.scale;
 
-    half8_t q[KS];
-    load_query(q, a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim, [&](int s) { return s * 16 + half * 8; });
-    if (flip)
-#pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = -q[s];
-    const int32_t lo_rel = a.first_distance - kChunkPad;
-    if (BIAS)
-        for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
-
     const int64_t head = b * a.held + h / a.group;
     const int8_t* const keys = a.keys + head * a.length * a.dim;
     const int8_t* const values = a.values + head * a.length * a.dim;
@@ -92,7 +84,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
             const int r = (key & 32) | ((key >> 2) & 3) << 3 | ((key >> 4) & 1) << 2 | (key & 3);
             offset[i] = key * a.dim + u * 16;
             last_offset[i] = (a.length - 1) * a.dim + u * 16;
-            at_lds[i] = (u * 128 + (r ^ (u & 7))) * 16;
+            at_lds[i] = (u * 129 + r) * 16;
         } else {
             const int v = p - 4 * a.dim, g = min(v / a.dim, 3), unit = min(v - g * a.dim, a.dim - 1);
             offset[i] = g * 16 * a.dim + unit * 16;
@@ -103,7 +95,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
     uint4_t raw[PIECES];
     half_t key_raw = 0, value_raw = 0;
-    // Keys of tile t + 1 and values of tile t, and the magnitudes that go with tile t + 1.  (Tiles past the end: the last keys again, into buffers that nobody reads.)
+    // Keys of tile t + 1 and values of tile t.  (Tiles past the end: the last keys again, into buffers that nobody reads.)
     auto fetch = [&](int32_t t) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
@@ -111,11 +103,15 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
                 const uint32_t o = min(offset[i] + (uint32_t)max(t + is_key[i], 0) * (uint32_t)(kTile * a.dim), last_offset[i]);
                 raw[i] = *reinterpret_cast<const uint4_t*>((is_key[i] ? keys : values) + o);
             }
-        if (wave == 0) {
-            const uint32_t at = (uint32_t)min((t + 1) * kTile + (lane & 3) * 16, a.length - 16) >> a.block_shift;
-            key_raw = key_top[at];
-            value_raw = value_top[at];
-        }
+    };
+    auto fetch_tops = [&](int32_t t) {      // a lane a group of keys from tile t on
+        const uint32_t at = (uint32_t)min(t * (int64_t)kTile + lane * 16, (int64_t)a.length - 16) >> a.block_shift;
+        key_raw = key_top[at];
+        value_raw = value_top[at];
+    };
+    auto convert_tops = [&](int32_t t) {
+        const float vs = kv_scale(value_raw);
+        facts[(t - t_begin + (lane >> 2)) & 15][lane & 3] = float4_t{(float)key_raw * (1.0f / 127.0f) * scale, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
     };
     auto convert = [&](int32_t t) {
 #pragma unroll
@@ -127,26 +123,29 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
                 *reinterpret_cast<half8_t*>(p) = lo;
                 *reinterpret_cast<half8_t*>(p + (is_key[i] ? 64 : D) * 16) = hi;
             }
-        if (wave == 0) {
-            const float vs = kv_scale(value_raw);
-            facts[(t + 1 - t_begin) & 1][lane & 3] = float4_t{(float)key_raw * (1.0f / 127.0f) * scale, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
-        }
     };
-    const int late = NW == 8 ? wave >> 2 : 0;
     if (t_begin < t_end) {
         fetch(t_begin - 1);
+        if (wave == 0) fetch_tops(t_begin);
+    }
+    half8_t q[KS];
+    load_query(q, a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim, [&](int s) { return s * 16 + half * 8; });
+    if (flip)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = -q[s];
+    const int32_t lo_rel = a.first_distance - kChunkPad;
+    if (BIAS)
+        for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
+
+    if (t_begin < t_end) {
         if (a.dim < D) {        // (units past the head's: zeros)
             for (int i = tid; i < 2 * kBuffer / 16; i += NTHR) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
             __syncthreads();
         }
         convert(t_begin - 1);
         fetch(t_begin);
+        if (wave == 0) convert_tops(t_begin);
         __syncthreads();
-        if (late) {
-            convert(t_begin);
-            fetch(t_begin + 1);
-            __syncthreads();
-        }
     }
 
     float16_tv acc[NT], s[2];
@@ -156,36 +155,33 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
     for (int n = 0; n < NT; ++n) acc[n] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     float top = -__builtin_inff(), sum = 0.0f;
     auto values_of = [&](int32_t t) {       // the values of tile t by their probabilities
-        const int8_t* const vl = lds + ((t - t_begin) & 1) * kBuffer + kKeyBytes;
+        const int8_t* const vl = lds + ((t - t_begin) & 1) * kBuffer + kKeyBytes + (half * 2 * D + col) * 16;
 #pragma unroll
         for (int su = 0; su < 2; ++su)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const half8_t v = *reinterpret_cast<const half8_t*>(vl + (((su * 2 + half) * 2 + e) * D + n * 32 + col) * 16);
+                    const half8_t v = *reinterpret_cast<const half8_t*>(vl + ((su * 4 + e) * D + n * 32) * 16);
                     acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[su][e], acc[n], 0, 0, 0);
                 }
     };
     auto scores_of = [&](int32_t t) {
-        const int8_t* const kl = lds + ((t - t_begin) & 1) * kBuffer;
+        const int8_t* const kl = lds + ((t - t_begin) & 1) * kBuffer + (half * 64 + col) * 16;
 #pragma unroll
         for (int su = 0; su < 2; ++su) {
-            fact[su] = facts[(t - t_begin) & 1][su * 2 + half];
+            fact[su] = facts[(t - t_begin) & 15][su * 2 + half];
             s[su] = float16_tv{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         }
 #pragma unroll
         for (int u = 0; u < KS; ++u)
 #pragma unroll
             for (int su = 0; su < 2; ++su) {
-                const half8_t k = *reinterpret_cast<const half8_t*>(kl + ((2 * u + half) * 64 + ((su * 32 + col) ^ (u & 7))) * 16);
+                const half8_t k = *reinterpret_cast<const half8_t*>(kl + (u * 129 + su * 32) * 16);
                 s[su] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[u], s[su], 0, 0, 0);
             }
     };
-    if (t_begin < t_end) {
-        if (t_begin * kTile < any_sees) scores_of(t_begin);
-        __syncthreads();
-    }
+    if (t_begin < t_end && t_begin * kTile < any_sees) scores_of(t_begin);
     for (int32_t t = t_begin; t < t_end; ++t) {
         const int32_t k0 = t * kTile;
         const bool active = k0 < any_sees;
@@ -266,17 +262,19 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
                 sum = __builtin_fmaf(part, fact[su][2], sum);
             }
         }
-        convert(t + late);
-        fetch(t + 1 + late);
+        convert(t);
+        fetch(t + 1);
+        if (wave == 0 && t - t_begin >= 8) {        // eight tiles' magnitudes at a time, into the half of the ring that has been read
+            if (((t - t_begin) & 7) == 0 && lane < 32) fetch_tops(t + 8);
+            if (((t - t_begin) & 7) == 1 && lane < 32) convert_tops(t + 7);
+        }
         __syncthreads();
         if (active) {           // (behind the last tile: scores that nobody looks at)
             values_of(t);
             scores_of(t + 1);
             products_in_step<4 * NT + 2 * KS>();
         }
-        __syncthreads();
     }
-    if (!late && NW == 8 && t_begin < t_end) __syncthreads();
     sum += __shfl_xor(sum, 32);
     if (q_first + col >= a.tokens) return;
     if (a.splits > 1) {
@@ -313,29 +311,26 @@ __global__ __launch_bounds__(NW * 64) void k_kv_chunk(KvAttention a) {
         }
 }
 
-template <int NT, int NW, bool BIAS, bool MASK>
+template <int NT, bool BIAS, bool MASK>
 static int chunk_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
-    const int lds = 2 * 2 * 64 * NT * 32 * 2 + (BIAS ? (a.distances - a.first_distance + 2 * kChunkPad) * 4 : 0);
+    const int lds = 2 * (NT * 2 * 129 * 16 + 64 * NT * 32 * 2) + (BIAS ? (a.distances - a.first_distance + 2 * kChunkPad) * 4 : 0);
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_kv_chunk<NT, NW, BIAS, MASK>, 160 * 1024 - 256, done)) return e;
-    hipLaunchKernelGGL((k_kv_chunk<NT, NW, BIAS, MASK>), dim3(grid), dim3(NW * 64), lds, st, a);
+    if (int e = enable_dynamic_lds((const void*)k_kv_chunk<NT, BIAS, MASK>, 158 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_kv_chunk<NT, BIAS, MASK>), dim3(grid), dim3(kChunkWaves * 64), lds, st, a);
     return 0;
 }
 
-template <int NT, int NW>
+template <int NT>
 static int chunk_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
-    if (a.table) return a.mask ? chunk_launch<NT, NW, true, true>(a, grid, st) : chunk_launch<NT, NW, true, false>(a, grid, st);
-    return a.mask ? chunk_launch<NT, NW, false, true>(a, grid, st) : chunk_launch<NT, NW, false, false>(a, grid, st);
+    if (a.table) return a.mask ? chunk_launch<NT, true, true>(a, grid, st) : chunk_launch<NT, true, false>(a, grid, st);
+    return a.mask ? chunk_launch<NT, false, true>(a, grid, st) : chunk_launch<NT, false, false>(a, grid, st);
 }
-
-int kv_chunk_rows(int32_t tokens, int32_t dim) { return tokens > 128 && dim <= 128 ? 256 : 128; }
 
 int kv_chunk_launch(const KvAttention& a, int32_t batch, hipStream_t st) {
     const int64_t grid = (int64_t)batch * a.heads * a.row_tiles * a.splits;
     if (!grid_fits(grid)) return CPMK_ETOOBIG;
     const unsigned g = (unsigned)grid;
-    if (kv_chunk_rows(a.tokens, a.dim) == 256) return a.dim <= 64 ? chunk_launch<2, 8>(a, g, st) : a.dim <= 96 ? chunk_launch<3, 8>(a, g, st) : chunk_launch<4, 8>(a, g, st);
-    return a.dim <= 64 ? chunk_launch<2, 4>(a, g, st) : a.dim <= 96 ? chunk_launch<3, 4>(a, g, st) : a.dim <= 128 ? chunk_launch<4, 4>(a, g, st) : chunk_launch<8, 4>(a, g, st);
+    return a.dim <= 64 ? chunk_launch<2>(a, g, st) : a.dim <= 96 ? chunk_launch<3>(a, g, st) : a.dim <= 128 ? chunk_launch<4>(a, g, st) : chunk_launch<8>(a, g, st);
 }
 
 }  // namespace cpmk
