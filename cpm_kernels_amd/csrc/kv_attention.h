@@ -27,6 +27,7 @@ struct KvAttention {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTile = 64;           // keys a wave takes at a time
 constexpr int32_t kFar = 1 << 30;   // positions and rows stay below
+constexpr int kLazy = 8;             // log2 of how far the running maximum may lie below the true one
 constexpr int kChunkRows = 128;     // queries of a workgroup (kv_chunk.hip)
 constexpr int kChunkLeast = 4;       // tiles of a part, at least (kv_chunk.hip)
 constexpr int kChunkPad = 96;        // distances beyond the table's ends that a tile of 32 queries and 64 keys can reach into
@@ -74,6 +75,21 @@ __device__ __forceinline__ float kv_bias(const KvAttention& a, int32_t head, int
     rel = max(a.first_distance, min(rel, a.distances - 1));
     const int32_t bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
     return (float)a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))] * kLog2e;
+}
+
+// Workgroup x of units * inner ones: the `inner` workgroups of a unit, which read the same keys, follow one another on one XCD, and units are dealt to the XCDs in turn (of sequences of
+// unequal length no XCD gets the long ones).
+__device__ __forceinline__ void kv_deal(uint32_t x, uint32_t units, uint32_t inner, uint32_t& unit, uint32_t& in) {
+    const uint32_t whole = units & ~7u;
+    if (x < whole * inner) {
+        const uint32_t y = x >> 3, u = y / inner;
+        unit = u * 8 + (x & 7);
+        in = y - u * inner;
+    } else {
+        x -= whole * inner;
+        in = x / (units - whole);
+        unit = whole + (x - in * (units - whole));
+    }
 }
 
 // Eight units of a query from each of `first[]` on, zeros past the head's last one.  Every load is made, inside the row, so that none waits for another.

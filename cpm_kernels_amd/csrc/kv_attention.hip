@@ -17,166 +17,250 @@ namespace cpmk {
 
 constexpr int kWaves = 4;
 
-// DS: 64-unit steps of a head.
-template <int DS, int WAVES, bool BIAS, bool MASK>
-__global__ __launch_bounds__(WAVES * 64) void k_kv_attend(KvAttention a) {
-    __shared__ float joined[WAVES][16][64 + 4];
-    __shared__ float stat[WAVES][2][16];
+// The largest of a value over the four sixteens of lanes (no trip through the LDS crossbar).
+__device__ __forceinline__ float quad_max(float m) {
+    // (a bit cast of a vector's element itself takes the first one's)
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    m = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// DS: 64-unit steps of a head, CT: sixteens of rows.
+template <int DS, int CT, bool BIAS, bool MASK>
+__global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAttention a) {
+    constexpr int ROWS = CT * 16;
+    __shared__ float joined[kWaves][ROWS][64 + 4];
+    __shared__ float stat[kWaves][2][ROWS];
     extern __shared__ half_t table[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint32_t w = blockIdx.x;
+    uint32_t w, rt_of;
+    kv_deal(blockIdx.x, gridDim.x / (uint32_t)a.row_tiles, a.row_tiles, w, rt_of);
+    const int32_t rt = rt_of;
     const int32_t split = w % (uint32_t)a.splits;
     w /= (uint32_t)a.splits;
-    const int32_t rt = w % (uint32_t)a.row_tiles;
-    w /= (uint32_t)a.row_tiles;
     const int32_t kvh = w % (uint32_t)a.held;
     const int64_t b = w / (uint32_t)a.held;
-    const int64_t tile_of = blockIdx.x / (uint32_t)a.splits;
-    const int32_t rows = a.tokens * a.group;
-    const int32_t row = min(rt * 16 + col, rows - 1);       // (rows past the end repeat the last one)
-    const int32_t query = row / a.group, g = row - query * a.group;
-    const KvRange range = kv_range(a, b, min(rt * 16 + 15, rows - 1) / a.group, WAVES);
+    const int32_t rows = a.tokens * a.group, r_first = rt * ROWS, r_last = min(r_first + ROWS, rows) - 1;
+    const KvRange range = kv_range(a, b, r_last / a.group, kWaves);
     if (split >= range.parts) return;
-    const int32_t where = range.pos + query;                // position of the query
-    const int32_t limit = a.causal ? min(range.len, where + 1) : range.len;
-
-    half8_t q[2 * DS];
-    load_query(q, a.q + b * a.q_batch + (int64_t)(kvh * a.group + g) * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim,
-               [&](int s) { return (s >> 1) * 64 + quad * 16 + (s & 1) * 8; });
-    const int entries = a.distances - a.first_distance;
-    if (BIAS) {
-        // the bias of every distance from first_distance on, for each head of the tile
-        const int slots = min(a.group, 16);
-        for (int i = tid; i < slots * entries; i += WAVES * 64) {
-            const int slot = i / entries, rel = i - slot * entries + a.first_distance;
-            const int head = kvh * a.group + (a.group <= 16 ? slot : (rt * 16 + slot) % a.group);
-            const int bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
-            table[i] = a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))];
-        }
-        __syncthreads();
-    }
-    const half_t* const biases = table + (a.group <= 16 ? g : col) * entries;
+    const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
 
     const int64_t head = b * a.held + kvh;
     const int8_t* const keys = a.keys + head * a.length * a.dim;
     const int8_t* const values = a.values + head * a.length * a.dim;
     const half_t* const key_top = a.key_top + (head * a.length >> a.block_shift);
     const half_t* const value_top = a.value_top + (head * a.length >> a.block_shift);
-    const uint8_t* const mask = MASK ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
-
-    float4_t acc[4 * DS];
+    int32_t query[CT], g[CT], limit[CT];
 #pragma unroll
-    for (int d = 0; d < 4 * DS; ++d) acc[d] = float4_t{0, 0, 0, 0};
-    float top = -__builtin_inff(), sum = 0.0f;
-    const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
-    for (int32_t t = t_begin + wave; t < t_end; t += WAVES) {
-        const int32_t k0 = t * kTile;
-        float4_t s[4];
+    for (int c = 0; c < CT; ++c) {
+        const int32_t row = min(r_first + c * 16 + col, r_last);       // (rows past the end repeat the last one)
+        query[c] = row / a.group;
+        g[c] = row - query[c] * a.group;
+        limit[c] = a.causal ? min(range.len, range.pos + query[c] + 1) : range.len;
+    }
+    // keys that every row sees (without a mask), distances of the first and last of the queries
+    const int32_t first_at = range.pos + r_first / a.group;
+    const int32_t all_see = a.causal ? min(range.len, first_at + 1) : range.len;
+
+    // A tile's operands are on their way while the one before it is multiplied.  Row r of the key operand is key 16 (r / 4) + 4 j + r % 4 of the tile, so that a
+    // lane's results are neighbours; units past the head's meet zeros of the query.
+    const int32_t key_row = (col >> 2) * 16 + (col & 3);
+    uint4_t kr[4 * DS], vr[4 * DS], mk[CT];
+    half_t kt, vt;
+    // keys that one workgroup looks at are read once (with the hint: 32 x 64 heads over up to 1024 keys 40.6 -> 36.2 us)
+    auto load = [&](const int8_t* p) { return CT == 1 ? __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)) : *reinterpret_cast<const uint4_t*>(p); };
+    auto fetch_keys = [&](int32_t t) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            // row r of this operand is key 16 (r / 4) + 4 j + r % 4, so that a lane's results are neighbours
-            const int32_t key = min(k0 + (col >> 2) * 16 + j * 4 + (col & 3), a.length - 1);
-            s[j] = float4_t{0, 0, 0, 0};
+            const uint32_t o = (uint32_t)min(t * kTile + key_row + j * 4, a.length - 1) * (uint32_t)a.dim;
 #pragma unroll
             for (int d = 0; d < DS; ++d) {
-                const int u = d * 64 + quad * 16;       // (units past the head's meet zeros of the query)
-                half8_t lo, hi;
-                halves_of(*reinterpret_cast<const uint4_t*>(keys + (int64_t)key * a.dim + (u < a.dim ? u : 0)), lo, hi);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, q[2 * d], s[j], 0, 0, 0);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, q[2 * d + 1], s[j], 0, 0, 0);
+                const int u = d * 64 + quad * 16;
+                kr[j * DS + d] = load(keys + (o + (uint32_t)(u < a.dim ? u : 0)));
             }
         }
-        const int32_t mine = k0 + quad * 16, at = min(mine, a.length - 16);
-        const float factor = (float)key_top[at >> a.block_shift] * (1.0f / 127.0f) * a.scale;
-        const float vs = kv_scale(value_top[at >> a.block_shift]), add = __builtin_log2f(vs);
-        float x[16];
+        const int32_t at = min(t * kTile + quad * 16, a.length - 16);
+        kt = key_top[(uint32_t)at >> a.block_shift];
+        vt = value_top[(uint32_t)at >> a.block_shift];
+        if (MASK)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            float bias = add;
-            if (BIAS) bias = __builtin_fmaf((float)biases[max(a.first_distance, min(where - (mine + j), a.distances - 1)) - a.first_distance], kLog2e, add);
-            x[j] = __builtin_fmaf(s[j >> 2][j & 3], factor, bias);
-            if (mine + j >= limit) x[j] = -__builtin_inff();
+            for (int c = 0; c < CT; ++c) {
+                struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
+                mk[c] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(a.mask + b * a.mask_batch + query[c] * a.mask_token + at));
+            }
+    };
+    auto fetch_values = [&](int32_t t) {
+        const uint32_t o = (uint32_t)min(t * kTile + quad * 16, a.length - 16) * (uint32_t)a.dim + col * 16;
+#pragma unroll
+        for (int d = 0; d < 4 * DS; ++d) vr[d] = load(values + (o + (uint32_t)(d * 16 < a.dim ? d * 256 : 0)));
+    };
+    if (t_begin + wave < t_end) {
+        fetch_keys(t_begin + wave);
+        fetch_values(t_begin + wave);
+    }
+    half8_t q[CT][2 * DS];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+        load_query(q[c], a.q + b * a.q_batch + (int64_t)(kvh * a.group + g[c]) * a.q_head + (int64_t)query[c] * a.q_token, a.q_unit, a.dim,
+                   [&](int s) { return (s >> 1) * 64 + quad * 16 + (s & 1) * 8; });
+    const int entries = a.distances - a.first_distance;
+    const half_t* biases[CT];
+    if (BIAS) {
+        // the bias of every distance from first_distance on, for each head of the tile
+        const int slots = min(a.group, ROWS);
+        for (int i = tid; i < slots * entries; i += kWaves * 64) {
+            const int slot = i / entries, rel = i - slot * entries + a.first_distance;
+            const int head = kvh * a.group + (a.group <= ROWS ? slot : (r_first + slot) % a.group);
+            const int bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
+            table[i] = a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))];
         }
-        if (MASK) {
-            struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
-            const Byte16Any keep = *reinterpret_cast<const Byte16Any*>(mask + at);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (!(keep.w[j >> 2] >> ((j & 3) * 8) & 0xffu)) x[j] = -__builtin_inff();
+        for (int c = 0; c < CT; ++c) biases[c] = table + (a.group <= ROWS ? g[c] : c * 16 + col) * entries - a.first_distance;
+        __syncthreads();
+    }
+
+    float4_t acc[CT][4 * DS];
+    float top[CT], sum[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+#pragma unroll
+        for (int d = 0; d < 4 * DS; ++d) acc[c][d] = float4_t{0, 0, 0, 0};
+        top[c] = -__builtin_inff();
+        sum[c] = 0.0f;
+    }
+    for (int32_t t = t_begin + wave; t < t_end; t += kWaves) {
+        const int32_t k0 = t * kTile, mine = k0 + quad * 16;
+        float4_t s[CT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) s[c][j] = float4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                half8_t lo, hi;
+                halves_of(kr[j * DS + d], lo, hi);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    s[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, q[c][2 * d], s[c][j], 0, 0, 0);
+                    s[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, q[c][2 * d + 1], s[c][j], 0, 0, 0);
+                }
+            }
         }
-        float m = x[0];
+        const float factor = (float)kt * (1.0f / 127.0f) * a.scale, vs = kv_scale(vt), add = __builtin_amdgcn_logf(vs), inverse = __builtin_amdgcn_rcpf(vs);
+        uint4_t keep[CT];
+        if (MASK)
 #pragma unroll
-        for (int j = 1; j < 16; ++j) m = fmaxf(m, x[j]);
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        if (__builtin_amdgcn_ballot_w64(m > top)) {
-            const float now = fmaxf(m, top);
-            const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
-            top = now;
-            sum *= f;
+            for (int c = 0; c < CT; ++c) keep[c] = mk[c];
+        if (t + kWaves < t_end) fetch_keys(t + kWaves);
+        half8_t p[CT][2];
 #pragma unroll
-            for (int d = 0; d < 4 * DS; ++d) acc[d] *= f;
+        for (int c = 0; c < CT; ++c) {
+            float x[16];
+            // (one bias for the whole tile where all its distances lie beyond the table's end)
+            const bool far = BIAS && first_at - (k0 + kTile - 1) >= a.distances - 1;
+            if (BIAS && !far) {
+                const int32_t where = range.pos + query[c];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float bias = (float)biases[c][max(a.first_distance, min(where - (mine + j), a.distances - 1))];
+                    x[j] = __builtin_fmaf(s[c][j >> 2][j & 3], factor, __builtin_fmaf(bias, kLog2e, add));
+                }
+            } else {
+                const float shift = BIAS ? __builtin_fmaf((float)biases[c][a.distances - 1], kLog2e, add) : add;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = __builtin_fmaf(s[c][j >> 2][j & 3], factor, shift);
+            }
+            if (k0 + kTile > all_see) {
+                const int32_t left = limit[c] - mine;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = j < left ? x[j] : -__builtin_inff();
+            }
+            if (MASK)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = (keep[c][j >> 2] >> ((j & 3) * 8) & 0xffu) ? x[j] : -__builtin_inff();
+            float m = x[0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) m = fmaxf(m, x[j]);
+            m = quad_max(m);
+            if (__builtin_amdgcn_ballot_w64(m > top[c] + kLazy)) {
+                const float now = fmaxf(m, top[c]);
+                const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[c] - now);
+                top[c] = now;
+                sum[c] *= f;
+#pragma unroll
+                for (int d = 0; d < 4 * DS; ++d) acc[c][d] *= f;
+            }
+            const float base = top[c] == -__builtin_inff() ? 0.0f : top[c];
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float e = __builtin_amdgcn_exp2f(x[j] - base);
+                part += e;
+                p[c][j >> 3][j & 7] = (half_t)e;
+            }
+            sum[c] = __builtin_fmaf(part, inverse, sum[c]);
         }
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        float part = 0.0f;
-        half8_t p[2];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float e = __builtin_amdgcn_exp2f(x[j] - base);
-            part += e;
-            p[j >> 3][j & 7] = (half_t)e;
-        }
-        sum = __builtin_fmaf(part, 1.0f / vs, sum);
 #pragma unroll
         for (int d = 0; d < 4 * DS; ++d) {
-            const int u = d * 16;
             half8_t lo, hi;
-            halves_of(*reinterpret_cast<const uint4_t*>(values + (int64_t)at * a.dim + ((u < a.dim ? u : 0) + col) * 16), lo, hi);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[0], acc[d], 0, 0, 0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[1], acc[d], 0, 0, 0);
+            halves_of(vr[d], lo, hi);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[c][0], acc[c][d], 0, 0, 0);
+                acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][1], acc[c][d], 0, 0, 0);
+            }
         }
+        if (t + kWaves < t_end) fetch_values(t + kWaves);
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (quad == 0) {
-        stat[wave][0][col] = top;
-        stat[wave][1][col] = sum;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        sum[c] += __shfl_xor(sum[c], 16);
+        sum[c] += __shfl_xor(sum[c], 32);
+        if (quad == 0) {
+            stat[wave][0][c * 16 + col] = top[c];
+            stat[wave][1][c * 16 + col] = sum[c];
+        }
     }
     // the waves' sums under the largest of their maxima, 64 units at a time
+    float* const part = a.parts + ((head * a.row_tiles + rt) * a.splits + split) * ROWS * (a.dim + 2);
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
-    if (ds) __syncthreads();
+        if (ds) __syncthreads();
 #pragma unroll
-    for (int d = 0; d < 4; ++d) *reinterpret_cast<float4_t*>(&joined[wave][col][d * 16 + quad * 4]) = acc[ds * 4 + d];
-    __syncthreads();
-    for (int i = tid; i < 16 * 64; i += WAVES * 64) {
-        const int r = i >> 6, u = ds * 64 + (i & 63);
-        if (rt * 16 + r >= rows || u >= a.dim) continue;
-        float m = stat[0][0][r];
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int v = 1; v < WAVES; ++v) m = fmaxf(m, stat[v][0][r]);
-        const float base = m == -__builtin_inff() ? 0.0f : m;
-        float value = 0.0f, total = 0.0f;
+            for (int d = 0; d < 4; ++d) *reinterpret_cast<float4_t*>(&joined[wave][c * 16 + col][d * 16 + quad * 4]) = acc[c][ds * 4 + d];
+        __syncthreads();
+        for (int i = tid; i < ROWS * 64; i += kWaves * 64) {
+            const int r = i >> 6, u = ds * 64 + (i & 63);
+            if (r_first + r > r_last || u >= a.dim) continue;
+            float m = stat[0][0][r];
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
-            const float f = __builtin_amdgcn_exp2f(stat[v][0][r] - base);
-            value = __builtin_fmaf(joined[v][r][i & 63], f, value);
-            total = __builtin_fmaf(stat[v][1][r], f, total);
-        }
-        if (a.splits > 1) {
-            float* const part = a.parts + (tile_of * a.splits + split) * 16 * (a.dim + 2);
-            part[r * a.dim + u] = value;
-            if (u == 0) {
-                part[16 * a.dim + r] = m;
-                part[16 * a.dim + 16 + r] = total;
+            for (int v = 1; v < kWaves; ++v) m = fmaxf(m, stat[v][0][r]);
+            const float base = m == -__builtin_inff() ? 0.0f : m;
+            float value = 0.0f, total = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                const float f = __builtin_amdgcn_exp2f(stat[v][0][r] - base);
+                value = __builtin_fmaf(joined[v][r][i & 63], f, value);
+                total = __builtin_fmaf(stat[v][1][r], f, total);
             }
-        } else {
-            const int32_t rr = rt * 16 + r, qq = rr / a.group;
-            a.out[b * a.out_batch + (int64_t)(kvh * a.group + rr - qq * a.group) * a.out_head + (int64_t)qq * a.out_token + (int64_t)u * a.out_unit] =
-                (half_t)(total == 0.0f ? 0.0f : value / total);
+            if (a.splits > 1) {
+                part[r * a.dim + u] = value;
+                if (u == 0) {
+                    part[ROWS * a.dim + r] = m;
+                    part[ROWS * a.dim + ROWS + r] = total;
+                }
+            } else {
+                const int32_t rr = r_first + r, qq = rr / a.group;
+                a.out[b * a.out_batch + (int64_t)(kvh * a.group + rr - qq * a.group) * a.out_head + (int64_t)qq * a.out_token + (int64_t)u * a.out_unit] =
+                    (half_t)(total == 0.0f ? 0.0f : value / total);
+            }
         }
-    }
     }
 }
 
@@ -200,13 +284,30 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
     m = wave_max(m);
     const float base = m == -__builtin_inff() ? 0.0f : m;
     float total = 0.0f, value[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < range.parts; ++i) {
-        const float f = __builtin_amdgcn_exp2f(tops[i * size] - base);
-        total = __builtin_fmaf(tops[i * size + rows], f, total);
+    for (int first = 0; first < range.parts; first += 64) {
+        // a lane a part: its weight; then eight parts' sums at a time, all on their way together
+        const bool real = first + lane < range.parts;
+        const float* const mine = tops + (first + (real ? lane : 0)) * size;
+        const float weight = real ? __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
+        total = __builtin_fmaf(real ? mine[rows] : 0.0f, weight, total);
+        const int n = min(64, range.parts - first);
+        for (int i = 0; i < n; i += 8) {
+            float x[8][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (c * 64 + lane < a.dim) value[c] = __builtin_fmaf(part[i * size + in_tile * a.dim + c * 64 + lane], f, value[c]);
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c * 64 < a.dim) x[k][c] = part[(first + min(i + k, n - 1)) * size + in_tile * a.dim + min(c * 64 + lane, a.dim - 1)];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = i + k < n ? __shfl(weight, i + k) : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c * 64 < a.dim) value[c] = __builtin_fmaf(x[k][c], f, value[c]);
+            }
+        }
     }
+    total = wave_sum(total);
     half_t* const out = a.out + b * a.out_batch + (int64_t)(h * group + g) * a.out_head + (int64_t)query * a.out_token;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -221,22 +322,28 @@ struct KvPlan {
 static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length) {
     KvPlan p;
     p.chunks = tokens > 32;
-    p.rows = p.chunks ? kChunkRows : 16;
+    p.rows = p.chunks ? kChunkRows : tokens * (heads / held) > 16 && dim <= 128 ? 32 : 16;
     p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
     const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, most = ceil_div(length, kTile * (p.chunks ? kChunkLeast : kWaves));
-    const int64_t want = ceil_div((p.chunks ? 1 : 4) * (int64_t)compute_units(), base);
+    const int64_t want = ceil_div((p.chunks ? 1 : 2) * (int64_t)compute_units(), base);
     p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
     return p;
 }
 
-template <int DS>
-static void kv_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
-    const size_t lds = a.table ? (size_t)(a.group < 16 ? a.group : 16) * (a.distances - a.first_distance) * sizeof(half_t) : 0;
-    const dim3 g(grid), t(kWaves * 64);
-    if (a.table && a.mask) hipLaunchKernelGGL((k_kv_attend<DS, kWaves, true, true>), g, t, lds, st, a);
-    else if (a.table) hipLaunchKernelGGL((k_kv_attend<DS, kWaves, true, false>), g, t, lds, st, a);
-    else if (a.mask) hipLaunchKernelGGL((k_kv_attend<DS, kWaves, false, true>), g, t, lds, st, a);
-    else hipLaunchKernelGGL((k_kv_attend<DS, kWaves, false, false>), g, t, lds, st, a);
+template <int DS, int CT, bool BIAS, bool MASK>
+static int kv_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
+    const size_t lds = BIAS ? (size_t)(a.group < CT * 16 ? a.group : CT * 16) * (a.distances - a.first_distance) * sizeof(half_t) : 0;
+    static std::atomic<bool> done[64];
+    if (BIAS)
+        if (int e = enable_dynamic_lds((const void*)k_kv_attend<DS, CT, BIAS, MASK>, 32 * 1024 * (int)sizeof(half_t), done)) return e;
+    hipLaunchKernelGGL((k_kv_attend<DS, CT, BIAS, MASK>), dim3(grid), dim3(kWaves * 64), lds, st, a);
+    return 0;
+}
+
+template <int DS, int CT>
+static int kv_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
+    if (a.table) return a.mask ? kv_launch<DS, CT, true, true>(a, grid, st) : kv_launch<DS, CT, true, false>(a, grid, st);
+    return a.mask ? kv_launch<DS, CT, false, true>(a, grid, st) : kv_launch<DS, CT, false, false>(a, grid, st);
 }
 
 }  // namespace cpmk
@@ -287,12 +394,12 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     const int64_t grid = (int64_t)batch * kv_heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
     if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
     hipStream_t st = (hipStream_t)stream;
-    if (plan.chunks) {
-        if (int e = kv_chunk_launch(a, batch, st)) return e;
-    } else if (dim <= 64) kv_launch<1>(a, (unsigned)grid, st);
-    else if (dim <= 128) kv_launch<2>(a, (unsigned)grid, st);
-    else if (dim <= 192) kv_launch<3>(a, (unsigned)grid, st);
-    else kv_launch<4>(a, (unsigned)grid, st);
+    const unsigned g = (unsigned)grid;
+    int e;
+    if (plan.chunks) e = kv_chunk_launch(a, batch, st);
+    else if (plan.rows == 32) e = dim <= 64 ? kv_launch<1, 2>(a, g, st) : kv_launch<2, 2>(a, g, st);
+    else e = dim <= 64 ? kv_launch<1, 1>(a, g, st) : dim <= 128 ? kv_launch<2, 1>(a, g, st) : dim <= 192 ? kv_launch<3, 1>(a, g, st) : kv_launch<4, 1>(a, g, st);
+    if (e) return e;
     if (a.splits > 1)
         hipLaunchKernelGGL(k_kv_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan.rows, (int)plan.chunks, (uint32_t)rows);
     return launch_status();

@@ -16,7 +16,6 @@
 
 namespace cpmk {
 
-constexpr int kLazy = 8;
 constexpr int kChunkWaves = kChunkRows / 32;
 
 // N products whose operands come from LDS one each: so many reads ahead that a read's latency lies behind products (the compiler keeps two ahead).
@@ -42,14 +41,16 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
     float* const biases = reinterpret_cast<float*>(lds + 2 * kBuffer);
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+    const uint32_t inner = (uint32_t)a.group * a.row_tiles * a.splits;
+    uint32_t unit, w;
+    kv_deal(blockIdx.x, gridDim.x / inner, inner, unit, w);
+    const int64_t b = unit / (uint32_t)a.held;
     const int32_t split = w % (uint32_t)a.splits;
     w /= (uint32_t)a.splits;
-    const int64_t tile_of = w;
-    const int32_t qt = w % (uint32_t)a.row_tiles;
-    w /= (uint32_t)a.row_tiles;
-    const int32_t h = w % (uint32_t)a.heads;
-    const int64_t b = w / (uint32_t)a.heads;
+    // (of a causal chunk the last queries see most keys: their workgroups come first)
+    const int32_t qt = a.row_tiles - 1 - (int32_t)(w % (uint32_t)a.row_tiles);
+    const int32_t h = (unit - (uint32_t)b * a.held) * a.group + w / (uint32_t)a.row_tiles;
+    const int64_t tile_of = (b * a.heads + h) * a.row_tiles + qt;
     const KvRange range = kv_range(a, b, min(qt * ROWS + ROWS - 1, a.tokens - 1), kChunkLeast);
     if (split >= range.parts) return;
 
