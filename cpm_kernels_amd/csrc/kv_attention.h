@@ -1,6 +1,6 @@
 // What the kernels of the attention over the 8-bit key/value cache share (kv_attention.hip: few queries, kv_chunk.hip: many).
 #pragma once
-#include "common.h"
+#include "kv_ints.h"
 
 namespace cpmk {
 
@@ -31,26 +31,6 @@ constexpr int kLazy = 8;             // log2 of how far the running maximum may 
 constexpr int kChunkRows = 128;     // queries of a workgroup (kv_chunk.hip)
 constexpr int kChunkLeast = 4;       // tiles of a part, at least (kv_chunk.hip)
 constexpr int kChunkPad = 96;        // distances beyond the table's ends that a tile of 32 queries and 64 keys can reach into
-
-// sixteen bytes as integers -> halves, exactly: 1024 + 128 + q has q in its last bits
-__device__ __forceinline__ void halves_of(uint4_t p, half8_t& lo, half8_t& hi) {
-    uint32_t h[8];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        const uint32_t u = p[d] ^ 0x80808080u;
-        h[2 * d] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-        h[2 * d + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    }
-    const half2_t off = {(half_t)1152.0f, (half_t)1152.0f};
-    uint4_t a, b;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        a[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[d]) - off);
-        b[d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, h[4 + d]) - off);
-    }
-    lo = __builtin_bit_cast(half8_t, a);
-    hi = __builtin_bit_cast(half8_t, b);
-}
 
 __device__ __forceinline__ float kv_scale(half_t top) { return fmaxf((float)top * (1.0f / 127.0f), 0x1p-34f); }
 

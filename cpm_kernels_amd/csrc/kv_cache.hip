@@ -15,7 +15,7 @@
 // bytes in both, sixteen units of a token and sixteen tokens of a unit.  Such a run is the "minor" axis here, and a lane takes a piece of 4 (major) x 16 (minor) elements:
 // four 16-byte accesses to the cache; to and from the fp16 side 32 contiguous bytes four times where the minor axis is contiguous there too ("straight"), 8 bytes sixteen
 // times where the major axis is ("crossed"), single halves otherwise and at the ends of a range.
-#include "common.h"
+#include "kv_ints.h"
 
 namespace cpmk {
 
@@ -33,6 +33,7 @@ struct KvArgs {
     KvSide side[2];
     const int32_t *pos_each, *count_each;
     int32_t pos, tokens, heads, dim, length, block;
+    int32_t block_shift;
     int32_t span;           // tokens of a workgroup: whole blocks (write), a multiple of 16 (read)
     int32_t pieces;         // of a workgroup, span * dim / 64
     uint32_t chunks;        // workgroups of a head
@@ -168,6 +169,72 @@ __device__ __forceinline__ void write_piece(const KvArgs& a, const KvSide& s, ui
     }
 }
 
+// One token a sequence, the decode step: a wave a head's key or value, whose units its lanes hold.  Its integers are all that is written unless the token is larger than what its block holds, in which case
+// the block's older ones are read and rounded again.  Bound by latency: of the general kernel, which passes over the whole block either way, 32 x 64 heads of 64 took 13.2 us.
+template <bool V>
+__device__ __forceinline__ void write_token(const KvArgs& a, const KvSide& s, int64_t b, int32_t h, int32_t pos) {
+    const int lane = threadIdx.x & 63;
+    const int64_t head = b * a.heads + h;
+    const half_t* const x = s.x + b * s.batch + h * s.head;
+    const int32_t first = pos & -a.block;
+    half_t* const top = s.top + head * (a.length / a.block) + pos / a.block;
+    const uint32_t old = first < pos ? min((uint32_t)(__builtin_bit_cast(uint16_t, *top) & 0x7fff), 0x7bffu) : 0u;
+    half_t v[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        v[c] = 0;
+        if (c * 64 + lane < a.dim) v[c] = x[(int64_t)(c * 64 + lane) * s.unit];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint16_t w = __builtin_bit_cast(uint16_t, v[c]), w0 = w & 0x7fff;
+        const uint16_t r = w0 > 0x7c00 ? (uint16_t)0 : w0 == 0x7c00 ? (uint16_t)(w - 1) : w;
+        v[c] = __builtin_bit_cast(half_t, r);
+        m = max(m, (uint32_t)(r & 0x7fff));
+    }
+    m = max(wave_max_u32_uniform(m), old);
+    const float now = (float)__builtin_bit_cast(half_t, (uint16_t)m);
+    const float y = now > 0.0f ? 127.0f / now * kUp : 0.0f;
+    int8_t* const ints = s.ints + head * a.length * a.dim;
+    int8_t* const at = V ? ints + (int64_t)(pos >> 4) * 16 * a.dim + (pos & 15) : ints + (int64_t)pos * a.dim;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c * 64 + lane < a.dim) at[(c * 64 + lane) * (V ? 16 : 1)] = (int8_t)nearest_bits((float)v[c] * y);
+    if (m == old) return;
+    if (lane == 0) *top = __builtin_bit_cast(half_t, (uint16_t)m);
+    if (first == pos) return;
+    const float again = (float)__builtin_bit_cast(half_t, (uint16_t)old) / now * kUp;
+    // sixteen bytes at a time: whole keys; whole groups of values, of the last one the bytes before the token
+    const int32_t part = V ? pos & 15 : 0, pieces = ((V ? (pos + 15) & -16 : pos) - first) * a.dim / 16, partial = V && part ? pieces - a.dim : pieces;
+    uint4_t* const p = reinterpret_cast<uint4_t*>(ints + (int64_t)first * a.dim);
+    for (int i = lane; i < pieces; i += 64) {
+        const uint4_t w = p[i];
+        uint4_t r;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            uint32_t q[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q[k] = nearest_bits((float)((int32_t)(w[d] << (24 - 8 * k)) >> 24) * again);
+            r[d] = pack4_i8(q[0], q[1], q[2], q[3]);
+        }
+        if (i < partial) p[i] = r;
+        else
+            for (int k = 0; k < part; ++k) reinterpret_cast<int8_t*>(p + i)[k] = (int8_t)(r[k >> 2] >> (8 * (k & 3)));
+    }
+}
+
+__global__ __launch_bounds__(256) void k_kv_write_token(KvArgs a, uint32_t waves) {
+    const uint32_t w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (w >= waves) return;
+    const uint32_t head = w >> 1;
+    const int64_t b = head / (uint32_t)a.heads;
+    const int32_t h = head - (uint32_t)b * a.heads, pos = a.pos_each ? a.pos_each[b] : a.pos;
+    if (pos < 0 || pos >= a.length || (a.count_each && a.count_each[b] <= 0)) return;
+    if (w & 1) write_token<true>(a, a.side[1], b, h, pos);
+    else write_token<false>(a, a.side[0], b, h, pos);
+}
+
 // grid: chunks x heads x batch x (keys, values)
 __global__ __launch_bounds__(512) void k_kv_write(KvArgs a) {
     __shared__ uint32_t tops[65];
@@ -193,34 +260,42 @@ __device__ __forceinline__ void read_piece(const KvArgs& a, const KvSide& s, int
     if ((int)threadIdx.x >= a.pieces) return;
     const int64_t head = b * a.heads + h, end = (int64_t)from + a.tokens;
     int major[4], minor;
-    piece_of<V>(threadIdx.x, a.dim, a.span, s.mode != kStraight, major, minor);
+    piece_of<V>(threadIdx.x, a.dim, 16, s.mode != kStraight, major, minor);
+    // (a piece's tokens lie in one group of sixteen, which lies in the cache or outside of it)
+    const int64_t group = first + ((V ? minor : major[0]) & -16);
     const int64_t t_lo = first + (V ? minor : major[0]), t_hi = first + (V ? minor + 15 : major[3]);
     if (t_lo >= end || t_hi < from) return;
-    const int8_t* const ints = s.ints + head * a.length * a.dim;
-    const half_t* const top = s.top + head * (a.length / a.block);
-    half_t* const x = const_cast<half_t*>(s.x) + b * s.batch + h * s.head;
+    const bool inside = group >= 0 && group < a.length;
+    const int8_t* const ints = s.ints + (head * a.length + (inside ? group : 0)) * a.dim;
+    const int skip = inside ? (int)(first - group) : 0;                    // tokens from the group to the workgroup's first one
+    uint4_t p[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int o = V ? major[e] * 16 : (inside ? major[e] + skip : 0) * a.dim + minor;
+        p[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(ints + o));
+    }
+    const half_t top = s.top[head * (a.length >> a.block_shift) + ((inside ? group : 0) >> a.block_shift)];
+    const float f = inside ? (float)top / 127.0f : 0.0f;
     half8_t v[4][2];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int64_t t = first + (V ? minor : major[e]);
-        const bool inside = t >= 0 && t < a.length;         // (sixteen tokens of a value lie inside or outside together)
-        const int64_t at = inside ? t : 0;
-        const uint4_t p = *reinterpret_cast<const uint4_t*>(V ? ints + at * a.dim + major[e] * 16 : ints + at * a.dim + minor);
-        const float f = inside ? (float)top[at / a.block] / 127.0f : 0.0f;
+        half8_t lo, hi;
+        halves_of(p[e], lo, hi);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float q = (float)((int32_t)(p[i >> 2] << (24 - 8 * (i & 3))) >> 24);
-            v[e][i >> 3][i & 7] = inside ? round_f16(q * f) : (half_t)0.0f;
+        for (int i = 0; i < 8; ++i) {       // (a product rounded once, to fp16)
+            v[e][0][i] = inside ? (half_t)((float)lo[i] * f) : (half_t)0.0f;
+            v[e][1][i] = inside ? (half_t)((float)hi[i] * f) : (half_t)0.0f;
         }
     }
-    auto place = [&](int64_t t, int u) { return x + (t - from) * s.token + u * s.unit; };
+    half_t* const x = const_cast<half_t*>(s.x) + b * s.batch + h * s.head + (first - from) * s.token;
+    auto place = [&](int t, int u) { return x + t * s.token + u * s.unit; };
     const bool whole = t_lo >= from && t_hi < end;
     if (whole && s.mode == kStraight) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            half_t* p = V ? place(first + minor, major[e]) : place(first + major[e], minor);
-            store_half8_any(p, v[e][0]);
-            store_half8_any(p + 8, v[e][1]);
+            half_t* o = V ? place(minor, major[e]) : place(major[e], minor);
+            store_half8_any(o, v[e][0]);
+            store_half8_any(o + 8, v[e][1]);
         }
     } else if (whole && s.mode == kCrossed) {
 #pragma unroll
@@ -228,7 +303,7 @@ __device__ __forceinline__ void read_piece(const KvArgs& a, const KvSide& s, int
             half4_t q;
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[e] = v[e][i >> 3][i & 7];
-            *reinterpret_cast<Half4Any*>(V ? place(first + minor + i, major[0]) : place(first + major[0], minor + i)) = __builtin_bit_cast(Half4Any, q);
+            *reinterpret_cast<Half4Any*>(V ? place(minor + i, major[0]) : place(major[0], minor + i)) = __builtin_bit_cast(Half4Any, q);
         }
     } else {
 #pragma unroll
@@ -236,7 +311,7 @@ __device__ __forceinline__ void read_piece(const KvArgs& a, const KvSide& s, int
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int64_t t = first + (V ? minor + i : major[e]);
-                if (t >= from && t < end) *place(t, V ? major[e] : minor + i) = v[e][i >> 3][i & 7];
+                if (t >= from && t < end) *place(V ? minor + i : major[e], V ? major[e] : minor + i) = v[e][i >> 3][i & 7];
             }
     }
 }
@@ -289,7 +364,13 @@ int cpmk_kv_write_int8(int32_t batch, int32_t heads, int32_t tokens, int32_t dim
     a.side[1] = {(const half_t*)v, v_batch, v_head, v_token, v_unit, (int8_t*)values, (half_t*)value_absmax, kv_mode(true, v_token, v_unit)};
     a.pos_each = (const int32_t*)pos_each;
     a.count_each = (const int32_t*)count_each;
-    a.pos = pos, a.tokens = tokens, a.heads = heads, a.dim = dim, a.length = length, a.block = block;
+    a.pos = pos, a.tokens = tokens, a.heads = heads, a.dim = dim, a.length = length, a.block = block, a.block_shift = __builtin_ctz((unsigned)block);
+    if (tokens == 1) {
+        const int64_t waves = (int64_t)batch * heads * 2;
+        if (waves > 0x7fffffffll) return CPMK_ETOOBIG;
+        hipLaunchKernelGGL(k_kv_write_token, dim3((unsigned)ceil_div(waves, 4)), dim3(256), 0, (hipStream_t)stream, a, (uint32_t)waves);
+        return launch_status();
+    }
     // blocks that a sequence's tokens can lie in, 64 elements a lane, about 256 lanes a workgroup
     const int64_t behind = pos_each ? block - 1 : pos % block;
     int64_t blocks = ceil_div(behind + tokens, block);
@@ -317,7 +398,7 @@ int cpmk_kv_read_int8(int32_t batch, int32_t heads, int32_t tokens, int32_t dim,
     a.side[1] = {(const half_t*)v, out_batch, out_head, out_token, out_unit, (int8_t*)values, (half_t*)value_absmax, kv_mode(true, out_token, out_unit)};
     a.pos_each = (const int32_t*)from_each;
     a.count_each = nullptr;
-    a.pos = from, a.tokens = tokens, a.heads = heads, a.dim = dim, a.length = length, a.block = block;
+    a.pos = from, a.tokens = tokens, a.heads = heads, a.dim = dim, a.length = length, a.block = block, a.block_shift = __builtin_ctz((unsigned)block);
     const int64_t groups = ceil_div((from_each ? 15 : from & 15) + (int64_t)tokens, 16);
     int64_t some = 16384 / dim / 16;
     some = some > groups ? groups : some;
