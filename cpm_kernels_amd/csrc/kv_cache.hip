@@ -273,6 +273,7 @@ __device__ __forceinline__ void read_piece(const KvArgs& a, const KvSide& s, int
     for (int e = 0; e < 4; ++e) {
         const int o = V ? major[e] * 16 : (inside ? major[e] + skip : 0) * a.dim + minor;
         p[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(ints + o));
+        if (!inside) p[e] = uint4_t{0, 0, 0, 0};
     }
     const half_t top = s.top[head * (a.length >> a.block_shift) + ((inside ? group : 0) >> a.block_shift)];
     const float f = inside ? (float)top / 127.0f : 0.0f;
@@ -283,8 +284,8 @@ __device__ __forceinline__ void read_piece(const KvArgs& a, const KvSide& s, int
         halves_of(p[e], lo, hi);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {       // (a product rounded once, to fp16)
-            v[e][0][i] = inside ? (half_t)((float)lo[i] * f) : (half_t)0.0f;
-            v[e][1][i] = inside ? (half_t)((float)hi[i] * f) : (half_t)0.0f;
+            v[e][0][i] = (half_t)((float)lo[i] * f);
+            v[e][1][i] = (half_t)((float)hi[i] * f);
         }
     }
     half_t* const x = const_cast<half_t*>(s.x) + b * s.batch + h * s.head + (first - from) * s.token;

@@ -10,16 +10,22 @@
 Activations of this package are (batch, heads * dim_head, tokens): ``k.view(batch, heads, dim_head, tokens).transpose(2, 3)`` is what goes
 in, and a result for such queries has the same layout in memory.
 """
+from functools import lru_cache
+
 import torch
 from ..kernels import kv_write_int8, kv_read_int8, kv_attention_int8, kv_attention_int8_workspace
 from ..kernels.kv_cache import BLOCKS
 from ._common import cur_stream
 
 
-def _check_tokens(x: torch.Tensor, device, shape):
-    assert x.is_cuda and x.dtype == torch.float16 and x.ndim == 4 and x.device == device
-    assert x.size(0) == shape[0] and x.size(3) == shape[2] and (shape[1] is None or x.size(1) == shape[1])
+def _check_tokens(x: torch.Tensor, device):
+    assert x.dtype == torch.float16 and x.device == device
     assert not (x.requires_grad and torch.is_grad_enabled()), "the cache keeps no gradients"
+
+
+@lru_cache(maxsize=1024)
+def _workspace(device, *sizes):         # (how keys are divided depends on the device's number of compute units; the call costs more than the look-up)
+    return kv_attention_int8_workspace(*sizes)
 
 
 def _each(x, batch, device):
@@ -72,17 +78,18 @@ class QuantizedKV:
         With positions on the device a sequence at a negative one is left alone, and tokens that would come to lie behind the cache are dropped.
         What the sequence held behind the tokens written counts no longer."""
         device = self._here()
-        _check_tokens(k, device, (self.batch, self.heads, self.dim))
-        _check_tokens(v, device, (self.batch, self.heads, self.dim))
-        assert k.size(2) == v.size(2)
-        tokens = k.size(2)
+        _check_tokens(k, device)
+        _check_tokens(v, device)
+        assert k.ndim == 4 and k.shape == v.shape
+        batch, heads, tokens, dim = k.shape
+        assert batch == self.batch and heads == self.heads and dim == self.dim
         pos_each, pos = _each(pos, self.batch, device)
         assert pos_each is not None or 0 <= pos <= self.length - tokens, "tokens outside of the cache"
         count_each = None
         if count is not None:
             assert isinstance(count, torch.Tensor)
             count_each, _ = _each(count, self.batch, device)
-        kv_write_int8(self.batch, self.heads, tokens, self.dim, self.length, self.block, k.data_ptr(), k.stride(), v.data_ptr(), v.stride(), pos_each, pos,
+        kv_write_int8(batch, heads, tokens, dim, self.length, self.block, k.data_ptr(), k.stride(), v.data_ptr(), v.stride(), pos_each, pos,
                       count_each, self.keys.data_ptr(), self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), cur_stream())
 
     def read(self, start=0, tokens: int = None, columns: bool = False):
@@ -114,9 +121,10 @@ class QuantizedKV:
         bias, mapping, bidirectional: PositionEmbedding's weight (query heads, num_buckets) and the table of position_embedding_init.
         The result has the shape of q, and its layout where q is dense."""
         device = self._here()
-        _check_tokens(q, device, (self.batch, None, self.dim))
-        heads, queries = q.size(1), q.size(2)
-        assert (heads % self.heads == 0) if self.heads else heads == 0
+        _check_tokens(q, device)
+        assert q.ndim == 4
+        batch, heads, queries, dim = q.shape
+        assert batch == self.batch and dim == self.dim and ((heads % self.heads == 0) if self.heads else heads == 0)
         lens_each, keys = _each(lens, self.batch, device)
         assert lens_each is not None or 0 <= keys <= self.length, "more keys than the cache has"
         pos_each, first = _each(-1 if pos is None else pos, self.batch, device)
@@ -136,10 +144,10 @@ class QuantizedKV:
             assert not (bias.requires_grad and torch.is_grad_enabled()), "the cache keeps no gradients"
             bias_ptr, mapping_ptr, buckets, distances = bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0)
         out = torch.empty_like(q)
-        size = kv_attention_int8_workspace(self.batch, heads, self.heads, queries, self.dim, self.length)
+        size = _workspace(device.index, batch, heads, self.heads, queries, dim, self.length)
         space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        kv_attention_int8(self.batch, heads, self.heads, queries, self.dim, self.length, self.block, q.data_ptr(), q.stride(), self.keys.data_ptr(),
+        kv_attention_int8(batch, heads, self.heads, queries, dim, self.length, self.block, q.data_ptr(), q.stride(), self.keys.data_ptr(),
                           self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), lens_each, keys, pos_each, first, causal,
-                          self.dim ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, bidirectional, mask_ptr, mask_batch,
+                          dim ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, bidirectional, mask_ptr, mask_batch,
                           mask_token, out.data_ptr(), out.stride(), None if space is None else space.data_ptr(), cur_stream())
         return out
