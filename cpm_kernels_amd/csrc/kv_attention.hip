@@ -12,6 +12,7 @@
 // Work is divided over the keys too where rows are few: a workgroup takes every tile of 64 keys of its part, wave by wave, and its waves join their sums
 // through LDS; parts leave theirs in the workspace and a second kernel joins them.
 #include "kv_attention.h"
+#include <algorithm>
 
 namespace cpmk {
 
@@ -315,18 +316,22 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
 }
 
 // Which kernel a call takes, and into how many parts its keys are cut.
+//   Up to 64 queries on k_kv_attend, more on k_kv_chunk: 32 heads over 1024 (8 sequences) and 8192 keys (one), us, the one and the other: 33 queries of 64 units 21.6, 25.3 and 25.4, 29.7,
+//   64 22.1, 26.0 and 25.8, 30.3, 96 26.7, 31.6 and 26.6, 32.1; of 128 units 33 31.7, 34.0 and 33.1, 37.3, 64 32.4, 35.1 and 34.0, 38.8, 96 43.1, 43.7 and 36.0, 41.8.
+//   Parts as long as all workgroups run at once, two a compute unit, never more: a second round costs what a first does (4 x 64 heads over up to 32768 keys, eight to a head of the cache: 512 workgroups
+//   45 us, 1024 46, 2048 63 and the joining 6, 9, 22).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads over 1024 keys in one part 26.6 us, in two 45.2).
 struct KvPlan {
     int rows, row_tiles, splits;
     bool chunks;
 };
 static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length) {
     KvPlan p;
-    p.chunks = tokens > 32;
+    p.chunks = tokens > 64;
     p.rows = p.chunks ? kChunkRows : tokens * (heads / held) > 16 && dim <= 128 ? 32 : 16;
     p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
-    const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, most = ceil_div(length, kTile * (p.chunks ? kChunkLeast : kWaves));
-    const int64_t want = ceil_div((p.chunks ? 1 : 2) * (int64_t)compute_units(), base);
-    p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+    const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, tiles = ceil_div(length, kTile), units = compute_units();
+    const int64_t twice = std::min(2 * units / base, tiles / (p.chunks ? 16 : kWaves)), once = p.chunks ? std::min(units / base, tiles / kChunkLeast) : 1;
+    p.splits = (int)std::max<int64_t>(1, std::max(twice, once));
     return p;
 }
 
