@@ -105,6 +105,14 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
                 raw[i] = *reinterpret_cast<const uint4_t*>((is_key[i] ? keys : values) + o);
             }
     };
+    uint4_t keep[2];
+    auto fetch_mask = [&](int32_t t) {
+#pragma unroll
+        for (int su = 0; su < 2; ++su) {
+            struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
+            keep[su] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(mask + min(t * (int64_t)kTile + su * 32 + half * 16, (int64_t)a.length - 16)));
+        }
+    };
     auto fetch_tops = [&](int32_t t) {      // a lane a group of keys from tile t on
         const uint32_t at = (uint32_t)min(t * (int64_t)kTile + lane * 16, (int64_t)a.length - 16) >> a.block_shift;
         key_raw = key_top[at];
@@ -128,6 +136,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
     if (t_begin < t_end) {
         fetch(t_begin - 1);
         if (wave == 0) fetch_tops(t_begin);
+        if (MASK) fetch_mask(t_begin);
     }
     half8_t q[KS];
     load_query(q, a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim, [&](int s) { return s * 16 + half * 8; });
@@ -222,12 +231,9 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
 #pragma unroll
                         for (int j = 0; j < 16; ++j) s[su][j] = j < left ? s[su][j] : -__builtin_inff();
                     }
-                    if (MASK) {
-                        struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
-                        const Byte16Any keep = *reinterpret_cast<const Byte16Any*>(mask + min(mine, a.length - 16));
+                    if (MASK)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) s[su][j] = (keep.w[j >> 2] >> ((j & 3) * 8) & 0xffu) ? s[su][j] : -__builtin_inff();
-                    }
+                        for (int j = 0; j < 16; ++j) s[su][j] = (keep[su][j >> 2] >> ((j & 3) * 8) & 0xffu) ? s[su][j] : -__builtin_inff();
                     factor[su] = 1.0f;
                     add[su] = 0.0f;
                 }
@@ -263,6 +269,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
                 sum = __builtin_fmaf(part, fact[su][2], sum);
             }
         }
+        if (MASK) fetch_mask(t + 1);
         convert(t);
         fetch(t + 1);
         if (wave == 0 && t - t_begin >= 8) {        // eight tiles' magnitudes at a time, into the half of the ring that has been read
