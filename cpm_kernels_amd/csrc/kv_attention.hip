@@ -16,8 +16,6 @@
 
 namespace cpmk {
 
-constexpr int kWaves = 4;
-
 // The largest of a value over the four sixteens of lanes (no trip through the LDS crossbar).
 __device__ __forceinline__ float quad_max(float m) {
     // (a bit cast of a vector's element itself takes the first one's)
@@ -29,12 +27,12 @@ __device__ __forceinline__ float quad_max(float m) {
     return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
-// DS: 64-unit steps of a head, CT: sixteens of rows.
-template <int DS, int CT, bool BIAS, bool MASK>
-__global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAttention a) {
+// DS: 64-unit steps of a head, CT: sixteens of rows, WAVES of a workgroup.
+template <int DS, int CT, int WAVES, bool BIAS, bool MASK>
+__global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAttention a) {
     constexpr int ROWS = CT * 16;
-    __shared__ float joined[kWaves][ROWS][64 + 4];
-    __shared__ float stat[kWaves][2][ROWS];
+    __shared__ float joined[WAVES][ROWS][64 + 4];
+    __shared__ float stat[WAVES][2][ROWS];
     extern __shared__ half_t table[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -46,7 +44,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
     const int32_t kvh = w % (uint32_t)a.held;
     const int64_t b = w / (uint32_t)a.held;
     const int32_t rows = a.tokens * a.group, r_first = rt * ROWS, r_last = min(r_first + ROWS, rows) - 1;
-    const KvRange range = kv_range(a, b, r_last / a.group, kWaves);
+    const KvRange range = kv_range(a, b, r_last / a.group, WAVES);
     if (split >= range.parts) return;
     const int32_t t_begin = split * range.per_part, t_end = min(t_begin + range.per_part, range.tiles);
 
@@ -113,7 +111,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
     if (BIAS) {
         // the bias of every distance from first_distance on, for each head of the tile
         const int slots = min(a.group, ROWS);
-        for (int i = tid; i < slots * entries; i += kWaves * 64) {
+        for (int i = tid; i < slots * entries; i += WAVES * 64) {
             const int slot = i / entries, rel = i - slot * entries + a.first_distance;
             const int head = kvh * a.group + (a.group <= ROWS ? slot : (r_first + slot) % a.group);
             const int bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
@@ -133,7 +131,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
         top[c] = -__builtin_inff();
         sum[c] = 0.0f;
     }
-    for (int32_t t = t_begin + wave; t < t_end; t += kWaves) {
+    for (int32_t t = t_begin + wave; t < t_end; t += WAVES) {
         const int32_t k0 = t * kTile, mine = k0 + quad * 16;
         float4_t s[CT][4];
 #pragma unroll
@@ -156,7 +154,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
         if (MASK)
 #pragma unroll
             for (int c = 0; c < CT; ++c) keep[c] = mk[c];
-        if (t + kWaves < t_end) fetch_keys(t + kWaves);
+        if (t + WAVES < t_end) fetch_keys(t + WAVES);
         half8_t p[CT][2];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -215,7 +213,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
                 acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][1], acc[c][d], 0, 0, 0);
             }
         }
-        if (t + kWaves < t_end) fetch_values(t + kWaves);
+        if (t + WAVES < t_end) fetch_values(t + WAVES);
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -236,16 +234,16 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
 #pragma unroll
             for (int d = 0; d < 4; ++d) *reinterpret_cast<float4_t*>(&joined[wave][c * 16 + col][d * 16 + quad * 4]) = acc[c][ds * 4 + d];
         __syncthreads();
-        for (int i = tid; i < ROWS * 64; i += kWaves * 64) {
+        for (int i = tid; i < ROWS * 64; i += WAVES * 64) {
             const int r = i >> 6, u = ds * 64 + (i & 63);
             if (r_first + r > r_last || u >= a.dim) continue;
             float m = stat[0][0][r];
 #pragma unroll
-            for (int v = 1; v < kWaves; ++v) m = fmaxf(m, stat[v][0][r]);
+            for (int v = 1; v < WAVES; ++v) m = fmaxf(m, stat[v][0][r]);
             const float base = m == -__builtin_inff() ? 0.0f : m;
             float value = 0.0f, total = 0.0f;
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) {
+            for (int v = 0; v < WAVES; ++v) {
                 const float f = __builtin_amdgcn_exp2f(stat[v][0][r] - base);
                 value = __builtin_fmaf(joined[v][r][i & 63], f, value);
                 total = __builtin_fmaf(stat[v][1][r], f, total);
@@ -266,7 +264,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAt
 }
 
 // Parts joined under the largest of their maxima: a wave a row, its lanes along the units.  `rows` of them lie together (sixteen rows of a head of the cache, or queries of a query head).
-__global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int chunks, uint32_t total_rows) {
+__global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int chunks, int least, uint32_t total_rows) {
     const int lane = threadIdx.x & 63;
     const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= total_rows) return;
@@ -276,7 +274,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
     const int32_t h = w % (uint32_t)heads;
     const int64_t b = w / (uint32_t)heads;
     const int32_t rt = r / rows, in_tile = r - rt * rows, query = r / group, g = r - query * group;
-    const KvRange range = kv_range(a, b, min(rt * rows + rows - 1, of_head - 1) / group, chunks ? kChunkLeast : kWaves);
+    const KvRange range = kv_range(a, b, min(rt * rows + rows - 1, of_head - 1) / group, least);
     const int64_t size = (int64_t)rows * (a.dim + 2);
     const float* const part = a.parts + ((b * heads + h) * a.row_tiles + rt) * a.splits * size;
     const float* const tops = part + rows * a.dim + in_tile;
@@ -318,10 +316,12 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
 // Which kernel a call takes, and into how many parts its keys are cut.
 //   Up to 64 queries on k_kv_attend, more on k_kv_chunk: 32 heads over 1024 (8 sequences) and 8192 keys (one), us, the one and the other: 33 queries of 64 units 21.6, 25.3 and 25.4, 29.7,
 //   64 22.1, 26.0 and 25.8, 30.3, 96 26.7, 31.6 and 26.6, 32.1; of 128 units 33 31.7, 34.0 and 33.1, 37.3, 64 32.4, 35.1 and 34.0, 38.8, 96 43.1, 43.7 and 36.0, 41.8.
-//   Parts as long as all workgroups run at once, two a compute unit, never more: a second round costs what a first does (4 x 64 heads over up to 32768 keys, eight to a head of the cache: 512 workgroups
-//   45 us, 1024 46, 2048 63 and the joining 6, 9, 22).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads over 1024 keys in one part 26.6 us, in two 45.2).
+//   Workgroups of eight waves where they are few (8 x 32 heads of 64 units over 3000 keys: 28 us in fours, 24 in eights), of four where there are two to a compute unit anyway (32 x 64 over up to 1024: 36 and
+//   40); heads of more than 128 units need more registers than eight waves have.
+//   Parts as long as all workgroups run at once, never more: a second round costs what a first does (4 x 64 heads over up to 32768 keys, eight to a head of the cache, in workgroups of four waves: two
+//   a compute unit 45 us, four 46, sixteen 63 and the joining 6, 9, 22).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads over 1024 keys in one part 26.6 us, in two 45.2).
 struct KvPlan {
-    int rows, row_tiles, splits;
+    int rows, row_tiles, splits, waves;
     bool chunks;
 };
 static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length) {
@@ -330,25 +330,31 @@ static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens
     p.rows = p.chunks ? kChunkRows : tokens * (heads / held) > 16 && dim <= 128 ? 32 : 16;
     p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
     const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, tiles = ceil_div(length, kTile), units = compute_units();
-    const int64_t twice = std::min(2 * units / base, tiles / (p.chunks ? 16 : kWaves)), once = p.chunks ? std::min(units / base, tiles / kChunkLeast) : 1;
-    p.splits = (int)std::max<int64_t>(1, std::max(twice, once));
+    p.waves = dim <= 128 && base < 2 * units ? 8 : 4;
+    const int64_t splits = p.chunks ? std::max(std::min(2 * units / base, tiles / 16), std::min(units / base, tiles / kChunkLeast)) : std::min(8 / p.waves * units / base, tiles / p.waves);
+    p.splits = (int)std::max<int64_t>(1, splits);
     return p;
 }
 
-template <int DS, int CT, bool BIAS, bool MASK>
+template <int DS, int CT, int WAVES, bool BIAS, bool MASK>
 static int kv_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
     const size_t lds = BIAS ? (size_t)(a.group < CT * 16 ? a.group : CT * 16) * (a.distances - a.first_distance) * sizeof(half_t) : 0;
     static std::atomic<bool> done[64];
     if (BIAS)
-        if (int e = enable_dynamic_lds((const void*)k_kv_attend<DS, CT, BIAS, MASK>, 32 * 1024 * (int)sizeof(half_t), done)) return e;
-    hipLaunchKernelGGL((k_kv_attend<DS, CT, BIAS, MASK>), dim3(grid), dim3(kWaves * 64), lds, st, a);
+        if (int e = enable_dynamic_lds((const void*)k_kv_attend<DS, CT, WAVES, BIAS, MASK>, 32 * 1024 * (int)sizeof(half_t), done)) return e;
+    hipLaunchKernelGGL((k_kv_attend<DS, CT, WAVES, BIAS, MASK>), dim3(grid), dim3(WAVES * 64), lds, st, a);
     return 0;
 }
 
-template <int DS, int CT>
+template <int DS, int CT, int WAVES>
 static int kv_launch(const KvAttention& a, unsigned grid, hipStream_t st) {
-    if (a.table) return a.mask ? kv_launch<DS, CT, true, true>(a, grid, st) : kv_launch<DS, CT, true, false>(a, grid, st);
-    return a.mask ? kv_launch<DS, CT, false, true>(a, grid, st) : kv_launch<DS, CT, false, false>(a, grid, st);
+    if (a.table) return a.mask ? kv_launch<DS, CT, WAVES, true, true>(a, grid, st) : kv_launch<DS, CT, WAVES, true, false>(a, grid, st);
+    return a.mask ? kv_launch<DS, CT, WAVES, false, true>(a, grid, st) : kv_launch<DS, CT, WAVES, false, false>(a, grid, st);
+}
+
+template <int DS, int CT>
+static int kv_launch(const KvAttention& a, int waves, unsigned grid, hipStream_t st) {
+    return waves == 8 ? kv_launch<DS, CT, 8>(a, grid, st) : kv_launch<DS, CT, 4>(a, grid, st);
 }
 
 }  // namespace cpmk
@@ -402,11 +408,13 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     const unsigned g = (unsigned)grid;
     int e;
     if (plan.chunks) e = kv_chunk_launch(a, batch, st);
-    else if (plan.rows == 32) e = dim <= 64 ? kv_launch<1, 2>(a, g, st) : kv_launch<2, 2>(a, g, st);
-    else e = dim <= 64 ? kv_launch<1, 1>(a, g, st) : dim <= 128 ? kv_launch<2, 1>(a, g, st) : dim <= 192 ? kv_launch<3, 1>(a, g, st) : kv_launch<4, 1>(a, g, st);
+    else if (plan.rows == 32) e = dim <= 64 ? kv_launch<1, 2>(a, plan.waves, g, st) : kv_launch<2, 2>(a, plan.waves, g, st);
+    else if (dim <= 128) e = dim <= 64 ? kv_launch<1, 1>(a, plan.waves, g, st) : kv_launch<2, 1>(a, plan.waves, g, st);
+    else e = dim <= 192 ? kv_launch<3, 1, 4>(a, g, st) : kv_launch<4, 1, 4>(a, g, st);
     if (e) return e;
     if (a.splits > 1)
-        hipLaunchKernelGGL(k_kv_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan.rows, (int)plan.chunks, (uint32_t)rows);
+        hipLaunchKernelGGL(k_kv_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan.rows, (int)plan.chunks, plan.chunks ? kChunkLeast : plan.waves,
+                           (uint32_t)rows);
     return launch_status();
 }
 
