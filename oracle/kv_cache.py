@@ -110,7 +110,7 @@ def attention(q, keys, values, key_absmax, value_absmax, lens, scale, causal, po
                 out[b, h, i] = p @ v[seen] / total
                 size = p @ np.abs(v[seen]) / total
                 # exponent: fp32 chains of dim additions; the factor, the product, the bias and log2 of the magnitude (|.| <= 40) rounded once each
-                off = ((np.abs(k[seen]) @ np.abs(row)) * scale * (dim + 8) * 2.0 ** -24 + (np.abs(x) + np.abs(bias) + 40) * 2.0 ** -22).max()
+                off = ((np.abs(k[seen]) @ np.abs(row)) * abs(scale) * (dim + 8) * 2.0 ** -24 + (np.abs(x) + np.abs(bias) + 40) * 2.0 ** -22).max()
                 count = seen.sum()
                 bound[b, h, i] = size * (2.0 ** -11 + 2 * off + 2 * (count + 64) * 2.0 ** -24) + \
                     count * 127 * 2.0 ** -25 * (p * s[seen]).max() / total + np.abs(out[b, h, i]) * 2.0 ** -11 + 2.0 ** -25

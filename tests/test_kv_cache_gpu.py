@@ -64,7 +64,7 @@ def _ints(x):
 WRITES = [  # b, h, tokens, dim, length, block, pos
     (1, 1, 1, 16, 16, 16, 0), (2, 3, 1, 64, 128, 64, 100), (1, 2, 1, 80, 96, 32, 95), (1, 1, 64, 64, 64, 64, 0), (2, 2, 37, 64, 256, 64, 0),
     (2, 2, 37, 128, 256, 64, 61), (1, 2, 200, 80, 256, 16, 7), (1, 1, 300, 256, 384, 128, 70), (1, 3, 129, 240, 256, 128, 127), (3, 1, 500, 48, 512, 32, 12),
-    (1, 1, 1000, 16, 1024, 16, 24), (2, 1, 5, 64, 64, 64, 59),
+    (1, 1, 1000, 16, 1024, 16, 24), (2, 1, 5, 64, 64, 64, 59), (2, 2, 1, 256, 256, 128, 131), (1, 3, 1, 208, 64, 16, 47),
 ]
 
 
@@ -262,6 +262,47 @@ def test_attention_of_unequal_sequences(gpu, n):
         c.keys[i, :, keys:] = 77
         c.values[i, :, (keys + 15) // 16:] = -99
     assert torch.equal(c.attention(q[1], lens), got)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 40, 70, 200])
+def test_attention_in_parts(gpu, n, d):
+    """Caches so long that their keys are divided among workgroups, for sequences that fill all parts, one, some of the last and none."""
+    print("attention parts", n, d, flush=True)
+    rng = np.random.default_rng(n + d)
+    lens = _ints([0, 1, 64, 65, 1000, 2111, 2999, 3008])
+    both, q, got = _attend(rng, 8, 1, 1, n, d, 3008, 32, lens)
+    assert not bool(got[0].any())
+    pos = _ints([5, 0, 2000, -40, 3000, 1, 2700, 100])
+    _attend(rng, 8, 2, 2, n, d, 3008, 16, lens, layout="columns", pos=pos, **_bias(rng, 2, True))
+    mask = torch.from_numpy(rng.random((8, n, 3008)) < 0.01).cuda()
+    mask[4] = False
+    _, _, got = _attend(rng, 8, 2, 1, n, d, 3008, 64, lens, causal=False, mask=mask)
+    assert not bool(got[4].any())
+
+
+@pytest.mark.parametrize("n", [1, 20, 100])
+def test_attention_of_other_scales(gpu, n):
+    """A negative factor turns the order of the scores around, 0 makes the mean of the values; a large one leaves one key."""
+    print("attention scales", n, flush=True)
+    rng = np.random.default_rng(n)
+    for scale in (-0.125, 0.0, 4.0, -4.0):
+        both = _Both(rng, 2, 2, 256, 64, 64)
+        q = _tokens(rng, 2, 2, n, 64, "rows")
+        want, bound = ok.attention(q[0], both.k, both.v, both.ka, both.va, np.full(2, 250), scale, True)
+        err = np.abs(both.cache.attention(q[1], 250, scale=scale).cpu().numpy().astype(np.float64) - want)
+        assert (err <= bound).all(), (scale, (err / np.maximum(bound, 1e-30)).max())
+
+
+@pytest.mark.parametrize("buckets,distances,bidirectional", [(32, 128, True), (8, 20, False), (64, 1024, False), (64, 512, True), (4, 3, True), (1, 1, False)])
+@pytest.mark.parametrize("n,group", [(1, 1), (1, 20), (9, 4), (150, 1)])
+def test_attention_with_bias_tables_of_any_size(gpu, n, group, buckets, distances, bidirectional):
+    print("attention bias tables", n, group, buckets, distances, bidirectional, flush=True)
+    rng = np.random.default_rng(n + buckets)
+    mapping = torch.from_numpy(np.sort(rng.integers(0, max(buckets // (2 if bidirectional else 1), 1), distances)).astype(np.int32)).cuda()
+    bias = dict(bias=torch.from_numpy(rng.standard_normal((group, buckets)).astype(np.float16)).cuda(), mapping=mapping, bidirectional=bidirectional)
+    _attend(rng, 1, group, group, n, 64, 1472, 64, 1450, causal=False, pos=700, **bias)
+    _attend(rng, 1, group, group, n, 64, 1472, 64, 1450, **bias)
 
 
 def test_attention_beside_magnitudes_far_apart(gpu):
