@@ -13,9 +13,9 @@ in, and a result for such queries has the same layout in memory.
 from functools import lru_cache
 
 import torch
-from ..kernels import kv_write_int8, kv_read_int8, kv_attention_int8, kv_attention_int8_workspace
 from ..kernels.kv_cache import BLOCKS
-from ._common import cur_stream
+from ..library import cpmk          # (the launchers themselves: what the kernels layer checks is checked here, and a layer of forty arguments costs 1 us)
+from ._common import cur_stream, _device
 
 
 def _check_tokens(x: torch.Tensor, device):
@@ -25,7 +25,7 @@ def _check_tokens(x: torch.Tensor, device):
 
 @lru_cache(maxsize=1024)
 def _workspace(device, *sizes):         # (how keys are divided depends on the device's number of compute units; the call costs more than the look-up)
-    return kv_attention_int8_workspace(*sizes)
+    return cpmk.kv_attention_int8_workspace(*sizes)
 
 
 def _each(x, batch, device):
@@ -68,8 +68,10 @@ class QuantizedKV:
                    zeros(*tops, dtype=torch.float16))
 
     def _here(self):
-        assert self.keys.device.index == torch.cuda.current_device(), "the cache lies on another device than the current one"
-        return self.keys.device
+        here = _device() if _device is not None and torch.cuda.is_initialized() else torch.cuda.current_device()
+        device = self.keys.device
+        assert device.index == here, "the cache lies on another device than the current one"
+        return device
 
     def write(self, k: torch.Tensor, v: torch.Tensor, pos, count=None) -> None:
         """k, v (batch, heads, tokens, dim) to the positions pos .. pos + tokens - 1 of every sequence; pos an int, or an int32 tensor with one for each.
@@ -89,8 +91,8 @@ class QuantizedKV:
         if count is not None:
             assert isinstance(count, torch.Tensor)
             count_each, _ = _each(count, self.batch, device)
-        kv_write_int8(batch, heads, tokens, dim, self.length, self.block, k.data_ptr(), k.stride(), v.data_ptr(), v.stride(), pos_each, pos,
-                      count_each, self.keys.data_ptr(), self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), cur_stream())
+        cpmk.kv_write_int8(batch, heads, tokens, dim, self.length, self.block, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), pos_each, pos,
+                           count_each, self.keys.data_ptr(), self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), cur_stream())
 
     def read(self, start=0, tokens: int = None, columns: bool = False):
         """Keys and values of the positions start .. start + tokens - 1 (start an int or an int32 tensor with one for each sequence; tokens: up to the
@@ -107,8 +109,9 @@ class QuantizedKV:
             out = torch.empty(shape, dtype=torch.float16, device=device)
             return out.transpose(2, 3) if columns else out
         k, v = buffer(), buffer()
-        kv_read_int8(self.batch, self.heads, tokens, self.dim, self.length, self.block, self.keys.data_ptr(), self.values.data_ptr(),
-                     self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), from_each, first, k.data_ptr(), v.data_ptr(), k.stride(), cur_stream())
+        cpmk.kv_read_int8(self.batch, self.heads, tokens, self.dim, self.length, self.block, self.keys.data_ptr(), self.values.data_ptr(),
+                          self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), from_each, first, k.data_ptr(), v.data_ptr(), *k.stride(),
+                          cur_stream())
         return k, v
 
     def attention(self, q: torch.Tensor, lens, scale: float = None, causal: bool = True, pos=None, mask: torch.Tensor = None,
@@ -146,8 +149,8 @@ class QuantizedKV:
         out = torch.empty_like(q)
         size = _workspace(device.index, batch, heads, self.heads, queries, dim, self.length)
         space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        kv_attention_int8(batch, heads, self.heads, queries, dim, self.length, self.block, q.data_ptr(), q.stride(), self.keys.data_ptr(),
-                          self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), lens_each, keys, pos_each, first, causal,
-                          dim ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, bidirectional, mask_ptr, mask_batch,
-                          mask_token, out.data_ptr(), out.stride(), None if space is None else space.data_ptr(), cur_stream())
+        cpmk.kv_attention_int8(batch, heads, self.heads, queries, dim, self.length, self.block, q.data_ptr(), *q.stride(), self.keys.data_ptr(),
+                          self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), lens_each, keys, pos_each, first, int(bool(causal)),
+                          dim ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, int(bool(bidirectional)), mask_ptr, mask_batch,
+                          mask_token, out.data_ptr(), *out.stride(), None if space is None else space.data_ptr(), cur_stream())
         return out
