@@ -11,6 +11,10 @@
 //
 // Work is divided over the keys too where rows are few: a workgroup takes every tile of 64 keys of its part, wave by wave, and its waves join their sums
 // through LDS; parts leave theirs in the workspace and a second kernel joins them.
+//
+// Bound by reading the cache: 32 x 64 heads of 64 units over 512 to 1024 keys (202 MB) 36 us, with nothing but the loads 34; 4 x 64 heads of 128 over 16384 to 32768, eight to a head of the
+// cache (201 MB), 42 and 39 us, and 4.7 the joining.  One matrix instruction's sixteen columns hold one query there; conversion, scores and softmax of a tile are 270 operations a wave beside the
+// 8 KB that it reads.
 #include "kv_attention.h"
 #include <algorithm>
 

@@ -10,6 +10,11 @@
 // matrix pipe meanwhile are the other workgroups of the compute unit, three of them for heads of up to 64 units, two up to 128.  One workgroup of eight waves, half of them a
 // phase behind the others, was 20 % slower with 64 units (8 x 64 heads of 512 queries over 1024 keys: 138 against 114 us) and between 3 % slower and 6 % faster with 128.
 //
+// Bound by the vector and the matrix instructions together: 32 heads of 2000 queries over 8011 keys of 128 units (230 GFLOP) take 270 to 296 us, in which a SIMD's matrix pipe is busy for 223 thousand cycles of 550 and its vector
+// instructions issue for 296 (a wave and tile: 32 products, 130 operations of the softmax, 32 of them exponentials, 96 of the conversion); a wave of each side by side reaches two thirds of the sum at
+// best.  8 x 64 heads of 512 queries over 1024 of 64 units with a position bias (52 GFLOP) 108 us.  The scores of the next tile between the exponentials of this one, in the same wave, took 329 us for 296 and
+// 144 for 110: both tiles' scores do not fit the registers beside the sums.
+//
 // LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at 129 u + 64 h + r, read along r; the odd distance spreads the eight unit steps that
 // neighbouring lanes write over the banks.  Values (group of sixteen keys g, half s, unit) at (2 g + s) D + unit.
 #include "kv_attention.h"
