@@ -341,7 +341,8 @@ static int kv_check(int32_t batch, int32_t heads, int32_t tokens, int32_t dim, i
     if (block != 16 && block != 32 && block != 64 && block != 128) return CPMK_EBADARG;
     if (dim % 16 || length % block) return CPMK_EALIGN;
     if (dim > 256 || (int64_t)length * dim > 0x7fffffffll) return CPMK_ETOOBIG;
-    return (int64_t)batch * heads == 0 || tokens == 0 || dim == 0 || length == 0 ? -1 : 0;
+    if ((int64_t)batch * heads == 0 || tokens == 0 || dim == 0) return -1;
+    return length == 0 ? CPMK_EBADARG : 0;
 }
 
 static int kv_mode(bool values, int64_t token, int64_t unit) {

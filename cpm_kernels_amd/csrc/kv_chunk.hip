@@ -144,10 +144,24 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
         if (MASK) fetch_mask(t_begin);
     }
     half8_t q[KS];
-    load_query(q, a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token, a.q_unit, a.dim, [&](int s) { return s * 16 + half * 8; });
-    if (flip)
+    {
+        // (steps of sixteen units lie in the head or behind it as a whole, and their distances are the same for all lanes: one addition a load)
+        const half_t* const p = a.q + b * a.q_batch + (int64_t)h * a.q_head + (int64_t)query * a.q_token + half * 8 * a.q_unit;
+        if (a.q_unit == 1) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = -q[s];
+            for (int s = 0; s < KS; ++s) q[s] = load_half8_any(p + min(s * 16, a.dim - 16));
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[s][e] = p[(min(s * 16, a.dim - 16) + e) * a.q_unit];
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s * 16 >= a.dim) q[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            if (flip) q[s] = -q[s];
+        }
+    }
     const int32_t lo_rel = a.first_distance - kChunkPad;
     if (BIAS)
         for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
@@ -306,22 +320,27 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
         }
         return;
     }
-    half_t* const out = a.out + b * a.out_batch + (int64_t)h * a.out_head + (int64_t)query * a.out_token;
+    half_t* const out = a.out + b * a.out_batch + (int64_t)h * a.out_head + (int64_t)query * a.out_token + half * 4 * a.out_unit;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (a.out_unit == 1) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int u = n * 32 + c * 8 + half * 4;
-            if (u >= a.dim) continue;
-            half4_t v;
+            for (int c = 0; c < 4; ++c) {
+                half4_t v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (half_t)(acc[n][c * 4 + e] * inv);
-            if (a.out_unit == 1) *reinterpret_cast<Half4Any*>(out + u) = __builtin_bit_cast(Half4Any, v);
-            else
+                for (int e = 0; e < 4; ++e) v[e] = (half_t)(acc[n][c * 4 + e] * inv);
+                if (n * 32 + c * 8 < a.dim) *reinterpret_cast<Half4Any*>(out + n * 32 + c * 8) = __builtin_bit_cast(Half4Any, v);
+            }
+    } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[(u + e) * a.out_unit] = v[e];
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (n * 32 + c * 8 < a.dim)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[(n * 32 + c * 8 + e) * a.out_unit] = (half_t)(acc[n][c * 4 + e] * inv);
+    }
 }
 
 template <int NT, bool BIAS, bool MASK>

@@ -33,6 +33,8 @@ def test_refusals_of_the_c_abi():
         for bad in (dict(d=272), dict(length=2 ** 25)):
             with pytest.raises(RuntimeError, match="limit"):
                 call(**bad)
+        with pytest.raises(RuntimeError, match="invalid argument"):         # (a cache without positions)
+            call(length=0, **(dict(len=0) if call is attend else {}))
         for empty in (dict(b=0, keys=N), dict(n=0, keys=N), dict(d=0, keys=N)):
             call(**empty)
     for bad in (dict(k=N), dict(pos=-1), dict(pos=61), dict(pos=2 ** 31 - 1)):
