@@ -281,6 +281,26 @@ def test_attention_in_parts(gpu, n, d):
     assert not bool(got[4].any())
 
 
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("n", [5, 256])
+def test_attention_of_long_parts(gpu, n, d):
+    """So many heads that a workgroup has dozens of tiles one after the other; two heads of one sequence are looked at."""
+    print("attention long parts", n, d, flush=True)
+    rng = np.random.default_rng(n + d)
+    b, h, length = 2, 128, 2688
+    cache = ct.QuantizedKV.empty(b, h, length, d, block=16)
+    k, v, q = (torch.randn((b, h, rows, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(i + d)).half() for i, rows in enumerate((length, length, n)))
+    cache.write(k, v, 0)
+    bias = _bias(rng, h, False)
+    got = cache.attention(q, 2650, **bias)
+    some = [0, 77]
+    want, bound = ok.attention(q[1:, some].cpu().numpy(), cache.keys[1:, some].cpu().numpy(), ok.by_token(cache.values[1:, some].cpu().numpy()),
+                               cache.key_absmax[1:, some].cpu().numpy(), cache.value_absmax[1:, some].cpu().numpy(), [2650], d ** -0.5, True,
+                               table=bias["bias"][some].cpu().numpy(), mapping=bias["mapping"].cpu().numpy())
+    err = np.abs(got[1:, some].cpu().numpy().astype(np.float64) - want)
+    assert (err <= bound).all(), (err / bound).max()
+
+
 @pytest.mark.parametrize("n", [1, 20, 100])
 def test_attention_of_other_scales(gpu, n):
     """A negative factor turns the order of the scores around, 0 makes the mean of the values; a large one leaves one key."""
