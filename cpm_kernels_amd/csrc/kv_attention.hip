@@ -33,7 +33,7 @@ __device__ __forceinline__ float quad_max(float m) {
 
 // DS: 64-unit steps of a head, CT: sixteens of rows, WAVES of a workgroup.
 template <int DS, int CT, int WAVES, bool BIAS, bool MASK>
-__global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAttention a) {
+__global__ __launch_bounds__(WAVES * 64, CT == 2 || DS > 2 ? 2 : DS == 2 ? 3 : 4) void k_kv_attend(KvAttention a) {
     constexpr int ROWS = CT * 16;
     __shared__ float joined[WAVES][ROWS][64 + 4];
     __shared__ float stat[WAVES][2][ROWS];
@@ -69,10 +69,11 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
     const int32_t first_at = range.pos + r_first / a.group;
     const int32_t all_see = a.causal ? min(range.len, first_at + 1) : range.len;
 
-    // A tile's operands are on their way while the one before it is multiplied.  Row r of the key operand is key 16 (r / 4) + 4 j + r % 4 of the tile, so that a
-    // lane's results are neighbours; units past the head's meet zeros of the query.
+    // A tile's values are on their way during its softmax, the next tile's keys while its values are multiplied: each in the registers that the other has just left, so that more waves
+    // fit a SIMD than with both of a tile in flight at once (heads of 256 units, 8 x 32 over 1024 keys: 45 and 33 us; of 128 21.5 and 20).  Row r of the key operand is key
+    // 16 (r / 4) + 4 j + r % 4 of the tile, so that a lane's results are neighbours; units past the head's meet zeros of the query.
     const int32_t key_row = (col >> 2) * 16 + (col & 3);
-    uint4_t kr[4 * DS], vr[4 * DS], mk[CT];
+    uint4_t raw[4 * DS], mk[CT];
     half_t kt, vt;
     // keys that one workgroup looks at are read once (with the hint: 32 x 64 heads over up to 1024 keys 40.6 -> 36.2 us)
     auto load = [&](const int8_t* p) { return CT == 1 ? __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)) : *reinterpret_cast<const uint4_t*>(p); };
@@ -83,7 +84,7 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
 #pragma unroll
             for (int d = 0; d < DS; ++d) {
                 const int u = d * 64 + quad * 16;
-                kr[j * DS + d] = load(keys + (o + (uint32_t)(u < a.dim ? u : 0)));
+                raw[j * DS + d] = load(keys + (o + (uint32_t)(u < a.dim ? u : 0)));
             }
         }
         const int32_t at = min(t * kTile + quad * 16, a.length - 16);
@@ -99,12 +100,9 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
     auto fetch_values = [&](int32_t t) {
         const uint32_t o = (uint32_t)min(t * kTile + quad * 16, a.length - 16) * (uint32_t)a.dim + col * 16;
 #pragma unroll
-        for (int d = 0; d < 4 * DS; ++d) vr[d] = load(values + (o + (uint32_t)(d * 16 < a.dim ? d * 256 : 0)));
+        for (int d = 0; d < 4 * DS; ++d) raw[d] = load(values + (o + (uint32_t)(d * 16 < a.dim ? d * 256 : 0)));
     };
-    if (t_begin + wave < t_end) {
-        fetch_keys(t_begin + wave);
-        fetch_values(t_begin + wave);
-    }
+    if (t_begin + wave < t_end) fetch_keys(t_begin + wave);
     half8_t q[CT][2 * DS];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -145,7 +143,7 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
 #pragma unroll
             for (int d = 0; d < DS; ++d) {
                 half8_t lo, hi;
-                halves_of(kr[j * DS + d], lo, hi);
+                halves_of(raw[j * DS + d], lo, hi);
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     s[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, q[c][2 * d], s[c][j], 0, 0, 0);
@@ -154,11 +152,7 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
             }
         }
         const float factor = (float)kt * (1.0f / 127.0f) * a.scale, vs = kv_scale(vt), add = __builtin_amdgcn_logf(vs), inverse = __builtin_amdgcn_rcpf(vs);
-        uint4_t keep[CT];
-        if (MASK)
-#pragma unroll
-            for (int c = 0; c < CT; ++c) keep[c] = mk[c];
-        if (t + WAVES < t_end) fetch_keys(t + WAVES);
+        fetch_values(t);
         half8_t p[CT][2];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -184,7 +178,7 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
             }
             if (MASK)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = (keep[c][j >> 2] >> ((j & 3) * 8) & 0xffu) ? x[j] : -__builtin_inff();
+                for (int j = 0; j < 16; ++j) x[j] = (mk[c][j >> 2] >> ((j & 3) * 8) & 0xffu) ? x[j] : -__builtin_inff();
             float m = x[0];
 #pragma unroll
             for (int j = 1; j < 16; ++j) m = fmaxf(m, x[j]);
@@ -210,14 +204,14 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : 1) void k_kv_attend(KvAtt
 #pragma unroll
         for (int d = 0; d < 4 * DS; ++d) {
             half8_t lo, hi;
-            halves_of(vr[d], lo, hi);
+            halves_of(raw[d], lo, hi);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[c][0], acc[c][d], 0, 0, 0);
                 acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][1], acc[c][d], 0, 0, 0);
             }
         }
-        if (t + WAVES < t_end) fetch_values(t + WAVES);
+        if (t + WAVES < t_end) fetch_keys(t + WAVES);
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -321,7 +315,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
 //   Up to 64 queries on k_kv_attend, more on k_kv_chunk: 32 heads over 1024 (8 sequences) and 8192 keys (one), us, the one and the other: 33 queries of 64 units 21.6, 25.3 and 25.4, 29.7,
 //   64 22.1, 26.0 and 25.8, 30.3, 96 26.7, 31.6 and 26.6, 32.1; of 128 units 33 31.7, 34.0 and 33.1, 37.3, 64 32.4, 35.1 and 34.0, 38.8, 96 43.1, 43.7 and 36.0, 41.8.
 //   Workgroups of eight waves where they are few (8 x 32 heads of 64 units over 3000 keys: 28 us in fours, 24 in eights), of four where there are two to a compute unit anyway (32 x 64 over up to 1024: 36 and
-//   40); heads of more than 128 units need more registers than eight waves have.
+//   40).
 //   Parts as long as all workgroups run at once, never more: a second round costs what a first does (4 x 64 heads over up to 32768 keys, eight to a head of the cache, in workgroups of four waves: two
 //   a compute unit 45 us, four 46, sixteen 63 and the joining 6, 9, 22).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads over 1024 keys in one part 26.6 us, in two 45.2).
 struct KvPlan {
@@ -334,7 +328,7 @@ static KvPlan kv_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens
     p.rows = p.chunks ? kChunkRows : tokens * (heads / held) > 16 && dim <= 128 ? 32 : 16;
     p.row_tiles = (int)ceil_div(p.chunks ? tokens : tokens * (heads / held), p.rows);
     const int64_t base = batch * (p.chunks ? heads : held) * p.row_tiles, tiles = ceil_div(length, kTile), units = compute_units();
-    p.waves = dim <= 128 && base < 2 * units ? 8 : 4;
+    p.waves = base < 2 * units ? 8 : 4;
     const int64_t splits = p.chunks ? std::max(std::min(2 * units / base, tiles / 16), std::min(units / base, tiles / kChunkLeast)) : std::min(8 / p.waves * units / base, tiles / p.waves);
     p.splits = (int)std::max<int64_t>(1, splits);
     return p;
@@ -414,7 +408,7 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     if (plan.chunks) e = kv_chunk_launch(a, batch, st);
     else if (plan.rows == 32) e = dim <= 64 ? kv_launch<1, 2>(a, plan.waves, g, st) : kv_launch<2, 2>(a, plan.waves, g, st);
     else if (dim <= 128) e = dim <= 64 ? kv_launch<1, 1>(a, plan.waves, g, st) : kv_launch<2, 1>(a, plan.waves, g, st);
-    else e = dim <= 192 ? kv_launch<3, 1, 4>(a, g, st) : kv_launch<4, 1, 4>(a, g, st);
+    else e = dim <= 192 ? kv_launch<3, 1>(a, plan.waves, g, st) : kv_launch<4, 1>(a, plan.waves, g, st);
     if (e) return e;
     if (a.splits > 1)
         hipLaunchKernelGGL(k_kv_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan.rows, (int)plan.chunks, plan.chunks ? kChunkLeast : plan.waves,
