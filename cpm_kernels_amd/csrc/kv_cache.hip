@@ -205,7 +205,7 @@ __device__ __forceinline__ void write_token(const KvArgs& a, const KvSide& s, in
 #pragma unroll
     for (int c = 0; c < 4; ++c)
         if (c * 64 + lane < a.dim) at[(c * 64 + lane) * (V ? 16 : 1)] = (int8_t)nearest_bits((float)v[c] * y);
-    if (m == old) return;
+    if (m == old && first < pos) return;         // (at a block's start what the magnitude was does not count, not even where it is 0 now)
     if (lane == 0) *top = __builtin_bit_cast(half_t, (uint16_t)m);
     if (first == pos) return;
     const float again = (float)__builtin_bit_cast(half_t, (uint16_t)old) / now * kUp;

@@ -135,6 +135,23 @@ def test_write_of_extreme_values(gpu, n, pos):
     both.check()
 
 
+@pytest.mark.parametrize("n", [1, 3])
+def test_write_of_zeros_over_other_tokens(gpu, n):
+    """Zeros (and what counts as zero) at a block's start leave the block the magnitude 0, whatever it held: the tokens behind them are rounded by their own."""
+    print("write zeros", n, flush=True)
+    rng = np.random.default_rng(n)
+    both = _Both(rng, 2, 2, 64, 32, 16)
+    x = np.zeros((2, 2, n, 32), np.float16)
+    x[1] = np.nan
+    t = torch.from_numpy(x).cuda()
+    for pos in (16, 48):
+        both.write((x, t), (x, t), pos)
+    both.check()
+    for i in range(2):
+        both.write(_tokens(rng, 2, 2, 1, 32, "rows", 1e-3), _tokens(rng, 2, 2, 1, 32, "rows", 1e-3), 16 + n + i)
+    both.check()
+
+
 READS = [(1, 1, 1, 16, 16, 16, 0), (2, 3, 101, 80, 256, 32, 13), (1, 2, 256, 64, 256, 64, 0), (2, 1, 300, 128, 256, 64, -20), (1, 1, 64, 256, 128, 128, 31),
          (1, 1, 5, 64, 64, 16, 70), (1, 1, 5, 64, 64, 16, -9), (2, 2, 33, 240, 96, 32, 16)]
 
