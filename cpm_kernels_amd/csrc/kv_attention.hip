@@ -13,7 +13,7 @@
 // through LDS; parts leave theirs in the workspace and a second kernel joins them.
 //
 // Bound by reading the cache: 32 x 64 heads of 64 units over 512 to 1024 keys (202 MB) 36 us, with nothing but the loads 34; 4 x 64 heads of 128 over 16384 to 32768, eight to a head of the
-// cache (201 MB), 42 and 39 us, and 4.7 the joining.  One matrix instruction's sixteen columns hold one query there; conversion, scores and softmax of a tile are 270 operations a wave beside the
+// cache (201 MB), 41 and 39 us, and 4.7 the joining.  One matrix instruction's sixteen columns hold one query there; conversion, scores and softmax of a tile are 270 operations a wave beside the
 // 8 KB that it reads.
 #include "kv_attention.h"
 #include <algorithm>
@@ -70,12 +70,12 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 || DS > 2 ? 2 : DS == 2 ? 3 : 4
     const int32_t all_see = a.causal ? min(range.len, first_at + 1) : range.len;
 
     // A tile's values are on their way during its softmax, the next tile's keys while its values are multiplied: each in the registers that the other has just left, so that more waves
-    // fit a SIMD than with both of a tile in flight at once (heads of 256 units, 8 x 32 over 1024 keys: 45 and 33 us; of 128 21.5 and 20).  Row r of the key operand is key
+    // fit a SIMD than with both of a tile in flight at once (8 x 32 heads of 256 units over 1024 keys: 33 us for 45, of 128 20 for 21.5).  Row r of the key operand is key
     // 16 (r / 4) + 4 j + r % 4 of the tile, so that a lane's results are neighbours; units past the head's meet zeros of the query.
     const int32_t key_row = (col >> 2) * 16 + (col & 3);
     uint4_t raw[4 * DS], mk[CT];
     half_t kt, vt;
-    // keys that one workgroup looks at are read once (with the hint: 32 x 64 heads over up to 1024 keys 40.6 -> 36.2 us)
+    // keys that one workgroup looks at are read once (32 x 64 heads over up to 1024 keys 36 us for 42, 4 x 64 of 128 over up to 32768 41 for 44.5)
     auto load = [&](const int8_t* p) { return CT == 1 ? __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)) : *reinterpret_cast<const uint4_t*>(p); };
     auto fetch_keys = [&](int32_t t) {
 #pragma unroll
@@ -312,12 +312,14 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttention a, int rows, int ch
 }
 
 // Which kernel a call takes, and into how many parts its keys are cut.
-//   Up to 64 queries on k_kv_attend, more on k_kv_chunk: 32 heads over 1024 (8 sequences) and 8192 keys (one), us, the one and the other: 33 queries of 64 units 21.6, 25.3 and 25.4, 29.7,
-//   64 22.1, 26.0 and 25.8, 30.3, 96 26.7, 31.6 and 26.6, 32.1; of 128 units 33 31.7, 34.0 and 33.1, 37.3, 64 32.4, 35.1 and 34.0, 38.8, 96 43.1, 43.7 and 36.0, 41.8.
-//   Workgroups of eight waves where they are few (8 x 32 heads of 64 units over 3000 keys: 28 us in fours, 24 in eights), of four where there are two to a compute unit anyway (32 x 64 over up to 1024: 36 and
-//   40).
-//   Parts as long as all workgroups run at once, never more: a second round costs what a first does (4 x 64 heads over up to 32768 keys, eight to a head of the cache, in workgroups of four waves: two
-//   a compute unit 45 us, four 46, sixteen 63 and the joining 6, 9, 22).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads over 1024 keys in one part 26.6 us, in two 45.2).
+//   Up to 64 queries on k_kv_attend, more on k_kv_chunk: 32 heads over 1024 (8 sequences) and 8192 keys (one), us, the one and the other: 33 queries of 64 units 21.4, 24.5 and 25.4, 29.7,
+//   64 21.5, 24.7 and 25.8, 30.3, 96 26.2, 32.9 and 26.6, 32.1; of 128 units 33 31.3, 32.4 and 33.1, 37.3, 64 31.9, 33.2 and 34.0, 38.8, 96 42.9, 44.3 and 36.0, 41.8; of 256 units 33 67.2,
+//   79.4 and 73.3, 78.8, 64 84.8, 81.7 and 75.1, 81.4, 96 112, 122 and 77.4, 85.0.
+//   Workgroups of eight waves where there are fewer than two to a compute unit (8 x 32 heads over 1024 keys, in fours and eights: 64 units 17.2 and 14.2 us, 128 24.0 and 20.0, 256 36.9 and 32.9), of
+//   four elsewhere (16 x 32 heads of 256 53 and 57, 32 x 64 of 64 over up to 1024 36 and 38).
+//   Parts as long as all workgroups run at once, one a compute unit of eight waves, two of four: with twice as many the joining grows by more than the reading shrinks (4 x 64 heads on 8 of 256
+//   units over up to 16384 keys 58 us, with twice the parts 65; 32 on 8 of 128 over up to 65536 38 and 43).  Chunks: one a compute unit, two where the parts keep 16 tiles (96 queries, 8 x 32 heads
+//   over 1024 keys in one part 26.6 us, in two 45.2).
 struct KvPlan {
     int rows, row_tiles, splits, waves;
     bool chunks;

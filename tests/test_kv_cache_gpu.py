@@ -342,6 +342,56 @@ def test_attention_with_bias_tables_of_any_size(gpu, n, group, buckets, distance
     _attend(rng, 1, group, group, n, 64, 1472, 64, 1450, **bias)
 
 
+@pytest.mark.parametrize("n,d,group", [(1, 64, 1), (1, 128, 1), (1, 192, 1), (1, 256, 2), (3, 128, 8), (20, 64, 1), (20, 112, 1), (70, 64, 1)])
+def test_attention_of_many_heads(gpu, n, d, group):
+    """More heads than compute units, a position bias and a mask: what few heads share among more waves or workgroups, each here does by itself."""
+    print("attention many heads", n, d, group, flush=True)
+    rng = np.random.default_rng(n + d)
+    b, h = 8 * group, 72
+    lens = _ints(([0, 1, 130, 64, 190, 77, 192, 100] * group)[:b])
+    _attend(rng, b, h, group, n, d, 192, 32, lens)
+    mask = torch.from_numpy(rng.random((b, n, 192)) < 0.6).cuda()
+    mask[4] = False
+    _, _, got = _attend(rng, b, h, group, n, d, 192, 64, lens, mask=mask, **_bias(rng, h, True))
+    assert not bool(got[4].any())
+
+
+@pytest.mark.parametrize("n,d", [(1, 64), (5, 256), (40, 128), (100, 64)])
+def test_attention_with_biases_of_minus_infinity(gpu, n, d):
+    """Keys at distances whose bias is -inf do not count: single ones, whole tiles, all keys behind the table's end."""
+    print("attention biases of -inf", n, d, flush=True)
+    rng = np.random.default_rng(n + d)
+    mapping = (np.arange(128) // 4).astype(np.int32)
+    table = rng.standard_normal((2, 32)).astype(np.float16)
+    both = _Both(rng, 2, 2, 640, d, 64)
+    q = _tokens(rng, 2, 2, n, d, "rows")
+    lens = np.array([600, 95])
+    for without in ([5], [31], list(range(8, 32)), [0, 31]):
+        bias = table.copy()
+        bias[:, without] = -np.inf
+        distance = np.clip((lens[:, None] - n + np.arange(n))[:, :, None] - np.arange(640), 0, 127)
+        want, bound = ok.attention(q[0], both.k, both.v, both.ka, both.va, lens, d ** -0.5, True, mask=~np.isin(mapping[distance], without), table=table, mapping=mapping)
+        got = both.cache.attention(q[1], _ints(lens), bias=torch.from_numpy(bias).cuda(), mapping=torch.from_numpy(mapping).cuda())
+        err = np.abs(got.cpu().numpy().astype(np.float64) - want)
+        assert (err <= bound).all(), (without, (err / np.maximum(bound, 1e-30)).max())
+
+
+@pytest.mark.parametrize("n,d", [(2, 64), (18, 128), (4, 256), (100, 64), (130, 128)])
+def test_attention_of_queries_that_are_no_numbers(gpu, n, d):
+    """A query with a NaN or an infinity gives NaN for itself; those beside it are as they were."""
+    print("attention no numbers", n, d, flush=True)
+    rng = np.random.default_rng(n + d)
+    both = _Both(rng, 2, 4, 384, d, 64)
+    q = _tokens(rng, 2, 8, n, d, "rows")
+    want, bound = ok.attention(q[0], both.k, both.v, both.ka, both.va, [380, 131], d ** -0.5, True)
+    q[1][0, 3, n // 2, 7] = float("nan")
+    q[1][1, 0, 0, 0] = float("inf")
+    got = both.cache.attention(q[1], _ints([380, 131])).cpu().numpy().astype(np.float64)
+    assert np.isnan(got[0, 3, n // 2]).all() and np.isnan(got[1, 0, 0]).any()
+    got[0, 3, n // 2], got[1, 0, 0] = want[0, 3, n // 2], want[1, 0, 0]
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_attention_beside_magnitudes_far_apart(gpu):
     """Blocks of values 2^20 times as large as others, in and out of sight, and blocks of zeros: probabilities keep their bits."""
     print("attention magnitudes", flush=True)
