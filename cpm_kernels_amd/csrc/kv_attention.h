@@ -49,12 +49,11 @@ __device__ __forceinline__ KvRange kv_range(const KvAttention& a, int64_t b, int
     return r;
 }
 
-// The biases of a head over the distances first .. first + count - 1, in units of log2, to LDS: entry i is that of distance first + i, those off the table's ends
-// at its ends.
-__device__ __forceinline__ float kv_bias(const KvAttention& a, int32_t head, int32_t rel) {
-    rel = max(a.first_distance, min(rel, a.distances - 1));
-    const int32_t bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
-    return (float)a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))] * kLog2e;
+// The bias of a head at a distance first_distance .. distances - 1 (others are as those at the ends).  With biases for both signs first_distance is -1 at least, where the table has
+// one distance only: a key behind the query takes the upper half of the buckets however short the table is.
+__device__ __forceinline__ half_t kv_bias(const KvAttention& a, int32_t head, int32_t rel) {
+    const int32_t bucket = a.mapping[min(abs(rel), a.distances - 1)] + (rel < 0 ? a.buckets / 2 : 0);
+    return a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))];
 }
 
 // Workgroup x of units * inner ones: the `inner` workgroups of a unit, which read the same keys, follow one another on one XCD, and units are dealt to the XCDs in turn (of sequences of

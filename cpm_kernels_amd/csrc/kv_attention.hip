@@ -116,8 +116,7 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 || DS > 2 ? 2 : DS == 2 ? 3 : 4
         for (int i = tid; i < slots * entries; i += WAVES * 64) {
             const int slot = i / entries, rel = i - slot * entries + a.first_distance;
             const int head = kvh * a.group + (a.group <= ROWS ? slot : (r_first + slot) % a.group);
-            const int bucket = a.mapping[rel < 0 ? -rel : rel] + (rel < 0 ? a.buckets / 2 : 0);
-            table[i] = a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))];
+            table[i] = kv_bias(a, head, rel);
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c) biases[c] = table + (a.group <= ROWS ? g[c] : c * 16 + col) * entries - a.first_distance;
@@ -393,7 +392,7 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     a.keys = (const int8_t*)keys, a.values = (const int8_t*)values, a.key_top = (const half_t*)key_absmax, a.value_top = (const half_t*)value_absmax;
     a.lens_each = (const int32_t*)lens_each, a.pos_each = (const int32_t*)pos_each, a.len = len, a.pos = pos;
     a.table = (const half_t*)bias, a.mapping = (const int32_t*)mapping, a.buckets = num_buckets, a.distances = max_distance;
-    a.first_distance = bidirectional ? 1 - max_distance : 0;
+    a.first_distance = bidirectional ? std::min(1 - max_distance, -1) : 0;
     a.mask = (const uint8_t*)mask, a.mask_batch = mask_batch, a.mask_token = mask_token;
     a.out = (half_t*)out, a.out_batch = out_batch, a.out_head = out_head, a.out_token = out_token, a.out_unit = out_unit;
     a.parts = (float*)workspace, a.scale = scale * kLog2e, a.causal = causal != 0;

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
     }
     const int32_t lo_rel = a.first_distance - kChunkPad;
     if (BIAS)
-        for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = kv_bias(a, h, i + lo_rel);
+        for (int i = tid; i < a.distances - a.first_distance + 2 * kChunkPad; i += NTHR) biases[i] = (float)kv_bias(a, h, max(a.first_distance, min(i + lo_rel, a.distances - 1))) * kLog2e;
 
     if (t_begin < t_end) {
         if (a.dim < D) {        // (units past the head's: zeros)

@@ -342,6 +342,20 @@ def test_attention_with_bias_tables_of_any_size(gpu, n, group, buckets, distance
     _attend(rng, 1, group, group, n, 64, 1472, 64, 1450, **bias)
 
 
+@pytest.mark.parametrize("buckets,distances", [(4, 1), (2, 1), (1, 1), (4, 2)])
+@pytest.mark.parametrize("n,group,d", [(1, 1, 64), (1, 20, 64), (9, 4, 128), (33, 2, 64), (5, 1, 256), (70, 1, 64), (150, 2, 128), (100, 1, 256)])
+def test_attention_with_two_sided_bias_tables_of_few_distances(gpu, n, group, d, buckets, distances):
+    """One bias for all keys up to a query's position and one for all behind it (or three): queries before the first key, among the keys, in the last of them."""
+    print("attention two-sided tables", n, group, d, buckets, distances, flush=True)
+    rng = np.random.default_rng(n + buckets)
+    mapping = torch.from_numpy(np.arange(distances).astype(np.int32) % max(buckets // 2, 1)).cuda()
+    bias = dict(bias=torch.from_numpy(rng.standard_normal((group, buckets)).astype(np.float16)).cuda(), mapping=mapping, bidirectional=True)
+    for pos in (-n // 2, 700, 1440 - n):
+        _attend(rng, 1, group, group, n, d, 1472, 64, 1450, causal=False, pos=_ints([pos]), **bias)
+    _attend(rng, 1, group, group, n, d, 1472, 64, 1450, **bias)
+    _attend(rng, 1, group, group, n, d, 192, 32, 131, causal=False, pos=60, **bias)
+
+
 @pytest.mark.parametrize("n,d,group", [(1, 64, 1), (1, 128, 1), (1, 192, 1), (1, 256, 2), (3, 128, 8), (20, 64, 1), (20, 112, 1), (70, 64, 1)])
 def test_attention_of_many_heads(gpu, n, d, group):
     """More heads than compute units, a position bias and a mask: what few heads share among more waves or workgroups, each here does by itself."""
