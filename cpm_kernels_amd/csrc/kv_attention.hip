@@ -364,7 +364,7 @@ extern "C" {
 
 int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length) {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || dim <= 0 || length <= 0 || heads % kv_heads) return 0;
-    if ((int64_t)tokens * (heads / kv_heads) > kFar) return 0;
+    if ((int64_t)tokens * (heads / kv_heads) > kFar || !grid_fits((int64_t)batch * heads)) return 0;
     const KvPlan p = kv_plan(batch, heads, kv_heads, tokens, dim, length);
     return p.splits > 1 ? (int64_t)batch * (p.chunks ? heads : kv_heads) * p.row_tiles * p.splits * p.rows * (dim + 2) * (int64_t)sizeof(float) : 0;
 }
@@ -379,7 +379,8 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
     if (batch < 0 || heads < 0 || kv_heads < 0 || tokens < 0 || dim < 0 || length < 0) return CPMK_EBADARG;
     if (block != 16 && block != 32 && block != 64 && block != 128) return CPMK_EBADARG;
     if (dim % 16 || length % block) return CPMK_EALIGN;
-    if ((int64_t)batch * heads * tokens * dim == 0) return 0;
+    if (batch == 0 || heads == 0 || tokens == 0 || dim == 0) return 0;
+    if (!grid_fits((int64_t)batch * heads)) return CPMK_ETOOBIG;         // (a row each at least; what is multiplied by it below stays below 2^63)
     if (kv_heads == 0 || heads % kv_heads || length == 0) return CPMK_EBADARG;
     if (any_null(q, keys, values, key_absmax, value_absmax, out)) return CPMK_EBADARG;
     if (!lens_each && (len < 0 || len > length)) return CPMK_EBADARG;

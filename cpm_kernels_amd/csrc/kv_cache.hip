@@ -342,6 +342,7 @@ static int kv_check(int32_t batch, int32_t heads, int32_t tokens, int32_t dim, i
     if (dim % 16 || length % block) return CPMK_EALIGN;
     if (dim > 256 || (int64_t)length * dim > 0x7fffffffll) return CPMK_ETOOBIG;
     if ((int64_t)batch * heads == 0 || tokens == 0 || dim == 0) return -1;
+    if (!grid_fits((int64_t)batch * heads)) return CPMK_ETOOBIG;         // (two workgroups a head at least; what is multiplied by it below stays below 2^63)
     return length == 0 ? CPMK_EBADARG : 0;
 }
 

@@ -50,6 +50,27 @@ def test_refusals_of_the_c_abi():
     assert cpmk.kv_attention_int8_workspace(0, 4, 4, 1, 64, 64) == 0 and cpmk.kv_attention_int8_workspace(1, 4, 3, 1, 64, 64) == 0
 
 
+def test_refusals_of_sizes_whose_products_leave_64_bits():
+    """A product of sizes that comes round to 0 is neither an empty call nor a small grid."""
+    from cpm_kernels_amd.library import cpmk
+    big = 2 ** 30
+
+    def refused(call, *args):
+        with pytest.raises(RuntimeError, match="limit"):
+            call(*args)
+    p = 16
+    refused(cpmk.kv_attention_int8, 2 ** 18, 2 ** 18, 2 ** 18, 2 ** 20, 256, 64, 16, p, *S, p, p, p, p, N, 8, N, -1, 1, 0.125, N, N, 0, 0, 0, N, 0, 0, p, *S, p, N)
+    refused(cpmk.kv_attention_int8, big, big, big, 16, 64, 64, 16, p, *S, p, p, p, p, N, 8, N, -1, 1, 0.125, N, N, 0, 0, 0, N, 0, 0, p, *S, p, N)
+    for tokens in (1, 2048, 4096):
+        refused(cpmk.kv_write_int8, big, big, tokens, 64, 4096, 16, p, *S, p, *S, N, 0, N, p, p, p, p, N)
+        refused(cpmk.kv_read_int8, big, big, tokens, 64, 4096, 16, p, p, p, p, N, 0, p, p, *S, N)
+    assert cpmk.kv_attention_int8_workspace(big, big, big, 16, 64, 64) == 0
+    assert cpmk.kv_attention_int8_workspace(2 ** 18, 2 ** 18, 2 ** 18, 2 ** 20, 256, 64) == 0
+    # (no work is no work whatever the other sizes are)
+    cpmk.kv_attention_int8(big, big, big, 0, 64, 64, 16, N, *S, N, N, N, N, N, 8, N, -1, 1, 0.125, N, N, 0, 0, 0, N, 0, 0, N, *S, N, N)
+    cpmk.kv_write_int8(big, big, 0, 64, 4096, 16, N, *S, N, *S, N, 0, N, N, N, N, N, N)
+
+
 def test_oracle_of_the_cache():
     """Ties away from zero, older integers rounded again, what lies behind a write untouched."""
     ints, top = np.full((1, 1, 32, 16), 9, np.int8), np.zeros((1, 1, 2), np.float16)
