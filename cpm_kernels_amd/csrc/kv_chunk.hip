@@ -305,6 +305,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
     sum += __shfl_xor(sum, 32);
     if (q_first + col >= a.tokens) return;
     if (a.splits > 1) {
+        struct __attribute__((packed, aligned(4))) Float4Any { float x, y, z, w; };         // (a workspace is aligned to 4 bytes)
         float* const part = a.parts + (tile_of * a.splits + split) * ROWS * (a.dim + 2);
         const int r = wave * 32 + col;
 #pragma unroll
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int u = n * 32 + c * 8 + half * 4;
-                if (u < a.dim) *reinterpret_cast<float4_t*>(part + r * a.dim + u) = float4_t{acc[n][c * 4], acc[n][c * 4 + 1], acc[n][c * 4 + 2], acc[n][c * 4 + 3]};
+                if (u < a.dim) *reinterpret_cast<Float4Any*>(part + r * a.dim + u) = Float4Any{acc[n][c * 4], acc[n][c * 4 + 1], acc[n][c * 4 + 2], acc[n][c * 4 + 3]};
             }
         if (half == 0) {
             part[ROWS * a.dim + r] = top;

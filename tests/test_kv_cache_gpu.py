@@ -498,6 +498,27 @@ def test_captured_steps(gpu):
         lens += 1
 
 
+@pytest.mark.parametrize("n,d", [(3, 64), (40, 128), (100, 64), (100, 128), (100, 256)])
+def test_workspaces_off_16_byte_boundaries(gpu, n, d):
+    """A workspace starts at any multiple of 4 bytes; what lies around it stays as it is."""
+    print("workspaces", n, d, flush=True)
+    rng = np.random.default_rng(n + d)
+    b, h, length, block = 2, 2, 2048, 64
+    both = _Both(rng, b, h, length, d, block)
+    c, q = both.cache, _tokens(rng, b, h, n, d, "rows")[1]
+    want = c.attention(q, 2000)
+    size = ck.kv_attention_int8_workspace(b, h, h, n, d, length) // 4
+    assert size > 0
+    for first in (0, 1, 2, 3):
+        space = torch.full((size + 8,), 7.0, dtype=torch.float32, device="cuda")
+        assert space.data_ptr() % 16 == 0
+        out = torch.empty_like(q)
+        ck.kv_attention_int8(b, h, h, n, d, length, block, q.data_ptr(), q.stride(), c.keys.data_ptr(), c.values.data_ptr(), c.key_absmax.data_ptr(), c.value_absmax.data_ptr(),
+                             None, 2000, None, -1, True, d ** -0.5, None, None, 0, 0, False, None, 0, 0, out.data_ptr(), out.stride(), space.data_ptr() + 4 * first,
+                             torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out, want) and bool((space[:first] == 7).all()) and bool((space[first + size:] == 7).all())
+
+
 def test_calls_on_two_streams(gpu):
     """Results do not depend on what runs beside them, and come out the same every time."""
     print("two streams", flush=True)
