@@ -151,6 +151,6 @@ class QuantizedKV:
         space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         cpmk.kv_attention_int8(batch, heads, self.heads, queries, dim, self.length, self.block, q.data_ptr(), *q.stride(), self.keys.data_ptr(),
                           self.values.data_ptr(), self.key_absmax.data_ptr(), self.value_absmax.data_ptr(), lens_each, keys, pos_each, first, int(bool(causal)),
-                          dim ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, int(bool(bidirectional)), mask_ptr, mask_batch,
+                          max(dim, 1) ** -0.5 if scale is None else scale, bias_ptr, mapping_ptr, buckets, distances, int(bool(bidirectional)), mask_ptr, mask_batch,
                           mask_token, out.data_ptr(), *out.stride(), None if space is None else space.data_ptr(), cur_stream())
         return out

@@ -579,6 +579,16 @@ def test_empty_calls(gpu):
     assert not bool(cache.attention(torch.ones((2, 8, 3, 64), dtype=torch.half, device="cuda"), 0).any())
 
 
+def test_heads_without_units(gpu):
+    """A cache of heads without units takes and gives empty tensors."""
+    cache = ct.QuantizedKV.empty(2, 3, 64, 0)
+    x = torch.empty((2, 3, 5, 0), dtype=torch.half, device="cuda")
+    cache.write(x, x, 7)
+    assert cache.read(0, 9)[1].shape == (2, 3, 9, 0)
+    for kw in ({}, dict(scale=1.0), dict(lens=_ints([3, 9]))):
+        assert cache.attention(x, kw.pop("lens", 12), **kw).shape == x.shape
+
+
 def test_refusals(gpu):
     half = dict(dtype=torch.half, device="cuda")
     cache = ct.QuantizedKV.empty(2, 2, 100, 64, block=32)
