@@ -13,14 +13,21 @@ in, and a result for such queries has the same layout in memory.
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from ..kernels.kv_cache import BLOCKS
 from ..library import cpmk          # (the launchers themselves: what the kernels layer checks is checked here, and a layer of forty arguments costs 1 us)
 from ._common import cur_stream, _device
 
 
+def _check_gradients(x: torch.Tensor):
+    assert not (x.requires_grad and torch.is_grad_enabled()), "the cache keeps no gradients"
+    # (no level of forward mode is entered, as a rule, and none is a look at one number; tangents count under no_grad too)
+    assert getattr(forward_ad, "_current_level", 0) < 0 or forward_ad.unpack_dual(x).tangent is None, "the cache keeps no gradients, nor those of forward mode"
+
+
 def _check_tokens(x: torch.Tensor, device):
     assert x.dtype == torch.float16 and x.device == device
-    assert not (x.requires_grad and torch.is_grad_enabled()), "the cache keeps no gradients"
+    _check_gradients(x)
 
 
 @lru_cache(maxsize=1024)
@@ -144,7 +151,7 @@ class QuantizedKV:
         if bias is not None:
             assert bias.dtype == torch.float16 and bias.ndim == 2 and bias.size(0) == heads and bias.is_contiguous() and bias.device == device
             assert mapping is not None and mapping.dtype == torch.int32 and mapping.ndim == 1 and mapping.is_contiguous() and mapping.device == device
-            assert not (bias.requires_grad and torch.is_grad_enabled()), "the cache keeps no gradients"
+            _check_gradients(bias)
             bias_ptr, mapping_ptr, buckets, distances = bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0)
         out = torch.empty_like(q)
         size = _workspace(device.index, batch, heads, self.heads, queries, dim, self.length)

@@ -3,6 +3,7 @@ derives from the roundings on the way.  Its rounding of integers is checked for 
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 import cpm_kernels_amd.kernels as ck
 import cpm_kernels_amd.torch as ct
@@ -587,6 +588,23 @@ def test_heads_without_units(gpu):
     assert cache.read(0, 9)[1].shape == (2, 3, 9, 0)
     for kw in ({}, dict(scale=1.0), dict(lens=_ints([3, 9]))):
         assert cache.attention(x, kw.pop("lens", 12), **kw).shape == x.shape
+
+
+def test_tangents_are_refused(gpu):
+    """Forward-mode tangents would be lost as silently as gradients."""
+    half = dict(dtype=torch.half, device="cuda")
+    cache = ct.QuantizedKV.empty(2, 2, 64, 64)
+    x, bias = torch.ones((2, 2, 5, 64), **half), torch.ones((2, 32), **half)
+    mapping = torch.zeros(128, dtype=torch.int32, device="cuda")
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: cache.write(dual, x, 0), lambda: cache.write(x, dual, 0), lambda: cache.attention(dual, 5),
+                     lambda: cache.attention(x, 5, bias=fw.make_dual(bias, bias), mapping=mapping)):
+            with pytest.raises(AssertionError, match="gradients"):
+                call()
+        cache.write(x, x, 0)
+        assert bool((cache.attention(x, 5, bias=bias, mapping=mapping) == 1).all())
+    assert cache.attention(dual, 5).shape == x.shape
 
 
 def test_refusals(gpu):
