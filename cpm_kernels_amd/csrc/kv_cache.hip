@@ -6,10 +6,7 @@
 // An infinity counts as +-65504, a NaN as 0: one bad element would take its block with it.  A write that begins inside a block meets the older tokens of its sequence there: the
 // block's magnitude becomes a' = max(a, max |new x|) and the older integers q' = round(q a / a').  Bytes behind the last token that is written stay as they are.
 //
-// One product and one addition an element give the rounded quotient.  127 x / a (and q a / a') has numerator and denominator of at most 18 and 11 bits
-// beside powers of two, so it lies exactly half-way between two integers or is off that point by at least 1 / (2 * 127 * 2047) = 2^-19 of its
-// size.  y = (127 / a) (1 + 2^-21), rounded, is within 2^-22.4 of what it should be, the product too: halves come out above the half-way point by 2^-23 at
-// least, everything else stays on its side (tests/native/kv_round_check.c: every pair).
+// One fused product and addition an element gives the rounded quotient (kv_round.h; tests/native/kv_round_fma_check.cpp goes through every pair with that header's own functions).
 //
 // Storage: keys (batch, heads, length, dim), values (batch, heads, length / 16, dim, 16): what the attention reads as matrix operands is 16 contiguous
 // bytes in both, sixteen units of a token and sixteen tokens of a unit.  Such a run is the "minor" axis here, and a lane takes a piece of 4 (major) x 16 (minor) elements:
@@ -20,6 +17,7 @@
 // kept, 85 registers for 124, the same took 24 us and ragged prompts 27 instead of 15.6.  Reading 16 x 64 x 1024 (403 MB) takes 85 us, 4.7 TB/s: the hint for data that is not read again changes neither loads nor
 // stores (83 to 87), nor do rows of 256 or 512 bytes a wave instead of 128 (82 to 87).
 #include "kv_ints.h"
+#include "kv_round.h"
 
 namespace cpmk {
 
@@ -61,13 +59,12 @@ __device__ __forceinline__ void piece_of(int idx, int dim, int apart, bool neigh
     }
 }
 
-// A product's nearest integer, halves (which the factor has moved up) away from zero: its low byte in the low byte of the bits.
-__device__ __forceinline__ uint32_t nearest_bits(float q) {
-    float t = q + 12582912.0f;          // 1.5 * 2^23
+// The nearest integer of x times a factor of kv_factor, halves away from zero: its low byte in the low byte of the bits.
+__device__ __forceinline__ uint32_t nearest_bits(float x, float factor) {
+    float t = kv_shifted(x, factor);
     asm("" : "+v"(t));
     return __builtin_bit_cast(uint32_t, t);
 }
-constexpr float kUp = 1.0f + 0x1p-21f;
 
 template <bool V>
 __device__ __forceinline__ void write_piece(const KvArgs& a, const KvSide& s, uint32_t* tops, int64_t b, int32_t h, int32_t first, int32_t pos, int32_t end) {
@@ -148,8 +145,8 @@ __device__ __forceinline__ void write_piece(const KvArgs& a, const KvSide& s, ui
     if (!some) return;
     const float now = (float)__builtin_bit_cast(half_t, (uint16_t)tops[slot]);
     const float was = (float)__builtin_bit_cast(half_t, (uint16_t)tops[blocks]);
-    const float y = now > 0.0f ? 127.0f / now * kUp : 0.0f;
-    const float again = now > 0.0f ? was / now * kUp : 0.0f;
+    const float y = now > 0.0f ? kv_factor(127.0f, now) : 0.0f;
+    const float again = now > 0.0f ? kv_factor(was, now) : 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         uint4_t out;
@@ -159,11 +156,11 @@ __device__ __forceinline__ void write_piece(const KvArgs& a, const KvSide& s, ui
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int i = d * 4 + k;
-                q[k] = nearest_bits((float)v[e][i >> 3][i & 7] * y);
+                q[k] = nearest_bits((float)v[e][i >> 3][i & 7], y);
                 if (!whole) {
                     const int32_t t = first + (V ? minor + i : major[e]);
                     const int32_t byte = (int32_t)(old[e][d] << (24 - 8 * k)) >> 24;
-                    if (t < pos) q[k] = nearest_bits((float)byte * again);
+                    if (t < pos) q[k] = nearest_bits((float)byte, again);
                     if (t >= end) q[k] = (uint32_t)byte;
                 }
             }
@@ -199,16 +196,16 @@ __device__ __forceinline__ void write_token(const KvArgs& a, const KvSide& s, in
     }
     m = max(wave_max_u32_uniform(m), old);
     const float now = (float)__builtin_bit_cast(half_t, (uint16_t)m);
-    const float y = now > 0.0f ? 127.0f / now * kUp : 0.0f;
+    const float y = now > 0.0f ? kv_factor(127.0f, now) : 0.0f;
     int8_t* const ints = s.ints + head * a.length * a.dim;
     int8_t* const at = V ? ints + (int64_t)(pos >> 4) * 16 * a.dim + (pos & 15) : ints + (int64_t)pos * a.dim;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.dim) at[(c * 64 + lane) * (V ? 16 : 1)] = (int8_t)nearest_bits((float)v[c] * y);
+        if (c * 64 + lane < a.dim) at[(c * 64 + lane) * (V ? 16 : 1)] = (int8_t)nearest_bits((float)v[c], y);
     if (m == old && first < pos) return;         // (at a block's start what the magnitude was does not count, not even where it is 0 now)
     if (lane == 0) *top = __builtin_bit_cast(half_t, (uint16_t)m);
     if (first == pos) return;
-    const float again = (float)__builtin_bit_cast(half_t, (uint16_t)old) / now * kUp;
+    const float again = kv_factor((float)__builtin_bit_cast(half_t, (uint16_t)old), now);
     // sixteen bytes at a time: whole keys; whole groups of values, of the last one the bytes before the token
     const int32_t part = V ? pos & 15 : 0, pieces = ((V ? (pos + 15) & -16 : pos) - first) * a.dim / 16, partial = V && part ? pieces - a.dim : pieces;
     uint4_t* const p = reinterpret_cast<uint4_t*>(ints + (int64_t)first * a.dim);
@@ -219,7 +216,7 @@ __device__ __forceinline__ void write_token(const KvArgs& a, const KvSide& s, in
         for (int d = 0; d < 4; ++d) {
             uint32_t q[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q[k] = nearest_bits((float)((int32_t)(w[d] << (24 - 8 * k)) >> 24) * again);
+            for (int k = 0; k < 4; ++k) q[k] = nearest_bits((float)((int32_t)(w[d] << (24 - 8 * k)) >> 24), again);
             r[d] = pack4_i8(q[0], q[1], q[2], q[3]);
         }
         if (i < partial) p[i] = r;

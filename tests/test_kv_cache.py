@@ -92,3 +92,13 @@ def test_rounding_of_every_pair(tmp_path):
     subprocess.run(["gcc", "-O2", "-ffp-contract=off", "-fopenmp", here, "-o", exe, "-lm"], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
     assert "0 differ" in out, out
+
+
+def test_rounding_of_every_pair_as_the_kernels_compile_it(tmp_path):
+    """The functions of csrc/kv_round.h themselves, a fused product and addition: what rounds is not left to a compiler's choice.  The factors are divisions rounded as IEEE says on both sides."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "kv_round_fma_check")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-ffp-contract=off", "-fopenmp", "-I", os.path.join(root, "cpm_kernels_amd", "csrc"),
+                    os.path.join(root, "tests", "native", "kv_round_fma_check.cpp"), "-o", exe], check=True)
+    out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
+    assert out.splitlines()[-1] == "0 differ", out
