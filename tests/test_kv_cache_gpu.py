@@ -499,6 +499,47 @@ def test_captured_steps(gpu):
         lens += 1
 
 
+@pytest.mark.parametrize("n", [1, 3, 40, 100])
+def test_calls_on_addresses(gpu, n):
+    """The kernels layer: every argument of the three calls, all strides unlike, keys in parts, against the same calls of QuantizedKV, bit for bit."""
+    print("calls on addresses", n, flush=True)
+    rng = np.random.default_rng(n)
+    b, held, heads, d, length, block = 3, 2, 4, 80, 2112, 32
+    both = _Both(rng, b, held, length, d, block)
+    c = both.cache
+    mine = [x.clone() for x in (c.keys, c.values, c.key_absmax, c.value_absmax)]
+    at = [x.data_ptr() for x in mine]
+    stream = torch.cuda.current_stream().cuda_stream
+    k, v, q = _tokens(rng, b, held, n, d, "rows")[1], _tokens(rng, b, held, n, d, "columns", 2.0)[1], _tokens(rng, b, heads, n, d, "strided")[1]
+    for pos_each, pos, count in ((None, 37, None), (_ints([0, 1990, -1]), 0, _ints([n, (n + 1) // 2, 1]))):
+        c.write(k, v, pos if pos_each is None else pos_each, count)
+        ck.kv_write_int8(b, held, n, d, length, block, k.data_ptr(), k.stride(), v.data_ptr(), v.stride(), None if pos_each is None else pos_each.data_ptr(), pos,
+                         None if count is None else count.data_ptr(), *at, stream)
+        assert all(torch.equal(x, y) for x, y in zip(mine, (c.keys, c.values, c.key_absmax, c.value_absmax)))
+    for start in (5, _ints([-3, 100, 2100])):
+        got = torch.empty((2, b, held, d, n), dtype=torch.half, device="cuda").transpose(3, 4)
+        each = isinstance(start, torch.Tensor)
+        ck.kv_read_int8(b, held, n, d, length, block, *at, start.data_ptr() if each else None, 0 if each else start, got[0].data_ptr(), got[1].data_ptr(), got[0].stride(), stream)
+        assert all(torch.equal(x, y) for x, y in zip(got, c.read(start, n)))
+    size = ck.kv_attention_int8_workspace(b, heads, held, n, d, length)
+    assert size > 0
+    bias = _bias(rng, heads, True)
+    mask = torch.from_numpy(rng.random((b, n, length + 5)) < 0.8).cuda()[..., 5:]
+    lens, pos = _ints([2112, 700, 65]), _ints([2000, 650, 3])
+    calls = [dict(lens=2100), dict(lens=lens, causal=False, scale=0.2), dict(lens=lens, pos=pos, mask=mask, **bias), dict(lens=2000, pos=1500, causal=False, mask=mask[:, 0])]
+    for call in calls:
+        where = {name: (call[name].data_ptr(), 0) if isinstance(call.get(name), torch.Tensor) else (None, call.get(name, -1)) for name in ("lens", "pos")}
+        m = call.get("mask")
+        masks = (None, 0, 0) if m is None else (m.data_ptr(), m.stride(0), m.stride(1) if m.ndim == 3 else 0)
+        table = (bias["bias"].data_ptr(), bias["mapping"].data_ptr(), 32, 128, True) if "bias" in call else (None, None, 0, 0, False)
+        out = torch.full((b, heads, n, 2 * d), 7.0, dtype=torch.half, device="cuda")
+        space = torch.empty(size, dtype=torch.uint8, device="cuda")
+        ck.kv_attention_int8(b, heads, held, n, d, length, block, q.data_ptr(), q.stride(), *at, *where["lens"], *where["pos"], call.get("causal", True),
+                             call.get("scale", d ** -0.5), *table, *masks, out.data_ptr(), out[..., ::2].stride(), space.data_ptr(), stream)
+        rest = dict(call)
+        assert torch.equal(out[..., ::2], c.attention(q, rest.pop("lens"), **rest)) and bool((out[..., 1::2] == 7).all())
+
+
 @pytest.mark.parametrize("n,d", [(3, 64), (40, 128), (100, 64), (100, 128), (100, 256)])
 def test_workspaces_off_16_byte_boundaries(gpu, n, d):
     """A workspace starts at any multiple of 4 bytes; what lies around it stays as it is."""
