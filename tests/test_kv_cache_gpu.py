@@ -465,6 +465,40 @@ def test_a_prompt_and_the_steps_behind_it(gpu):
     both.check()
 
 
+def test_beside_a_position_embedding(gpu):
+    """A module's own weight and the table of its distances, as a model has them: its biases are the module's, for a prompt and for the steps behind it."""
+    print("beside a position embedding", flush=True)
+    b, h, d, n, length = 2, 4, 64, 90, 192
+    for bidirectional in (True, False):
+        rng = np.random.default_rng(61)
+        pe = ct.PositionEmbedding(h, 32, 64, bidirectional).cuda().half()
+        both = _Both(rng, b, h, length, d, 32, fill=False)
+        k, v, q = (_tokens(rng, b, h, n, d, "columns") for _ in range(3))
+        both.write(k, v, 0)
+        mapping = torch.empty(pe.max_distance, dtype=torch.int32, device="cuda")
+        ck.position_embedding_init(pe.num_buckets, pe.max_distance, mapping.data_ptr(), pe.bidirectional, torch.cuda.current_stream().cuda_stream)
+        table = dict(table=pe.weight.detach().cpu().numpy(), mapping=mapping.cpu().numpy(), bidirectional=bidirectional)
+        distance = np.arange(n)[None, :] - np.arange(n)[:, None]
+        module = pe(n, n).detach().cpu().numpy().astype(np.float64)          # (heads, keys, queries)
+        assert all(np.array_equal(module[i], ok.bucket_bias(table["table"][i], table["mapping"], distance, bidirectional)) for i in range(h))
+        with pytest.raises(AssertionError, match="gradients"):
+            both.cache.attention(q[1], n, bias=pe.weight, mapping=mapping, bidirectional=pe.bidirectional)
+        with torch.no_grad():
+            for causal in (True, False):
+                want, bound = ok.attention(q[0], both.k, both.v, both.ka, both.va, np.full(b, n), d ** -0.5, causal, **table)
+                got = both.cache.attention(q[1], n, causal=causal, bias=pe.weight, mapping=mapping, bidirectional=pe.bidirectional)
+                assert (np.abs(got.cpu().numpy().astype(np.float64) - want) <= bound).all()
+            lens = np.full(b, n)
+            for _ in range(3):
+                k, v, q = (_tokens(rng, b, h, 1, d, "rows") for _ in range(3))
+                both.write(k, v, _ints(lens.tolist()))
+                lens += 1
+                want, bound = ok.attention(q[0], both.k, both.v, both.ka, both.va, lens, d ** -0.5, True, **table)
+                got = both.cache.attention(q[1], _ints(lens.tolist()), bias=pe.weight, mapping=mapping, bidirectional=pe.bidirectional)
+                assert (np.abs(got.cpu().numpy().astype(np.float64) - want) <= bound).all()
+        both.check()
+
+
 def test_captured_steps(gpu):
     """A step with positions on the device, captured and replayed with eager calls of other sizes between the replays; two graphs beside each other."""
     print("captured steps", flush=True)
