@@ -50,9 +50,10 @@ __device__ __forceinline__ KvRange kv_range(const KvAttention& a, int64_t b, int
 }
 
 // The bias of a head at a distance first_distance .. distances - 1 (others are as those at the ends).  With biases for both signs first_distance is -1 at least, where the table has
-// one distance only: a key behind the query takes the upper half of the buckets however short the table is.
+// one distance only: a key behind the query takes the upper half of the buckets however short the table is.  Numbers of buckets that the table does not have (position_embedding_init
+// gives such where the distances are no multiple of the buckets that are exact) count as the nearest that it has.
 __device__ __forceinline__ half_t kv_bias(const KvAttention& a, int32_t head, int32_t rel) {
-    const int32_t bucket = a.mapping[min(abs(rel), a.distances - 1)] + (rel < 0 ? a.buckets / 2 : 0);
+    const int32_t bucket = min(a.mapping[min(abs(rel), a.distances - 1)], a.buckets) + (rel < 0 ? a.buckets / 2 : 0);
     return a.table[(int64_t)head * a.buckets + max(0, min(bucket, a.buckets - 1))];
 }
 

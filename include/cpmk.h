@@ -503,7 +503,8 @@ int cpmk_kv_read_int8(int32_t batch, int32_t heads, int32_t tokens, int32_t dim,
  * h / (heads / kv_heads), at = the query's position: pos_each[b] + i, or pos + i, or, with a negative pos, lens[b] - tokens + i.  Key j counts where
  * j < lens_each[b] (or len), j <= at if causal, and mask[b * mask_batch + i * mask_token + j] != 0 if there is a mask (rows of `length` bytes; a
  * mask_token of 0 for one row a sequence).  A query that no key is left for gives zeros.  bias: the table of cpmk_position_embedding_forward, buckets
- * as there (mapping of cpmk_position_embedding_init), at most 1024 distances (both signs counted if bidirectional); NULL for none.
+ * as there (mapping of cpmk_position_embedding_init; a bucket number outside of the table counts as the nearest in it), at most 1024 distances (both
+ * signs counted if bidirectional); NULL for none.
  * workspace: cpmk_kv_attention_int8_workspace() bytes on the device, 4-byte aligned, the call's own until it has finished; NULL if that is 0. */
 int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length, int32_t block,
                            const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,

@@ -499,6 +499,27 @@ def test_beside_a_position_embedding(gpu):
         both.check()
 
 
+@pytest.mark.parametrize("n", [2, 90])
+def test_bucket_numbers_outside_of_the_table(gpu, n):
+    """They count as the nearest in it."""
+    print("buckets outside", n, flush=True)
+    rng = np.random.default_rng(n)
+    both = _Both(rng, 1, 2, 192, 64, 32)
+    q = _tokens(rng, 1, 2, n, 64, "rows")[1]
+    bias = torch.from_numpy(rng.standard_normal((2, 8)).astype(np.float16)).cuda()
+    for bidirectional in (False, True):
+        outside, inside = _ints([0, 7, 8, -1, 2 ** 31 - 1, -2 ** 31, 3]), _ints([0, 7, 7, 0, 7, 0, 3])
+        if bidirectional:
+            # (of keys behind the query 4 is added first: 3 + 4 is the last one)
+            outside, inside = _ints([0, 1, 4, -9, 2 ** 31 - 1, 2, 2 ** 31 - 2]), _ints([0, 1, 3, -4, 3, 2, 3])
+        for pos in (-n, 1 - n):
+            kw = dict(causal=not bidirectional, bias=bias, bidirectional=bidirectional)
+            if bidirectional:
+                kw["pos"] = _ints([pos])
+            got = both.cache.attention(q, 180, mapping=outside, **kw)
+            assert torch.equal(got, both.cache.attention(q, 180, mapping=inside, **kw))
+
+
 def test_captured_steps(gpu):
     """A step with positions on the device, captured and replayed with eager calls of other sizes between the replays; two graphs beside each other."""
     print("captured steps", flush=True)
