@@ -114,6 +114,31 @@ def test_write_token_by_token(gpu, block, d):
     both.check()
 
 
+@pytest.mark.parametrize("block,d", [(16, 80), (64, 64), (128, 32)])
+def test_tokens_one_by_one_stay_near_themselves(gpu, block, d):
+    """Half a step of a block's magnitude for the rounding when a token comes in, and half a step of the new one each time that its block grows."""
+    print("near themselves", block, d, flush=True)
+    rng = np.random.default_rng(block)
+    cache = ct.QuantizedKV.empty(2, 3, 2 * block, d, block)
+    k, v = (_tokens(rng, 2, 3, 2 * block, d, "rows") for _ in range(2))
+    off = [np.zeros((2, 3, 2 * block)) for _ in range(2)]
+    grown = 0
+    for i in range(2 * block):
+        before = [x[:, :, i // block].clone() for x in (cache.key_absmax, cache.value_absmax)]
+        cache.write(k[1][:, :, i:i + 1], v[1][:, :, i:i + 1], i)
+        first = i // block * block
+        for bound, old, new in zip(off, before, (cache.key_absmax, cache.value_absmax)):
+            new = new[:, :, i // block].cpu().numpy().astype(np.float64)
+            grows = (new > old.cpu().numpy()) & (i > first)
+            grown += grows.sum()
+            bound[:, :, first:i] += (grows * new / 254)[..., None]
+            bound[:, :, i] = new / 254
+    assert grown > 2 * 2 * 3 * 2
+    for x, bound, ints, top in zip((k, v), off, (cache.keys.cpu().numpy(), ok.by_token(cache.values.cpu().numpy())), (cache.key_absmax, cache.value_absmax)):
+        err = np.abs(ok.values_of(ints, top.cpu().numpy()) - x[0].astype(np.float64))
+        assert (err <= bound[..., None] * (1 + 1e-12)).all(), (err / bound[..., None]).max()
+
+
 @pytest.mark.parametrize("n,pos", [(40, 0), (1, 5), (23, 9)])
 def test_write_of_extreme_values(gpu, n, pos):
     """Infinities count as the largest finite numbers, NaN as nothing; zeros, subnormal magnitudes, halves between two integers."""
