@@ -40,7 +40,9 @@ def _each(x, batch, device):
     if isinstance(x, torch.Tensor):
         assert x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous() and x.device == device
         return x.data_ptr(), 0
-    return None, int(x)
+    number = int(x)
+    assert number == x, "positions and lengths are integers"
+    return None, number
 
 
 class QuantizedKV:

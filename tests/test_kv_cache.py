@@ -4,6 +4,7 @@ import subprocess
 
 import numpy as np
 import pytest
+import torch
 
 from oracle import kv_cache as ok
 
@@ -69,6 +70,17 @@ def test_refusals_of_sizes_whose_products_leave_64_bits():
     # (no work is no work whatever the other sizes are)
     cpmk.kv_attention_int8(big, big, big, 0, 64, 64, 16, N, *S, N, N, N, N, N, 8, N, -1, 1, 0.125, N, N, 0, 0, 0, N, 0, 0, N, *S, N, N)
     cpmk.kv_write_int8(big, big, 0, 64, 4096, 16, N, *S, N, *S, N, 0, N, N, N, N, N, N)
+
+
+def test_positions_and_lengths_that_are_no_integers():
+    """They are refused, not cut off; integers of any kind are taken."""
+    from cpm_kernels_amd.torch.kv_cache import _each
+    here = torch.device("cpu")
+    for x in (5, np.int32(5), np.int64(5), 5.0):
+        assert _each(x, 2, here) == (None, 5)
+    for x in (5.5, -0.25, float("nan"), float("inf"), None, "5", torch.tensor(5), torch.tensor([5, 5]), torch.tensor([5, 5, 5], dtype=torch.int32)):
+        with pytest.raises((AssertionError, TypeError, ValueError, OverflowError)):
+            _each(x, 2, here)
 
 
 def test_oracle_of_the_cache():
