@@ -9,6 +9,9 @@
 // that sum: the fp16 of p' then has its full width whatever the magnitudes are, and the sum below takes p' / s in fp32.  (Multiplying p by s instead would leave p' in the
 // subnormal numbers beside a block of much larger values.)  Keys of all-zero blocks take s = 2^-34, below the smallest that a block can have.
 //
+// Rounded to fewer than 32 bits are the probabilities p', to fp16, because the second product takes them as fp16 operands beside the integers (fp32 operands have a sixteenth of that rate), and the result.  The sum
+// takes the unrounded ones.  Relative to float64, over all results, the root of the mean square is 2.3 to 2.9 10^-4 where probabilities of 32 bits and the same rounding of the result have 2.1 10^-4.
+//
 // Work is divided over the keys too where rows are few: a workgroup takes every tile of 64 keys of its part, wave by wave, and its waves join their sums
 // through LDS; parts leave theirs in the workspace and a second kernel joins them.
 //
@@ -75,7 +78,9 @@ __global__ __launch_bounds__(WAVES * 64, CT == 2 || DS > 2 ? 2 : DS == 2 ? 3 : 4
     const int32_t key_row = (col >> 2) * 16 + (col & 3);
     uint4_t raw[4 * DS], mk[CT];
     half_t kt, vt;
-    // keys that one workgroup looks at are read once (32 x 64 heads over up to 1024 keys 36 us for 42, 4 x 64 of 128 over up to 32768 41 for 44.5)
+    // Rows of sixteen: up to 128 units they are all that there are, and what they look at is read once (32 x 64 heads over up to 1024 keys 36 us for 42 without the hint, 4 x 64 of 128 over up to 32768 41 for
+    // 44.5; 4 x 64 heads on 8 of 256 over 16384 55.0 for 57.4).  Above 128 units CT is 1 with more rows too, which read the keys again, and there the hint costs: 8 x 32 heads of 256 over 1024 keys, 33 queries 63.5 us for
+    // 52.4, 64 queries 82.6 for 65.1.
     auto load = [&](const int8_t* p) { return CT == 1 ? __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)) : *reinterpret_cast<const uint4_t*>(p); };
     auto fetch_keys = [&](int32_t t) {
 #pragma unroll

@@ -13,9 +13,11 @@
 // four 16-byte accesses to the cache; to and from the fp16 side 32 contiguous bytes four times where the minor axis is contiguous there too ("straight"), 8 bytes sixteen
 // times where the major axis is ("crossed"), single halves otherwise and at the ends of a range.
 //
-// Bound by memory.  Writing 8 x 64 heads x 512 tokens of 64 units (101 MB) takes 25 us: all loads, a barrier, then all stores, one and a half rounds of workgroups; with the pieces at a range's ends read twice instead of
-// kept, 85 registers for 124, the same took 24 us and ragged prompts 27 instead of 15.6.  Reading 16 x 64 x 1024 (403 MB) takes 85 us, 4.7 TB/s: the hint for data that is not read again changes neither loads nor
-// stores (83 to 87), nor do rows of 256 or 512 bytes a wave instead of 128 (82 to 87).
+// Bound by memory.  Writing 8 x 64 heads x 512 tokens of 64 units (101 MB) takes 25 us: all loads, a barrier, then all stores, two rounds of workgroups (124 registers, so 1024 of 2048 at once); with the
+// pieces at a range's ends read twice instead of kept, 85 registers (1280 at once), the same took 24 us and ragged prompts 27 instead of 15.6 (1280 workgroups: a round and a quarter here).  A block that the range cuts is
+// loaded element by element and written as a whole: 5 tokens in the middle of a block of 64 take 14.2 us for 32 x 64 heads of 64 units, 16 take 18.5, where one takes 4.2 (k_kv_write_token).
+// Reading 16 x 64 x 1024 (403 MB) takes 85 us, 4.7 TB/s: the hint for data that is not read again, which the loads carry, changes neither loads nor stores (83 to 87), nor do rows of 256 or 512 bytes a wave
+// instead of 128 (82 to 87).
 #include "kv_ints.h"
 #include "kv_round.h"
 
@@ -171,7 +173,9 @@ __device__ __forceinline__ void write_piece(const KvArgs& a, const KvSide& s, ui
 }
 
 // One token a sequence, the decode step: a wave a head's key or value, whose units its lanes hold.  Its integers are all that is written unless the token is larger than what its block holds, in which case
-// the block's older ones are read and rounded again.  Bound by latency: of the general kernel, which passes over the whole block either way, 32 x 64 heads of 64 took 13.2 us.
+// the block's older ones are read and rounded again, a wave's loads one behind another's store.  Bound by latency: 32 x 64 heads of 64 take 4.2 us where no block grows, 5.0 where one in fourteen does (as many
+// as do on average while a block of 64 fills), and where all do 6.5 in the middle of a block of 64 and 10.3 at its end; 32 x 8 heads of 256 in blocks of 128 take 3.9, and up to 16.8 where all grow.  Of the general kernel, which passes over the
+// whole block either way, 32 x 64 heads of 64 took 13.2 us.
 template <bool V>
 __device__ __forceinline__ void write_token(const KvArgs& a, const KvSide& s, int64_t b, int32_t h, int32_t pos) {
     const int lane = threadIdx.x & 63;

@@ -15,6 +15,9 @@
 // best.  8 x 64 heads of 512 queries over 1024 of 64 units with a position bias (52 GFLOP) 108 us.  The scores of the next tile between the exponentials of this one, in the same wave, took 329 us for 296 and
 // 144 for 110: both tiles' scores do not fit the registers beside the sums.
 //
+// Registers: with a bias and a mask, heads of up to 64 units have 27 registers a lane in scratch under the bound of three waves a SIMD (8 x 64 heads of 512 queries over 1024 keys 164 us; the bias alone 109,
+// the mask alone 130, neither 99), and with a mask heads of more than 128 units three (8 x 32 heads of 256, the same lengths, 301 us; without 292).  Above 128 units there is one form, of 256 units and one wave a SIMD.
+//
 // LDS, in pieces of 16 bytes: keys (unit step u, half h, row r) at 129 u + 64 h + r, read along r; the odd distance spreads the eight unit steps that
 // neighbouring lanes write over the banks.  Values (group of sixteen keys g, half s, unit) at (2 g + s) D + unit.
 #include "kv_attention.h"
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, NT == 2 ? 3 : NT <= 4 ? 2 : 1) vo
                 for (int j = 0; j < 16; ++j) {
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[su][j], factor[su], shift));
                     part += e;
-                    p[su][j >> 3][j & 7] = (half_t)e;
+                    p[su][j >> 3][j & 7] = (half_t)e;           // (an operand of the second product: kv_attention.hip)
                 }
                 sum = __builtin_fmaf(part, fact[su][2], sum);
             }
