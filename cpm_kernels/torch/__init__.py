@@ -10,7 +10,7 @@ import sys
 
 from cpm_kernels_amd.torch import *  # noqa: F401,F403
 
-SUBMODULES = ("arith", "embedding", "gelu", "gemm", "kv_cache", "layernorm", "mask", "position_embedding",
+SUBMODULES = ("arith", "attention", "embedding", "gelu", "gemm", "kv_cache", "layernorm", "mask", "position_embedding", "rotary",
               "softmax", "transpose", "utils")
 
 for _name in SUBMODULES:

@@ -1,0 +1,288 @@
+// What the kernels of the attention over fp16 keys and values share (attention.hip: forward, attention_bwd.hip: gradients).
+#pragma once
+#include "common.h"
+
+namespace cpmk {
+
+// (batch, heads, tokens, dim) fp16 under any strides, in elements
+struct AttnTensor {
+    half_t* p;
+    int64_t batch, head, token, unit;
+    __device__ __forceinline__ half_t* at(int64_t b, int64_t h) const { return p + b * batch + h * head; }
+};
+
+struct Attention {
+    AttnTensor q, k, v, out;
+    const int32_t *lens_each, *pos_each;
+    const half_t* table;            // (heads, buckets) or null
+    const int32_t* mapping;
+    const uint8_t* mask;
+    int64_t mask_batch, mask_token;
+    float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; or null
+    float* parts;
+    float scale;                    // with log2(e)
+    int32_t len, pos;               // pos < 0: the queries are the last of the keys
+    int32_t heads, held, group, tokens, dim, length, buckets, distances, first_distance;
+    int32_t causal;
+    int32_t row_tiles, splits;
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kAttnTile = 64;       // tokens a workgroup stages at a time
+constexpr int32_t kAttnFar = 1 << 30, kAttnLong = 1 << 29;       // positions stay below the one, numbers of tokens and keys up to the other: distances fit 32 bits
+constexpr int kBiasPad = 96;        // distances beyond the table's ends that a tile of 64 tokens and the 32 of a wave can reach into
+
+enum { kRows = 0, kColumns = 1, kAnyLayout = 2 };
+
+struct AttnRange {
+    int32_t len, pos;
+};
+__device__ __forceinline__ AttnRange attn_range(const Attention& a, int64_t b) {
+    AttnRange r;
+    r.len = max(0, min(a.lens_each ? a.lens_each[b] : a.len, a.length));
+    r.pos = a.pos_each ? max(-kAttnFar, min(a.pos_each[b], kAttnFar - 1)) : a.pos < 0 ? r.len - a.tokens : min(a.pos, kAttnFar - 1);
+    return r;
+}
+
+// The bucket of a distance (query - key) first_distance .. distances - 1; others are as those at the ends.  With biases for both signs first_distance is -1 at least: a key behind
+// the query takes the upper half of the buckets however short the table is.  Numbers of buckets that the table does not have count as the nearest that it has.
+__device__ __forceinline__ int32_t attn_bucket(const Attention& a, int32_t rel) {
+    const int32_t bucket = min(a.mapping[min(abs(rel), a.distances - 1)], a.buckets) + (rel < 0 ? a.buckets / 2 : 0);
+    return max(0, min(bucket, a.buckets - 1));
+}
+
+// The biases of a head by distance, times log2(e), in LDS: entry i is that of the distance i + first_distance - kBiasPad, clamped to the table's ends.
+__device__ __forceinline__ int attn_bias_entries(const Attention& a) { return a.distances - a.first_distance + 2 * kBiasPad; }
+__device__ __forceinline__ void attn_biases(const Attention& a, int32_t head, float* biases, int tid, int threads) {
+    const half_t* const row = a.table + (int64_t)head * a.buckets;
+    for (int i = tid; i < attn_bias_entries(a); i += threads)
+        biases[i] = (float)row[attn_bucket(a, max(a.first_distance, min(i + a.first_distance - kBiasPad, a.distances - 1)))] * kLog2e;
+}
+
+// Workgroup x of units * inner ones: the `inner` workgroups of a unit, which read the same keys, follow one another on one XCD, and units are dealt to the XCDs in turn.
+__device__ __forceinline__ void attn_deal(uint32_t x, uint32_t units, uint32_t inner, uint32_t& unit, uint32_t& in) {
+    const uint32_t whole = units & ~7u;
+    if (x < whole * inner) {
+        const uint32_t y = x >> 3, u = y / inner;
+        unit = u * 8 + (x & 7);
+        in = y - u * inner;
+    } else {
+        x -= whole * inner;
+        in = x / (units - whole);
+        unit = whole + (x - in * (units - whole));
+    }
+}
+
+// ---- tiles of 64 tokens in LDS -----------------------------------------------------------------------------------------------
+// A tile lies token by token, D units (64, 128 or 256) each, in pieces of eight units; piece c of token t at place c ^ swizzle(t) within its group of eight.  An operand of the matrix
+// instructions is read in one of two ways: eight units of a token a lane (16 bytes; 8 neighbouring lanes have neighbouring tokens, whose swizzles differ), or, transposed, four tokens of a
+// unit a lane (ds_read_b64_tr_b16: 16 lanes hand in the addresses of four tokens' 32 bytes, whose swizzles differ in the bits above the lowest).  Tokens 8 apart differ too: a thread that
+// brings eight tokens of a unit writes to them one after another, beside its neighbours'.
+__device__ __forceinline__ int attn_swizzle(int token) { return (((token & 3) << 1) | ((token >> 2) & 1)) ^ ((token >> 3) & 7); }
+
+template <int D>
+__device__ __forceinline__ int attn_place(int token, int piece) {
+    return token * D * 2 + (((piece & ~7) | ((piece ^ attn_swizzle(token)) & 7)) << 4);
+}
+
+// Lane's address for operands of rows = tokens: piece 2 s + half of token (lane & 31) + 32 blk is at (rows ^ ((2 s & 7) << 4 ^ blk << 6)) + blk * 32 rows + (s >> 2) * 128.
+template <int D>
+__device__ __forceinline__ uint32_t attn_rows_at(int lane) {
+    const int t = lane & 31;
+    return t * D * 2 + (((lane >> 5) ^ attn_swizzle(t)) << 4);
+}
+template <int D>
+__device__ __forceinline__ half8_t attn_rows(const int8_t* tile, uint32_t at, int blk, int s) {
+    return *reinterpret_cast<const half8_t*>(tile + ((at ^ (((2 * s) & 7) << 4) ^ (blk << 6)) + blk * 32 * D * 2 + (s >> 2) * 128));
+}
+// Lane's address for operands of rows = units: of unit block n (32 units), tokens 32 blk + 16 e + 4 half + {0..3, 8..11}: the order in which the results of a product with tokens as
+// rows lie in a lane's registers 8 e .. 8 e + 7.
+template <int D>
+__device__ __forceinline__ uint32_t attn_units_at(int lane) {
+    const int half = lane >> 5, j = lane & 15, c = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1), t = 4 * half + (j >> 2);
+    return t * D * 2 + ((c ^ ((j >> 2) << 1 | half)) << 4) + (j & 1) * 8;
+}
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef short short8_t __attribute__((ext_vector_type(8)));
+template <int D>
+__device__ __forceinline__ half8_t attn_units(const int8_t* tile, uint32_t at, int n, int blk, int e) {
+    const int x = ((n & 1) << 2) ^ (blk << 2) ^ (e << 1);
+    const int8_t* const p = tile + (blk * 32 + e * 16) * D * 2 + (n >> 1) * 128;
+    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + (at ^ (x << 4))));
+    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + 8 * D * 2 + (at ^ ((x ^ 1) << 4))));
+    return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A thread's share of a tile on its way from memory to LDS.  kRows: pieces of eight units as they lie.  kColumns: eight tokens of PIECES neighbouring units, turned in registers.
+// kAnyLayout: unit by unit.  Tokens past the last one and units past the head's are zeros.
+template <int D, int LAY, int THREADS>
+struct AttnShare {
+    static constexpr int PIECES = 64 * D / 8 / THREADS, RUN = D / 8, STEP = THREADS / RUN;      // (rows: a pass of the workgroup brings STEP tokens)
+    static_assert(PIECES >= 1 && (LAY != kColumns || PIECES <= 8), "share of a tile");
+    half8_t r[PIECES];
+
+    __device__ __forceinline__ void load(const half_t* base, int64_t token, int64_t unit, int dim, int32_t t0, int32_t tokens, int tid) {
+        const bool whole = t0 + kAttnTile <= tokens;
+        if constexpr (LAY == kRows) {
+            const int row = tid / RUN, u = min((tid % RUN) * 8, dim - 8);
+            if (whole) {
+                const half_t* p = base + (t0 + row) * token + u;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(p + i * STEP * token);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(t0 + row + i * STEP, tokens - 1) * token + u);
+            }
+        } else if constexpr (LAY == kColumns) {
+            const int tb = (tid & 7) * 8, u0 = (tid >> 3) * PIECES;
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(u0 + i, dim - 1) * unit + t0 + tb);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[i][e] = base[min(u0 + i, dim - 1) * unit + min(t0 + tb + e, tokens - 1)];
+            }
+        } else {
+            const int row = tid / RUN, u = (tid % RUN) * 8;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[i][e] = base[min(t0 + row + i * STEP, tokens - 1) * token + min(u + e, dim - 1) * unit];
+        }
+    }
+
+    // Zeros where there is nothing; with `guard` numbers that are none or infinite become zeros as well, and their tokens are entered in `bad` as those of tile `stamp`
+    __device__ __forceinline__ void clean(int dim, int32_t t0, int32_t tokens, int tid, bool guard, int32_t* bad, int32_t stamp) {
+        const bool whole = t0 + kAttnTile <= tokens && D == dim;
+        if (whole && !guard) return;
+        half8_t worst = {0, 0, 0, 0, 0, 0, 0, 0};
+        const half8_t none = worst;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            int units, at;      // how many of the eight are real
+            if constexpr (LAY == kColumns) {
+                at = (tid & 7) * 8;
+                units = (tid >> 3) * PIECES + i < dim ? max(0, min(8, tokens - t0 - at)) : 0;
+            } else {
+                at = tid / RUN + i * STEP;
+                units = t0 + at < tokens ? max(0, min(8, dim - (tid % RUN) * 8)) : 0;
+            }
+            r[i] = half8_fill(r[i], half8_keep(units), none);
+            worst = __builtin_elementwise_fma(r[i], none, worst);
+        }
+        if (!guard) return;
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) any |= !(worst[e] == (half_t)0);
+        if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(r[i][e] * (half_t)0 == (half_t)0)) {
+                    r[i][e] = (half_t)0;
+                    bad[LAY == kColumns ? (tid & 7) * 8 + e : tid / RUN + i * STEP] = stamp;
+                    bad[kAttnTile] = stamp;
+                }
+    }
+
+    __device__ __forceinline__ void store(int8_t* tile, int tid) const {
+        if constexpr (LAY == kColumns) {
+            const int u0 = (tid >> 3) * PIECES;
+            struct Run { half_t u[PIECES]; };
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int t = (tid & 7) * 8 + e;
+                typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
+                run_t v;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) v[i] = r[i][e];
+                *reinterpret_cast<run_t*>(tile + attn_place<D>(t, u0 >> 3) + (u0 & 7) * 2) = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) *reinterpret_cast<half8_t*>(tile + attn_place<D>(tid / RUN + i * STEP, tid % RUN)) = r[i];
+        }
+    }
+};
+
+// An operand that a wave keeps: eight units from 16 s + 8 half on of the lane's token, zeros past the head's last unit.
+template <int KS>
+__device__ __forceinline__ void attn_keep(half8_t (&x)[KS], const AttnTensor& t, const half_t* row, int dim, int half) {
+    if (t.unit == 1 && dim % 8 == 0) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x[s] = load_half8_any(row + min(s * 16 + half * 8, dim - 8));
+    } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] = row[min(s * 16 + half * 8 + e, dim - 1) * t.unit];
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) x[s] = half8_fill(x[s], half8_keep(dim - s * 16 - half * 8), half8_t{0, 0, 0, 0, 0, 0, 0, 0});
+}
+
+// Four mask bytes of keys key .. key + 3 (bytes past the row's end: 0)
+__device__ __forceinline__ uint32_t attn_mask4(const uint8_t* row, int32_t key, int32_t length) {
+    if (key + 4 <= length) return reinterpret_cast<const Byte4Any*>(row + key)->x;
+    uint32_t m = 0;
+    for (int e = 0; e < 4; ++e)
+        if (key + e < length) m |= (uint32_t)row[key + e] << (8 * e);
+    return m;
+}
+
+// A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times f, as fp16
+template <int NT>
+__device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, const float16_tv (&acc)[NT], float f, int dim, int half) {
+    if (t.unit == 1 && dim % 4 == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                half4_t v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (half_t)(acc[n][c * 4 + e] * f);
+                const int u = n * 32 + c * 8 + half * 4;
+                if (u < dim) *reinterpret_cast<Half4Any*>(row + u) = __builtin_bit_cast(Half4Any, v);
+            }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int u = n * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
+                if (u < dim) row[u * t.unit] = (half_t)(acc[n][i] * f);
+            }
+    }
+}
+
+constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+// The layout by which tiles of two tensors are brought
+inline int attn_layout(const AttnTensor& x, const AttnTensor& y, int32_t dim) {
+    if (x.unit == 1 && y.unit == 1 && dim % 8 == 0) return kRows;
+    return x.token == 1 && y.token == 1 ? kColumns : kAnyLayout;
+}
+
+// What forward and backward refuse; sets heads and the table's first distance.  0 or an error code; `empty`: tensors without elements whatever the numbers of tokens and keys.
+inline int attn_check(Attention& a, int32_t batch, int32_t heads, int32_t kv_heads, int bidirectional, bool& empty) {
+    empty = false;
+    if (batch < 0 || heads < 0 || kv_heads < 0 || a.tokens < 0 || a.dim < 0 || a.length < 0) return CPMK_EBADARG;
+    if (!a.lens_each && (a.len < 0 || a.len > a.length)) return CPMK_EBADARG;
+    if (batch == 0 || heads == 0 || a.dim == 0) {
+        empty = true;
+        return 0;
+    }
+    if (kv_heads == 0 || heads % kv_heads) return CPMK_EBADARG;
+    if (a.dim > 256 || a.tokens > kAttnLong || a.length > kAttnLong || !grid_fits((int64_t)batch * heads)) return CPMK_ETOOBIG;
+    if (a.table && (!a.mapping || a.buckets <= 0 || a.distances <= 0)) return CPMK_EBADARG;
+    if (a.table && (int64_t)a.distances * (bidirectional ? 2 : 1) > 1024) return CPMK_ETOOBIG;
+    a.heads = heads, a.held = kv_heads, a.group = heads / kv_heads;
+    a.first_distance = bidirectional ? (a.distances > 1 ? 1 - a.distances : -1) : 0;
+    if ((a.tokens > 0 && any_null(a.q.p, a.out.p)) || (a.length > 0 && any_null(a.k.p, a.v.p))) return CPMK_EBADARG;
+    return 0;
+}
+
+}  // namespace cpmk

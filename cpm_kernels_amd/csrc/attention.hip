@@ -1,0 +1,331 @@
+// Attention over fp16 keys and values, forward:
+//
+//     out[i] = sum_j p_ij v_j,   p_ij = exp(s_ij - m_i) / sum_j exp(s_ij - m_i),   s_ij = scale q_i k_j + bias[bucket(at_i - j)]
+//
+// over the keys j that length, causality and mask leave, in one pass over the keys: the running maximum m_i and the sum are kept beside the weighted values, which are scaled when the
+// maximum grows.  Nothing of the size of the scores is in memory.
+//
+// A workgroup has 128 queries of a head, 32 a wave, and goes over its keys in tiles of 64 that all its waves read from LDS.  Scores are formed transposed (keys as rows), so a lane holds
+// keys of one query, and its probabilities, rounded to fp16, are the second product's operand as they are.  fp16 keeps their bits: they are at most 2^15 and their maximum is 2^7 at least
+// (the running maximum follows the true one at a distance of up to 2^8), so what falls below fp16's normal range is less than 2^-21 of the row's largest.  Sums are fp32, of the
+// unrounded probabilities.  Where there are few rows the keys are cut into parts, which k_attn_join adds up.
+#include <algorithm>
+#include "attention.h"
+
+namespace cpmk {
+
+constexpr int kAttnRows = 128, kAttnLeast = 4;       // queries of a workgroup; tiles of a part, at least
+constexpr int kLazy = 8;            // log2 of how far the running maximum may lie below the true one
+constexpr float kLift = 7.0f;       // log2 of the largest probability's size right behind a change of the maximum
+
+// The keys that a tile of rows looks at, and the parts they are cut into (the same here and where the parts are joined).
+struct AttnParts {
+    int32_t keys, tiles, per_part, parts;
+};
+__device__ __forceinline__ AttnParts attn_parts(const Attention& a, const AttnRange& r, int32_t last_query, int least) {
+    AttnParts p;
+    p.keys = a.causal ? max(0, min(r.len, r.pos + last_query + 1)) : r.len;
+    p.tiles = (p.keys + kAttnTile - 1) / kAttnTile;
+    p.per_part = max((p.tiles + a.splits - 1) / a.splits, min(least, max(p.tiles, 1)));
+    p.parts = max(1, (p.tiles + p.per_part - 1) / p.per_part);
+    return p;
+}
+
+template <int NT, bool PLAIN, int LAY>
+__global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Attention a) {
+    constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
+    extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys and values, biases
+    __shared__ int32_t bad[2][kAttnTile + 1];
+    float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t inner = (uint32_t)a.group * a.row_tiles * a.splits;
+    uint32_t unit, w;
+    attn_deal(blockIdx.x, gridDim.x / inner, inner, unit, w);
+    const int64_t b = unit / (uint32_t)a.held;
+    const int32_t kvh = unit - (uint32_t)b * a.held;
+    const int32_t split = w % (uint32_t)a.splits;
+    w /= (uint32_t)a.splits;
+    // (of a causal chunk the last queries see most keys: their workgroups come first)
+    const int32_t qt = a.row_tiles - 1 - (int32_t)(w % (uint32_t)a.row_tiles);
+    const int32_t h = kvh * a.group + w / (uint32_t)a.row_tiles;
+    const AttnRange range = attn_range(a, b);
+    const AttnParts parts = attn_parts(a, range, min(qt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast);
+    if (split >= parts.parts) return;
+
+    const int32_t q_first = qt * kAttnRows + wave * 32;
+    const int32_t query = min(q_first + col, a.tokens - 1);         // (queries past the end repeat the last one)
+    const int32_t where = range.pos + query, limit = a.causal ? min(range.len, where + 1) : range.len;
+    // what all and what any of the wave's queries see, and what all of the workgroup's do
+    const int32_t last = min(q_first + 31, a.tokens - 1);
+    const int32_t all_see = a.causal ? min(range.len, range.pos + min(q_first, a.tokens - 1) + 1) : range.len;
+    const int32_t any_sees = q_first >= a.tokens ? 0 : a.causal ? min(range.len, range.pos + last + 1) : range.len;
+    const int32_t every_sees = a.causal ? min(range.len, range.pos + qt * kAttnRows + 1) : range.len;
+    const bool flip = a.scale < 0.0f;           // (so that the largest score is the largest product)
+    const float scale = flip ? -a.scale : a.scale;
+    const bool masked = !PLAIN && a.mask != nullptr, biased = !PLAIN && a.table != nullptr;
+    const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
+    const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
+
+    half8_t q[KS];
+    attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
+    if (flip)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = -q[s];
+    if (biased) attn_biases(a, h, biases, tid, 256);
+    const int32_t lo_rel = a.first_distance - kBiasPad;
+    if (tid <= kAttnTile) bad[0][tid] = bad[1][tid] = -1;
+
+    const int32_t t_begin = split * parts.per_part, t_end = min(t_begin + parts.per_part, parts.tiles);
+    AttnShare<D, LAY, 256> ks, vs;
+    auto load = [&](int32_t t) {
+        ks.load(keys, a.k.token, a.k.unit, a.dim, t * kAttnTile, range.len, tid);
+        vs.load(values, a.v.token, a.v.unit, a.dim, t * kAttnTile, range.len, tid);
+    };
+    auto store = [&](int32_t t) {
+        // (a value that is no finite number must not reach the queries that do not see it)
+        ks.clean(a.dim, t * kAttnTile, range.len, tid, false, nullptr, t);
+        vs.clean(a.dim, t * kAttnTile, range.len, tid, masked || t * kAttnTile + kAttnTile > every_sees, bad[t & 1], t);
+        int8_t* const buffer = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
+        ks.store(buffer, tid);
+        vs.store(buffer + kTileBytes, tid);
+    };
+    if (t_begin < t_end) load(t_begin);
+    __syncthreads();
+    if (t_begin < t_end) {
+        store(t_begin);
+        if (t_begin + 1 < t_end) load(t_begin + 1);
+    }
+    __syncthreads();
+
+    const uint32_t at_rows = attn_rows_at<D>(lane), at_units = attn_units_at<D>(lane);
+    float16_tv acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = kZero16;
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (int32_t t = t_begin; t < t_end; ++t) {
+        const int32_t k0 = t * kAttnTile;
+        const int8_t* const key_tile = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
+        const int8_t* const value_tile = key_tile + kTileBytes;
+        if (k0 < any_sees) {
+            float16_tv s[2] = {kZero16, kZero16};
+#pragma unroll
+            for (int u = 0; u < KS; ++u)
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) s[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D>(key_tile, at_rows, blk, u), q[u], s[blk], 0, 0, 0);
+            float factor = scale, add = 0.0f;
+            // one bias for the whole tile where all its distances lie beyond the table's end
+            const int32_t rel_min = range.pos + q_first - (k0 + kAttnTile - 1), rel_max = range.pos + last - k0;
+            const bool near = biased && rel_min < a.distances - 1 && rel_max > a.first_distance;
+            if (biased && !near) add = biases[(rel_min >= a.distances - 1 ? a.distances - 1 : a.first_distance) - lo_rel];
+            const bool spoilt = bad[t & 1][kAttnTile] == t;
+            if (masked || near || spoilt || k0 + kAttnTile > all_see) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int32_t key = k0 + blk * 32 + g * 8 + half * 4;
+                        uint32_t keep = 0x01010101u;
+                        if (masked) keep = attn_mask4(mask, key, a.length);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = __builtin_fmaf(s[blk][g * 4 + e], factor, add);
+                            if (near) x += biases[where - key - e - lo_rel];
+                            if (spoilt && bad[t & 1][key + e - k0] == t) x = __builtin_nanf("");
+                            s[blk][g * 4 + e] = key + e < limit && (keep >> (8 * e) & 0xffu) ? x : -__builtin_inff();
+                        }
+                    }
+                }
+                factor = 1.0f;
+                add = 0.0f;
+            }
+            float m = s[0][0];
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) m = fmaxf(m, s[blk][j]);
+            m = __builtin_fmaf(m, factor, add);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            if (__builtin_amdgcn_ballot_w64(m > top + kLazy)) {
+                const float now = fmaxf(m, top), f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+                top = now;
+                sum *= f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n] *= f;
+            }
+            const float shift = add - (top == -__builtin_inff() ? 0.0f : top) + kLift;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    half8_t p;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][e * 8 + j], factor, shift));
+                        sum += x;
+                        p[j] = (half_t)x;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_units<D>(value_tile, at_units, n, blk, e), p, acc[n], 0, 0, 0);
+                }
+        }
+        if (t + 1 < t_end) {
+            store(t + 1);
+            if (t + 2 < t_end) load(t + 2);
+        }
+        __syncthreads();
+    }
+    sum += __shfl_xor(sum, 32);
+    if (q_first + col >= a.tokens) return;
+    const int64_t row = (b * a.heads + h) * a.tokens + query;
+    if (a.splits > 1) {
+        struct __attribute__((packed, aligned(4))) Float4Any { float x, y, z, w; };         // (a workspace is aligned to 4 bytes)
+        float* const part = a.parts + (((b * a.heads + h) * a.row_tiles + qt) * a.splits + split) * kAttnRows * (a.dim + 2);
+        const int r = wave * 32 + col;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int u = n * 32 + c * 8 + half * 4;
+                if (u + 4 <= a.dim) *reinterpret_cast<Float4Any*>(part + r * a.dim + u) = Float4Any{acc[n][c * 4], acc[n][c * 4 + 1], acc[n][c * 4 + 2], acc[n][c * 4 + 3]};
+                else
+                    for (int e = 0; e < 4; ++e)
+                        if (u + e < a.dim) part[r * a.dim + u + e] = acc[n][c * 4 + e];
+            }
+        if (half == 0) {
+            part[kAttnRows * a.dim + r] = top;
+            part[kAttnRows * a.dim + kAttnRows + r] = sum;
+        }
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    attn_write<NT>(a.out, a.out.at(b, h) + query * a.out.token, acc, inv, a.dim, half);
+    if (a.lse && half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
+}
+
+// Parts joined under the largest of their maxima: a wave a row, its lanes along the units.
+__global__ __launch_bounds__(256) void k_attn_join(Attention a, uint32_t total_rows) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= total_rows) return;
+    const int32_t query = id % (uint32_t)a.tokens;
+    const uint32_t bh = id / (uint32_t)a.tokens;
+    const int64_t b = bh / (uint32_t)a.heads;
+    const int32_t h = bh - (uint32_t)b * a.heads;
+    const int32_t rt = query / kAttnRows, r = query - rt * kAttnRows;
+    const AttnRange range = attn_range(a, b);
+    const AttnParts p = attn_parts(a, range, min(rt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast);
+    const int64_t size = (int64_t)kAttnRows * (a.dim + 2);
+    const float* const part = a.parts + ((int64_t)bh * a.row_tiles + rt) * a.splits * size;
+    const float* const tops = part + kAttnRows * a.dim + r;
+    float m = -__builtin_inff();
+    for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, tops[i * size]);
+    m = wave_max(m);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    float total = 0.0f, value[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int first = 0; first < p.parts; first += 64) {
+        // a lane a part: its weight; then eight parts' sums at a time, all on their way together
+        const bool real = first + lane < p.parts;
+        const float* const mine = tops + (first + (real ? lane : 0)) * size;
+        const float weight = real ? __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
+        total = __builtin_fmaf(real ? mine[kAttnRows] : 0.0f, weight, total);
+        const int n = min(64, p.parts - first);
+        for (int i = 0; i < n; i += 8) {
+            float x[8][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c * 64 < a.dim) x[k][c] = part[(first + min(i + k, n - 1)) * size + r * a.dim + min(c * 64 + lane, a.dim - 1)];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = i + k < n ? __shfl(weight, i + k) : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c * 64 < a.dim) value[c] = __builtin_fmaf(x[k][c], f, value[c]);
+            }
+        }
+    }
+    total = wave_sum(total);
+    half_t* const out = a.out.at(b, h) + query * a.out.token;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c * 64 + lane < a.dim) out[(int64_t)(c * 64 + lane) * a.out.unit] = (half_t)(total == 0.0f ? 0.0f : value[c] / total);
+    if (a.lse && lane == 0) a.lse[id] = total == 0.0f ? __builtin_inff() : base - kLift + __builtin_amdgcn_logf(total);
+}
+
+// Into how many parts the keys are cut: as many as let the device's compute units each have a workgroup, of four tiles at least; none where rows are many.
+struct AttnPlan {
+    int row_tiles, splits;
+};
+static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t tokens, int64_t length) {
+    AttnPlan p;
+    p.row_tiles = (int)ceil_div(tokens, kAttnRows);
+    const int64_t base = batch * heads * p.row_tiles, tiles = ceil_div(length, kAttnTile), units = compute_units();
+    p.splits = (int)std::max<int64_t>(1, std::min(2 * units / base, tiles / kAttnLeast));
+    return p;
+}
+
+template <int NT, bool PLAIN, int LAY>
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
+    const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
+    static std::atomic<bool> done[64];
+    if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY>, 150 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY>), dim3(grid), dim3(256), lds, st, a);
+    return 0;
+}
+template <int NT, bool PLAIN>
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    const int lay = attn_layout(a.k, a.v, a.dim);
+    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
+}
+template <int NT>
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    return a.table || a.mask ? attn_launch<NT, false>(a, grid, st) : attn_launch<NT, true>(a, grid, st);
+}
+
+}  // namespace cpmk
+
+using namespace cpmk;
+
+extern "C" {
+
+int64_t cpmk_attention_forward_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length) {
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || dim <= 0 || length <= 0 || heads % kv_heads) return 0;
+    if (dim > 256 || tokens > kAttnLong || length > kAttnLong || !grid_fits((int64_t)batch * heads)) return 0;
+    const AttnPlan p = attn_plan(batch, heads, tokens, length);
+    return p.splits > 1 ? (int64_t)batch * heads * p.row_tiles * p.splits * kAttnRows * (dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
+int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length, const void* q, int64_t q_batch, int64_t q_head, int64_t q_token,
+                           int64_t q_unit, const void* k, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit, const void* v, int64_t v_batch, int64_t v_head, int64_t v_token,
+                           int64_t v_unit, const void* lens_each, int32_t len, const void* pos_each, int32_t pos, int causal, float scale, const void* bias, const void* mapping,
+                           int32_t num_buckets, int32_t max_distance, int bidirectional, const void* mask, int64_t mask_batch, int64_t mask_token, void* out, int64_t out_batch,
+                           int64_t out_head, int64_t out_token, int64_t out_unit, void* lse, void* workspace, void* stream) {
+    clear_stale_error();
+    Attention a;
+    a.q = {(half_t*)q, q_batch, q_head, q_token, q_unit}, a.k = {(half_t*)k, k_batch, k_head, k_token, k_unit}, a.v = {(half_t*)v, v_batch, v_head, v_token, v_unit};
+    a.out = {(half_t*)out, out_batch, out_head, out_token, out_unit};
+    a.lens_each = (const int32_t*)lens_each, a.pos_each = (const int32_t*)pos_each, a.len = len, a.pos = pos;
+    a.table = (const half_t*)bias, a.mapping = (const int32_t*)mapping, a.buckets = num_buckets, a.distances = max_distance;
+    a.mask = (const uint8_t*)mask, a.mask_batch = mask_batch, a.mask_token = mask_token;
+    a.lse = (float*)lse, a.scale = scale * kLog2e, a.causal = causal != 0;
+    a.tokens = tokens, a.dim = dim, a.length = length;
+    bool empty;
+    if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
+    if (empty || tokens == 0) return 0;
+    const AttnPlan plan = attn_plan(batch, heads, tokens, length);
+    a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
+    if (a.splits > 1 && !workspace) return CPMK_EBADARG;
+    const int64_t grid = (int64_t)batch * heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
+    if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned g = (unsigned)grid;
+    const int e = dim <= 64 ? attn_launch<2>(a, g, st) : dim <= 96 ? attn_launch<3>(a, g, st) : dim <= 128 ? attn_launch<4>(a, g, st) : attn_launch<8>(a, g, st);
+    if (e) return e;
+    if (a.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, (uint32_t)rows);
+    return launch_status();
+}
+
+}  // extern "C"

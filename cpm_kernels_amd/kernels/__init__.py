@@ -3,7 +3,9 @@ launchers this build adds (gemm_int8_scale, gemm_quantize, gemm_quantize_cols, g
 their `_ld` forms with padded rows, gemm_int8_scale_one, gemm_int8_scale_sum, gemm_fp16_sum, gemm_int8_scale_parts, gemm_fp16_parts,
 gemm_add_parts, gemm_int8_scale_split, gemm_fp16_split, gemm_quantize_cols_rows, gemm_backward_quantize_both, layernorm_affine_forward,
 layernorm_affine_forward_stats, layernorm_affine_backward, embedding_order_ids, embedding_backward_rows,
-embedding_backward_prepare) and the key/value cache in 8 bits (kv_write_int8, kv_read_int8, kv_attention_int8)."""
+embedding_backward_prepare) and the key/value cache in 8 bits (kv_write_int8, kv_read_int8, kv_attention_int8),
+the attention over fp16 keys and values with its gradients (attention_forward, attention_backward) and rotary positions (rotary_forward, rotary_backward)."""
+from .attention import attention_forward, attention_forward_workspace, attention_backward, attention_backward_workspace, rotary_forward, rotary_backward
 from .embedding import embedding_forward, embedding_backward_stage1, embedding_backward_stage2, embedding_step, \
     embedding_order_ids, embedding_backward_rows, embedding_backward_prepare
 from .gelu import gelu_forward, gelu_backward, gelu_inplace_forward

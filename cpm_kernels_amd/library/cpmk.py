@@ -42,6 +42,9 @@ _LAUNCHERS = {
     "transpose": "iiippp", "transpose_i8": "iiippp", "array_add": "piip", "adjustify_logits": "iipfffpp",
     "copy_extend_buffer": "iiippp",
     "kv_write_int8": "iiiiiipllllpllllpipppppp", "kv_read_int8": "iiiiiipppppippllllp", "kv_attention_int8": "iiiiiiipllllpppppipiifppiiipllpllllpp",
+    "attention_forward": "iiiiiipllllpllllpllllpipiifppiiipllpllllppp",
+    "attention_backward": "iiiiiipllllpllllpllllpipiifppiiipllpllllppllllpllllpllllpllllppp",
+    "rotary": "iiiiiipllllpllllipllllpllllppllifip",
     "has_nan_inf": "lppp", "copy_pos_hidden": "iiiippp", "async_status": "",
     "selftest_exchange_timeout": "ip",
 }
@@ -51,6 +54,7 @@ EXPORTED_SYMBOLS = sorted(["cpmk_" + n for n in _LAUNCHERS] + [
     "cpmk_version", "cpmk_error_string", "cpmk_device_count", "cpmk_get_device",
     "cpmk_set_device", "cpmk_device_props", "cpmk_exchange_capture_slots_left", "cpmk_gemm_sum_groups", "cpmk_gemm_sum_groups_for", "cpmk_gemm_sum_krows_groups",
     "cpmk_gemm_sum_groups_timed", "cpmk_kv_attention_int8_workspace",
+    "cpmk_attention_forward_workspace", "cpmk_attention_backward_workspace",
     "cpmk_gemm_depth_parts", "cpmk_gemm_fp16_copy_pays",
 ])
 
@@ -155,6 +159,16 @@ def gemm_fp16_copy_pays(m: int, k: int, n: int, batch: int, bT: int) -> int:
 @lib.bind("cpmk_kv_attention_int8_workspace", [ctypes.c_int32] * 6, ctypes.c_int64)
 def kv_attention_int8_workspace(batch: int, heads: int, kv_heads: int, tokens: int, dim: int, length: int) -> int:
     return lib.cpmk_kv_attention_int8_workspace(batch, heads, kv_heads, tokens, dim, length)
+
+
+@lib.bind("cpmk_attention_forward_workspace", [ctypes.c_int32] * 6, ctypes.c_int64)
+def attention_forward_workspace(batch: int, heads: int, kv_heads: int, tokens: int, dim: int, length: int) -> int:
+    return lib.cpmk_attention_forward_workspace(batch, heads, kv_heads, tokens, dim, length)
+
+
+@lib.bind("cpmk_attention_backward_workspace", [ctypes.c_int32] * 6 + [ctypes.c_int], ctypes.c_int64)
+def attention_backward_workspace(batch: int, heads: int, kv_heads: int, tokens: int, length: int, max_distance: int, bidirectional: int) -> int:
+    return lib.cpmk_attention_backward_workspace(batch, heads, kv_heads, tokens, length, max_distance, bidirectional)
 
 
 @lib.bind("cpmk_device_count", [ctypes.POINTER(ctypes.c_int)], ctypes.c_int)

@@ -195,6 +195,9 @@ PyMethodDef g_launchers[] = {
     CPMK_ENTRY(cpmk_copy_extend_buffer)
     CPMK_ENTRY(cpmk_has_nan_inf)
     CPMK_ENTRY(cpmk_copy_pos_hidden)
+    CPMK_ENTRY(cpmk_attention_forward)
+    CPMK_ENTRY(cpmk_attention_backward)
+    CPMK_ENTRY(cpmk_rotary)
     CPMK_ENTRY(cpmk_async_status)
     CPMK_ENTRY(cpmk_selftest_exchange_timeout)
 };

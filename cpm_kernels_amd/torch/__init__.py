@@ -12,6 +12,7 @@ from .arith import (
     ln_mul_add, ln_mul_add_inplace, ln_mul_addTH,
     ln_sub_div, ln_sub_div_inplace, ln_sub_divTH,
 )
+from .attention import attention, attentionTH
 from .embedding import Embedding, EmbeddingTH, OpEmbedding
 from .gelu import gelu, gelu_inplace, geluTH
 from .gemm import bmm
@@ -19,9 +20,10 @@ from .kv_cache import QuantizedKV
 from .layernorm import LayerNorm, LayerNormTH, normalize_inplace, normalizeTH
 from .mask import mask, mask_inplace, maskTH
 from .position_embedding import PositionEmbedding, PositionEmbeddingTH
+from .rotary import RotaryEmbedding, RotaryEmbeddingTH
 from .softmax import softmax, softmax_inplace, softmaxTH
 from .transpose import transpose, transposeTH
 from .utils import has_nan_inf
 
-# (gelu, mask, softmax and transpose name a function here and a submodule: the function wins)
+# (attention, gelu, mask, softmax and transpose name a function here and a submodule: the function wins)
 __all__ = sorted(n for n, v in list(globals().items()) if not n.startswith("_") and type(v).__name__ != "module")

@@ -11,6 +11,14 @@ def cur_stream() -> int:
     return _raw_stream(_device())
 
 
+def current_device(device):
+    """`device`, which has to be the current one: kernels are launched there."""
+    assert device.type == "cuda", "not on a GPU"
+    here = _device() if _device is not None and torch.cuda.is_initialized() else torch.cuda.current_device()
+    assert device.index == here, "the tensors lie on another device than the current one"
+    return device
+
+
 def check_half(x: torch.Tensor, ndim=None):
     assert x.is_cuda and x.is_contiguous() and x.dtype == torch.float16
     if ndim is not None:

@@ -1,0 +1,146 @@
+"""Attention over fp16 queries, keys and values without scores in memory, with gradients.  What ``bmm``, a position bias, ``mask``, ``softmax`` and ``bmm`` do one after
+another (the sequence of the reference's models), in one pass; for training, for chunks of a prompt and for single tokens over a cache of fp16.
+
+    out = attention(q, k, v, causal=True)                               # (batch, heads, tokens, dim), any strides
+    out = attention(q, k, v, lens=lens, pos=pos)                        # a decode step over the first lens keys of a buffer
+    out = attention(q, k, v, pos=0, bias=pe.weight, mapping=mapping)    # with PositionEmbedding's biases, which get gradients too
+
+Activations of this package are (batch, heads * dim_head, tokens): ``x.view(batch, heads, dim_head, tokens).transpose(2, 3)`` is what goes in, and the result and the
+gradients have the same layout in memory.
+"""
+import math
+from functools import lru_cache
+
+import torch
+from torch.autograd.function import once_differentiable
+from ..library import cpmk          # (the launchers themselves: what the kernels layer checks is checked here)
+from ._common import cur_stream, current_device
+from .kv_cache import _each
+
+MAX_DIM, MAX_DISTANCES = 256, 1024
+
+
+@lru_cache(maxsize=1024)
+def _workspace(device, *sizes):         # (how keys are divided depends on the device's number of compute units; the call costs more than the look-up)
+    return cpmk.attention_forward_workspace(*sizes)
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.preserve_format)
+
+
+class OpAttention(torch.autograd.Function):
+    """forward: one pass over the keys; backward: the probabilities computed again from what the forward pass kept of each row, the log of its sum."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, mapping, mask, lens, pos, scale, causal, bidirectional, keep):
+        batch, heads, tokens, dim = q.shape
+        kv_heads, length = k.size(1), k.size(2)
+        lens_each, keys = _each(lens, batch, q.device)
+        pos_each, first = _each(-1 if pos is None else pos, batch, q.device)
+        sizes = (batch, heads, kv_heads, tokens, dim, length)
+        rows = (lens_each, keys, pos_each, first, int(causal), scale)
+        table = (None, None, 0, 0, 0) if bias is None else (bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0), int(bidirectional))
+        seen = (None, 0, 0) if mask is None else (mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0)
+        out = _like(q)
+        lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if keep else None
+        size = _workspace(q.device.index, *sizes)
+        space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
+                               lse.data_ptr() if keep else None, space.data_ptr() if size else None, cur_stream())
+        if keep:
+            each = [x if isinstance(x, torch.Tensor) else None for x in (lens, pos)]
+            ctx.save_for_backward(q, k, v, bias, mapping, mask, out, lse, *each)
+            ctx.plain = (sizes, keys, first, int(causal), scale, table, seen)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, bias, mapping, mask, out, lse, lens, pos = ctx.saved_tensors
+        (batch, heads, kv_heads, tokens, dim, length), keys, first, causal, scale, table, seen = ctx.plain
+        current_device(q.device)
+        assert dout.dtype == torch.float16
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
+        if batch * heads * dim == 0:
+            return (dq, dk, dv, None if dbias is None else dbias.zero_()) + (None,) * 8
+        size = cpmk.attention_backward_workspace(batch, heads, kv_heads, tokens, length, 0 if dbias is None else mapping.size(0), table[4])
+        space = torch.empty(max(size, 4), dtype=torch.uint8, device=q.device)
+        cpmk.attention_backward(batch, heads, kv_heads, tokens, dim, length, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(),
+                                None if lens is None else lens.data_ptr(), keys, None if pos is None else pos.data_ptr(), first, causal, scale, *table, *seen,
+                                out.data_ptr(), *out.stride(), lse.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(),
+                                dv.data_ptr(), *dv.stride(), None if dbias is None else dbias.data_ptr(), space.data_ptr(), cur_stream())
+        return (dq, dk, dv, dbias) + (None,) * 8
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens=None, scale: float = None, causal: bool = True, pos=None, mask: torch.Tensor = None,
+              bias: torch.Tensor = None, mapping: torch.Tensor = None, bidirectional: bool = False) -> torch.Tensor:
+    """softmax(scale q k^T + position bias) v, with gradients to q, k, v and bias.  The arguments are those of QuantizedKV.attention.
+
+    q (batch, heads, queries, dim), k and v (batch, kv heads, length, dim), heads a multiple of the kv heads (neighbouring ones share a head of keys); scale: dim ** -0.5.
+    lens: the first lens keys of every sequence count (an int, or an int32 tensor with one for each; None: all).
+    pos: the first query's position (int, int32 tensor, or None: the queries are the last of the lens keys; sequences padded at their end want pos=0 with their lens);
+    causal: keys behind a query's position do not count.
+    mask: bool (batch, length) or (batch, 1 or queries, length), True where a key counts.  A query without keys gives zeros, and no gradients.
+    bias, mapping, bidirectional: PositionEmbedding's weight (heads, num_buckets) and the table of position_embedding_init.
+    The result has the shape of q, and its layout where q is dense; so have the gradients theirs."""
+    device = current_device(q.device)
+    for x in (q, k, v):
+        assert x.ndim == 4 and x.dtype == torch.float16 and x.device == device
+    batch, heads, queries, dim = q.shape
+    assert k.shape == v.shape and k.size(0) == batch and k.size(3) == dim and dim <= MAX_DIM
+    kv_heads, length = k.size(1), k.size(2)
+    assert (heads % kv_heads == 0) if kv_heads else heads == 0
+    if lens is None:
+        lens = length
+    lens_each, keys = _each(lens, batch, device)
+    assert lens_each is not None or 0 <= keys <= length, "more keys than there are"
+    if pos is not None:
+        pos_each, first = _each(pos, batch, device)
+        assert pos_each is not None or 0 <= first < 2 ** 30
+    scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
+    assert math.isfinite(scale)
+    if mask is not None:
+        assert mask.dtype == torch.bool and mask.device == device
+        if mask.ndim == 2:
+            mask = mask[:, None]
+        assert mask.ndim == 3 and mask.shape[::2] == (batch, length) and mask.size(1) in (1, queries)
+        assert mask.stride(2) == 1 or length <= 1
+    if bias is not None:
+        assert bias.dtype == torch.float16 and bias.ndim == 2 and bias.size(0) == heads and bias.size(1) > 0 and bias.is_contiguous() and bias.device == device
+        assert mapping is not None and mapping.dtype == torch.int32 and mapping.ndim == 1 and mapping.is_contiguous() and mapping.device == device
+        assert 0 < mapping.size(0) * (2 if bidirectional else 1) <= MAX_DISTANCES
+    wanted = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
+    return OpAttention.apply(q, k, v, bias, mapping, mask, lens, pos, scale, bool(causal), bool(bidirectional), wanted)
+
+
+def attentionTH(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens=None, scale: float = None, causal: bool = True, pos=None, mask: torch.Tensor = None,
+                bias: torch.Tensor = None, mapping: torch.Tensor = None, bidirectional: bool = False) -> torch.Tensor:
+    """Plain-torch formulation of the same, in fp32 (fp64 for fp64 tensors)."""
+    batch, heads, queries, dim = q.shape
+    kv_heads, length = k.size(1), k.size(2)
+    wide = torch.promote_types(q.dtype, torch.float32)
+
+    def each(x):
+        return x.long() if isinstance(x, torch.Tensor) else torch.full((batch,), int(x), dtype=torch.long, device=q.device)
+    lens = each(length if lens is None else lens).clamp(0, length)
+    at = (lens - queries if pos is None else each(pos))[:, None] + torch.arange(queries, device=q.device)
+    key, value = (x.to(wide).repeat_interleave(heads // kv_heads, 1) for x in (k, v))
+    scores = torch.matmul(q.to(wide), key.transpose(2, 3)) * (dim ** -0.5 if scale is None else scale)
+    index = torch.arange(length, device=q.device)
+    rel = at[:, :, None] - index
+    if bias is not None:
+        far = rel.abs() if bidirectional else rel.clamp(min=0)
+        bucket = mapping.long()[far.clamp(max=mapping.size(0) - 1)].clamp(max=bias.size(1))
+        if bidirectional:
+            bucket = bucket + torch.where(rel < 0, bias.size(1) // 2, 0)
+        scores = scores + bias.to(wide)[:, bucket.clamp(0, bias.size(1) - 1)].transpose(0, 1)
+    seen = (index < lens[:, None])[:, None].expand_as(rel)
+    if causal:
+        seen = seen & (rel >= 0)
+    if mask is not None:
+        seen = seen & (mask[:, None] if mask.ndim == 2 else mask)
+    seen = seen[:, None]
+    p = torch.softmax(scores.masked_fill(~seen, -1e30), 3) * seen
+    return torch.matmul(p, value).to(q.dtype)

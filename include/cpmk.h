@@ -517,6 +517,55 @@ int cpmk_kv_attention_int8(int32_t batch, int32_t heads, int32_t kv_heads, int32
                            void* workspace, void* stream);
 int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length);
 
+/* ---- attention over fp16 keys and values, its gradients, rotary positions (no counterpart in the reference, whose kernels keep the scores in memory) ----
+ * The fp16 tensors (batch, heads, tokens, dim) come with the strides of their axes, in elements.  dim at most 256, tokens and length at most 2^29. */
+
+/* out[b,h,i,:] = sum_j p_j v_j, p = softmax over j of scale * q[b,h,i,:] . k_j + bias[h, bucket(at - j)], query head h on head h / (heads / kv_heads) of the
+ * keys, at = the query's position: pos_each[b] + i, or pos + i, or, with a negative pos, lens[b] - tokens + i.  Key j of `length` counts where
+ * j < lens_each[b] (or len), j <= at if causal, and mask[b * mask_batch + i * mask_token + j] != 0 if there is a mask (rows of `length` bytes; a
+ * mask_token of 0 for one row a sequence).  A query that no key is left for gives zeros.  What lies in keys and values that a query does not see, numbers or
+ * not, does not reach its result.  bias: the table of cpmk_position_embedding_forward, buckets as there (mapping of cpmk_position_embedding_init; a bucket
+ * number outside of the table counts as the nearest in it), at most 1024 distances (both signs counted if bidirectional); NULL for none.
+ * lse: (batch, heads, tokens) fp32, log2 of the sum of exp2(log2(e) * score), +inf of a query without keys, or NULL.
+ * workspace: cpmk_attention_forward_workspace() bytes on the device, 4-byte aligned, the call's own until it has finished; NULL if that is 0. */
+int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length,
+                           const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
+                           const void* k /* fp16 */, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit,
+                           const void* v /* fp16 */, int64_t v_batch, int64_t v_head, int64_t v_token, int64_t v_unit,
+                           const void* lens_each /* (batch) int32 or NULL */, int32_t len, const void* pos_each /* (batch) int32 or NULL */, int32_t pos,
+                           int causal, float scale, const void* bias /* (heads, num_buckets) fp16 or NULL */, const void* mapping /* (max_distance) int32 */,
+                           int32_t num_buckets, int32_t max_distance, int bidirectional,
+                           const void* mask /* bool or NULL */, int64_t mask_batch, int64_t mask_token,
+                           void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit,
+                           void* lse, void* workspace, void* stream);
+int64_t cpmk_attention_forward_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length);
+/* The gradients of q, k, v (dq, dk, dv: fp16, written whole, zeros where nothing was seen) and, unless dbias is NULL, of the table (heads, num_buckets) of biases, from that of
+ * the result (dout) and the forward call's arguments, out and lse.  No atomics on sums: the same call gives the same bits.
+ * workspace: cpmk_attention_backward_workspace() bytes, 4-byte aligned (max_distance: 0 without dbias), the call's own until it has finished. */
+int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length,
+                            const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
+                            const void* k /* fp16 */, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit,
+                            const void* v /* fp16 */, int64_t v_batch, int64_t v_head, int64_t v_token, int64_t v_unit,
+                            const void* lens_each, int32_t len, const void* pos_each, int32_t pos, int causal, float scale, const void* bias, const void* mapping,
+                            int32_t num_buckets, int32_t max_distance, int bidirectional, const void* mask, int64_t mask_batch, int64_t mask_token,
+                            const void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit, const void* lse,
+                            const void* dout /* fp16 */, int64_t dout_batch, int64_t dout_head, int64_t dout_token, int64_t dout_unit,
+                            void* dq /* fp16 */, int64_t dq_batch, int64_t dq_head, int64_t dq_token, int64_t dq_unit,
+                            void* dk /* fp16 */, int64_t dk_batch, int64_t dk_head, int64_t dk_token, int64_t dk_unit,
+                            void* dv /* fp16 */, int64_t dv_batch, int64_t dv_head, int64_t dv_token, int64_t dv_unit,
+                            void* dbias /* (heads, num_buckets) fp16 or NULL */, void* workspace, void* stream);
+int64_t cpmk_attention_backward_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t length, int32_t max_distance, int bidirectional);
+/* Rotary positions of queries and keys (heads_k 0: queries alone): pair i of `part` units (even) turned by position * turns[i] of a whole turn (the other way if `inverse`: the
+ * gradient) and multiplied by magnitude, the pairs being units 2 i and 2 i + 1 (interleaved) or i and i + part / 2; other units are copied.  Position of token t:
+ * positions[b * pos_batch + t * pos_token], or, with a pos_token of 0, positions[b * pos_batch] + t, or, without positions, pos + t.  Outputs may be the inputs themselves. */
+int cpmk_rotary(int32_t batch, int32_t tokens, int32_t dim, int32_t part, int interleaved,
+                int32_t heads_q, const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
+                void* q_out /* fp16 */, int64_t qo_batch, int64_t qo_head, int64_t qo_token, int64_t qo_unit,
+                int32_t heads_k, const void* k /* fp16 */, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit,
+                void* k_out /* fp16 */, int64_t ko_batch, int64_t ko_head, int64_t ko_token, int64_t ko_unit,
+                const void* turns /* (part / 2) fp64 */, const void* positions /* int32 or NULL */, int64_t pos_batch, int64_t pos_token, int32_t pos,
+                float magnitude, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
