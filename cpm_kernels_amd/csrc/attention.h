@@ -19,6 +19,7 @@ struct Attention {
     const uint8_t* mask;
     int64_t mask_batch, mask_token;
     float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; or null
+    half_t* rest;                   // with lse: what the rounding of `out` left, times 2^11, under the same strides
     float* parts;
     float scale;                    // with log2(e)
     int32_t len, pos;               // pos < 0: the queries are the last of the keys
@@ -233,9 +234,16 @@ __device__ __forceinline__ uint32_t attn_mask4(const uint8_t* row, int32_t key, 
     return m;
 }
 
-// A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times f, as fp16
-template <int NT>
+constexpr float kRest = 2048.0f;        // fp16 has 11 bits: what a rounding leaves, times this, is as large as the number at most
+
+// A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times f, as fp16; or, REST, what that rounding leaves
+template <int NT, bool REST = false>
 __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, const float16_tv (&acc)[NT], float f, int dim, int half) {
+    const auto rounded = [&](float x) {
+        x *= f;
+        const half_t r = round_f16(x);
+        return REST ? (half_t)((x - (float)r) * kRest) : r;
+    };
     if (t.unit == 1 && dim % 4 == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -243,7 +251,7 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, con
             for (int c = 0; c < 4; ++c) {
                 half4_t v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (half_t)(acc[n][c * 4 + e] * f);
+                for (int e = 0; e < 4; ++e) v[e] = rounded(acc[n][c * 4 + e]);
                 const int u = n * 32 + c * 8 + half * 4;
                 if (u < dim) *reinterpret_cast<Half4Any*>(row + u) = __builtin_bit_cast(Half4Any, v);
             }
@@ -253,7 +261,7 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, con
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int u = n * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
-                if (u < dim) row[u * t.unit] = (half_t)(acc[n][i] * f);
+                if (u < dim) row[u * t.unit] = rounded(acc[n][i]);
             }
     }
 }

@@ -8,7 +8,8 @@
 // A workgroup has 128 queries of a head, 32 a wave, and goes over its keys in tiles of 64 that all its waves read from LDS.  Scores are formed transposed (keys as rows), so a lane holds
 // keys of one query, and its probabilities, rounded to fp16, are the second product's operand as they are.  fp16 keeps their bits: they are at most 2^15 and their maximum is 2^7 at least
 // (the running maximum follows the true one at a distance of up to 2^8), so what falls below fp16's normal range is less than 2^-21 of the row's largest.  Sums are fp32, of the
-// unrounded probabilities.  Where there are few rows the keys are cut into parts, which k_attn_join adds up.
+// unrounded probabilities.  For training (TRAIN) what their rounding leaves is multiplied by the values as well, and what the result's rounding leaves is kept: the
+// backward pass subtracts two nearly equal numbers where a query looks at one key, do_i v_j and do_i out_i, and the second has to be as exact as the first.  Where there are few rows the keys are cut into parts, which k_attn_join adds up.
 #include <algorithm>
 #include "attention.h"
 
@@ -31,7 +32,7 @@ __device__ __forceinline__ AttnParts attn_parts(const Attention& a, const AttnRa
     return p;
 }
 
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool PLAIN, int LAY, bool TRAIN>
 __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys and values, biases
@@ -158,15 +159,20 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    half8_t p;
+                    half8_t p, left;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][e * 8 + j], factor, shift));
                         sum += x;
                         p[j] = (half_t)x;
+                        if (TRAIN) left[j] = (half_t)(x - (float)p[j]);
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_units<D>(value_tile, at_units, n, blk, e), p, acc[n], 0, 0, 0);
+                    for (int n = 0; n < NT; ++n) {
+                        const half8_t v = attn_units<D>(value_tile, at_units, n, blk, e);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, acc[n], 0, 0, 0);
+                        if (TRAIN) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, left, acc[n], 0, 0, 0);
+                    }
                 }
         }
         if (t + 1 < t_end) {
@@ -200,7 +206,9 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     attn_write<NT>(a.out, a.out.at(b, h) + query * a.out.token, acc, inv, a.dim, half);
-    if (a.lse && half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
+    if (!TRAIN) return;
+    attn_write<NT, true>(a.out, a.rest + b * a.out.batch + h * a.out.head + query * a.out.token, acc, inv, a.dim, half);
+    if (half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
 }
 
 // Parts joined under the largest of their maxima: a wave a row, its lanes along the units.
@@ -250,7 +258,13 @@ __global__ __launch_bounds__(256) void k_attn_join(Attention a, uint32_t total_r
     half_t* const out = a.out.at(b, h) + query * a.out.token;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.dim) out[(int64_t)(c * 64 + lane) * a.out.unit] = (half_t)(total == 0.0f ? 0.0f : value[c] / total);
+        if (c * 64 + lane < a.dim) {
+            const int64_t at = (int64_t)(c * 64 + lane) * a.out.unit;
+            const float x = total == 0.0f ? 0.0f : value[c] / total;
+            const half_t r = round_f16(x);
+            out[at] = r;
+            if (a.lse) a.rest[out - a.out.p + at] = (half_t)((x - (float)r) * kRest);
+        }
     if (a.lse && lane == 0) a.lse[id] = total == 0.0f ? __builtin_inff() : base - kLift + __builtin_amdgcn_logf(total);
 }
 
@@ -266,14 +280,18 @@ static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t tokens, int64_t 
     return p;
 }
 
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool PLAIN, int LAY, bool TRAIN>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY>, 150 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY>), dim3(grid), dim3(256), lds, st, a);
+    if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY, TRAIN>, 150 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid), dim3(256), lds, st, a);
     return 0;
+}
+template <int NT, bool PLAIN, int LAY>
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, st);
 }
 template <int NT, bool PLAIN>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
@@ -302,7 +320,7 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
                            int64_t q_unit, const void* k, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit, const void* v, int64_t v_batch, int64_t v_head, int64_t v_token,
                            int64_t v_unit, const void* lens_each, int32_t len, const void* pos_each, int32_t pos, int causal, float scale, const void* bias, const void* mapping,
                            int32_t num_buckets, int32_t max_distance, int bidirectional, const void* mask, int64_t mask_batch, int64_t mask_token, void* out, int64_t out_batch,
-                           int64_t out_head, int64_t out_token, int64_t out_unit, void* lse, void* workspace, void* stream) {
+                           int64_t out_head, int64_t out_token, int64_t out_unit, void* lse, void* rest, void* workspace, void* stream) {
     clear_stale_error();
     Attention a;
     a.q = {(half_t*)q, q_batch, q_head, q_token, q_unit}, a.k = {(half_t*)k, k_batch, k_head, k_token, k_unit}, a.v = {(half_t*)v, v_batch, v_head, v_token, v_unit};
@@ -310,11 +328,12 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
     a.lens_each = (const int32_t*)lens_each, a.pos_each = (const int32_t*)pos_each, a.len = len, a.pos = pos;
     a.table = (const half_t*)bias, a.mapping = (const int32_t*)mapping, a.buckets = num_buckets, a.distances = max_distance;
     a.mask = (const uint8_t*)mask, a.mask_batch = mask_batch, a.mask_token = mask_token;
-    a.lse = (float*)lse, a.scale = scale * kLog2e, a.causal = causal != 0;
+    a.lse = (float*)lse, a.rest = (half_t*)rest, a.scale = scale * kLog2e, a.causal = causal != 0;
     a.tokens = tokens, a.dim = dim, a.length = length;
     bool empty;
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty || tokens == 0) return 0;
+    if (lse && !rest) return CPMK_EBADARG;
     const AttnPlan plan = attn_plan(batch, heads, tokens, length);
     a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;

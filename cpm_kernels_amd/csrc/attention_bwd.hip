@@ -43,23 +43,24 @@ __global__ __launch_bounds__(256) void k_attn_facts(AttentionGrad a, uint32_t qu
     const int32_t t = tile * 64 + mine;
     float square = 0.0f, dot = 0.0f;
     if (t < tokens) {
-        const half_t *const px = x.at(b, h) + t * x.token, *const py = y.at(b, h) + t * y.token;
+        const half_t *const px = x.at(b, h) + t * x.token, *const py = y.at(b, h) + t * y.token, *const pr = a.rest + (py - y.p);
         for (int u = part * 8; u < a.dim; u += 32) {
-            half8_t vx, vy = {0, 0, 0, 0, 0, 0, 0, 0};
+            half8_t vx, vy = {0, 0, 0, 0, 0, 0, 0, 0}, vr = vy;
             if (x.unit == 1 && u + 8 <= a.dim) vx = load_half8_any(px + u);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) vx[e] = u + e < a.dim ? px[(u + e) * x.unit] : (half_t)0;
             if (of_queries) {
-                if (y.unit == 1 && u + 8 <= a.dim) vy = load_half8_any(py + u);
+                if (y.unit == 1 && u + 8 <= a.dim) vy = load_half8_any(py + u), vr = load_half8_any(pr + u);
                 else
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) vy[e] = u + e < a.dim ? py[(u + e) * y.unit] : (half_t)0;
+                    for (int e = 0; e < 8; ++e)
+                        if (u + e < a.dim) vy[e] = py[(u + e) * y.unit], vr[e] = pr[(u + e) * y.unit];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 square = __builtin_fmaf((float)vx[e], (float)vx[e], square);
-                dot = __builtin_fmaf((float)vx[e], (float)vy[e], dot);
+                dot = __builtin_fmaf((float)vx[e], __builtin_fmaf((float)vr[e], 1.0f / kRest, (float)vy[e]), dot);
             }
         }
     }
@@ -485,7 +486,7 @@ int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int3
                             int64_t q_unit, const void* k, int64_t k_batch, int64_t k_head, int64_t k_token, int64_t k_unit, const void* v, int64_t v_batch, int64_t v_head, int64_t v_token,
                             int64_t v_unit, const void* lens_each, int32_t len, const void* pos_each, int32_t pos, int causal, float scale, const void* bias, const void* mapping,
                             int32_t num_buckets, int32_t max_distance, int bidirectional, const void* mask, int64_t mask_batch, int64_t mask_token, const void* out, int64_t out_batch,
-                            int64_t out_head, int64_t out_token, int64_t out_unit, const void* lse, const void* dout, int64_t dout_batch, int64_t dout_head, int64_t dout_token,
+                            int64_t out_head, int64_t out_token, int64_t out_unit, const void* lse, const void* rest, const void* dout, int64_t dout_batch, int64_t dout_head, int64_t dout_token,
                             int64_t dout_unit, void* dq, int64_t dq_batch, int64_t dq_head, int64_t dq_token, int64_t dq_unit, void* dk, int64_t dk_batch, int64_t dk_head, int64_t dk_token,
                             int64_t dk_unit, void* dv, int64_t dv_batch, int64_t dv_head, int64_t dv_token, int64_t dv_unit, void* dbias, void* workspace, void* stream) {
     clear_stale_error();
@@ -496,12 +497,12 @@ int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int3
     a.lens_each = (const int32_t*)lens_each, a.pos_each = (const int32_t*)pos_each, a.len = len, a.pos = pos;
     a.table = (const half_t*)bias, a.mapping = (const int32_t*)mapping, a.buckets = num_buckets, a.distances = max_distance, a.dtable = (half_t*)dbias;
     a.mask = (const uint8_t*)mask, a.mask_batch = mask_batch, a.mask_token = mask_token;
-    a.lse = (float*)lse, a.scale = scale * kLog2e, a.natural_scale = scale, a.causal = causal != 0;
+    a.lse = (float*)lse, a.rest = (half_t*)rest, a.scale = scale * kLog2e, a.natural_scale = scale, a.causal = causal != 0;
     a.tokens = tokens, a.dim = dim, a.length = length, a.splits = 1, a.parts = nullptr;
     bool empty;
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty) return 0;
-    if ((tokens > 0 && any_null(lse, dout, dq)) || (length > 0 && any_null(dk, dv)) || !workspace || (dbias && !bias)) return CPMK_EBADARG;
+    if ((tokens > 0 && any_null(lse, rest, dout, dq)) || (length > 0 && any_null(dk, dv)) || !workspace || (dbias && !bias)) return CPMK_EBADARG;
     a.row_tiles = (int32_t)ceil_div(tokens, kGradRows), a.query_tiles = (int32_t)ceil_div(tokens, kAttnTile), a.key_tiles = (int32_t)ceil_div(length, kAttnTile);
     const int64_t query_blocks = (int64_t)batch * heads * a.query_tiles, key_blocks = (int64_t)batch * kv_heads * a.key_tiles;
     if (!grid_fits(query_blocks + key_blocks)) return CPMK_ETOOBIG;

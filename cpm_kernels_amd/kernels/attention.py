@@ -36,13 +36,14 @@ def attention_forward(batch: int, heads: int, kv_heads: int, tokens: int, dim: i
                       mask: DevicePointer, mask_batch: int, mask_token: int,      # rows of length bools, strides in bytes; or None
                       out: DevicePointer, out_strides: Strides,      # (batch, heads, tokens, dim)  fp16
                       lse: DevicePointer,                            # (batch, heads, tokens)  fp32, or None
+                      rest: DevicePointer,                           # fp16 under out's strides, or None: with lse, for attention_backward
                       workspace: DevicePointer,                      # attention_forward_workspace() bytes
                       stream: CUDAStream):
     """softmax(scale q k^T + position bias) v; queries without a key give zeros."""
     _check(heads, kv_heads, dim)
     cpmk.attention_forward(batch, heads, kv_heads, tokens, dim, length, q, *q_strides, k, *k_strides, v, *v_strides, lens_each, len, pos_each, pos,
                            int(bool(causal)), scale, bias, mapping, num_buckets, max_distance, int(bool(bidirectional)), mask, mask_batch, mask_token,
-                           out, *out_strides, lse, workspace, stream)
+                           out, *out_strides, lse, rest, workspace, stream)
 
 
 def attention_backward(batch: int, heads: int, kv_heads: int, tokens: int, dim: int, length: int,
@@ -51,7 +52,7 @@ def attention_backward(batch: int, heads: int, kv_heads: int, tokens: int, dim: 
                        bias: DevicePointer, mapping: DevicePointer, num_buckets: int, max_distance: int, bidirectional: bool,
                        mask: DevicePointer, mask_batch: int, mask_token: int,
                        out: DevicePointer, out_strides: Strides,      # (batch, heads, tokens, dim)  fp16, of attention_forward
-                       lse: DevicePointer,                            # (batch, heads, tokens)  fp32, of attention_forward
+                       lse: DevicePointer, rest: DevicePointer,       # (batch, heads, tokens)  fp32; fp16 under out's strides; of attention_forward
                        dout: DevicePointer, dout_strides: Strides,    # (batch, heads, tokens, dim)  fp16
                        dq: DevicePointer, dq_strides: Strides,        # (batch, heads, tokens, dim)  fp16
                        dk: DevicePointer, dk_strides: Strides,        # (batch, kv_heads, length, dim)  fp16
@@ -63,7 +64,7 @@ def attention_backward(batch: int, heads: int, kv_heads: int, tokens: int, dim: 
     _check(heads, kv_heads, dim)
     cpmk.attention_backward(batch, heads, kv_heads, tokens, dim, length, q, *q_strides, k, *k_strides, v, *v_strides, lens_each, len, pos_each, pos,
                             int(bool(causal)), scale, bias, mapping, num_buckets, max_distance, int(bool(bidirectional)), mask, mask_batch, mask_token,
-                            out, *out_strides, lse, dout, *dout_strides, dq, *dq_strides, dk, *dk_strides, dv, *dv_strides, dbias, workspace, stream)
+                            out, *out_strides, lse, rest, dout, *dout_strides, dq, *dq_strides, dk, *dk_strides, dv, *dv_strides, dbias, workspace, stream)
 
 
 def rotary_forward(batch: int, tokens: int, dim: int, part: int, interleaved: bool,

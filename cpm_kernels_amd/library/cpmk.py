@@ -42,8 +42,8 @@ _LAUNCHERS = {
     "transpose": "iiippp", "transpose_i8": "iiippp", "array_add": "piip", "adjustify_logits": "iipfffpp",
     "copy_extend_buffer": "iiippp",
     "kv_write_int8": "iiiiiipllllpllllpipppppp", "kv_read_int8": "iiiiiipppppippllllp", "kv_attention_int8": "iiiiiiipllllpppppipiifppiiipllpllllpp",
-    "attention_forward": "iiiiiipllllpllllpllllpipiifppiiipllpllllppp",
-    "attention_backward": "iiiiiipllllpllllpllllpipiifppiiipllpllllppllllpllllpllllpllllppp",
+    "attention_forward": "iiiiiipllllpllllpllllpipiifppiiipllpllllpppp",
+    "attention_backward": "iiiiiipllllpllllpllllpipiifppiiipllpllllpppllllpllllpllllpllllppp",
     "rotary": "iiiiiipllllpllllipllllpllllppllifip",
     "has_nan_inf": "lppp", "copy_pos_hidden": "iiiippp", "async_status": "",
     "selftest_exchange_timeout": "ip",

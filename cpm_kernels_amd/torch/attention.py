@@ -30,7 +30,8 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 
 
 class OpAttention(torch.autograd.Function):
-    """forward: one pass over the keys; backward: the probabilities computed again from what the forward pass kept of each row, the log of its sum."""
+    """forward: one pass over the keys; backward: the probabilities computed again from what the forward pass kept of each row, the log
+    of its sum and what its result's rounding left."""
 
     @staticmethod
     def forward(ctx, q, k, v, bias, mapping, mask, lens, pos, scale, causal, bidirectional, keep):
@@ -43,21 +44,21 @@ class OpAttention(torch.autograd.Function):
         table = (None, None, 0, 0, 0) if bias is None else (bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0), int(bidirectional))
         seen = (None, 0, 0) if mask is None else (mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0)
         out = _like(q)
-        lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if keep else None
+        lse, rest = (torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
         size = _workspace(q.device.index, *sizes)
         space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
-                               lse.data_ptr() if keep else None, space.data_ptr() if size else None, cur_stream())
+                               lse.data_ptr() if keep else None, rest.data_ptr() if keep else None, space.data_ptr() if size else None, cur_stream())
         if keep:
             each = [x if isinstance(x, torch.Tensor) else None for x in (lens, pos)]
-            ctx.save_for_backward(q, k, v, bias, mapping, mask, out, lse, *each)
+            ctx.save_for_backward(q, k, v, bias, mapping, mask, out, lse, rest, *each)
             ctx.plain = (sizes, keys, first, int(causal), scale, table, seen)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, bias, mapping, mask, out, lse, lens, pos = ctx.saved_tensors
+        q, k, v, bias, mapping, mask, out, lse, rest, lens, pos = ctx.saved_tensors
         (batch, heads, kv_heads, tokens, dim, length), keys, first, causal, scale, table, seen = ctx.plain
         current_device(q.device)
         assert dout.dtype == torch.float16
@@ -69,7 +70,7 @@ class OpAttention(torch.autograd.Function):
         space = torch.empty(max(size, 4), dtype=torch.uint8, device=q.device)
         cpmk.attention_backward(batch, heads, kv_heads, tokens, dim, length, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(),
                                 None if lens is None else lens.data_ptr(), keys, None if pos is None else pos.data_ptr(), first, causal, scale, *table, *seen,
-                                out.data_ptr(), *out.stride(), lse.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(),
+                                out.data_ptr(), *out.stride(), lse.data_ptr(), rest.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(),
                                 dv.data_ptr(), *dv.stride(), None if dbias is None else dbias.data_ptr(), space.data_ptr(), cur_stream())
         return (dq, dk, dv, dbias) + (None,) * 8
 

@@ -526,7 +526,8 @@ int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t k
  * mask_token of 0 for one row a sequence).  A query that no key is left for gives zeros.  What lies in keys and values that a query does not see, numbers or
  * not, does not reach its result.  bias: the table of cpmk_position_embedding_forward, buckets as there (mapping of cpmk_position_embedding_init; a bucket
  * number outside of the table counts as the nearest in it), at most 1024 distances (both signs counted if bidirectional); NULL for none.
- * lse: (batch, heads, tokens) fp32, log2 of the sum of exp2(log2(e) * score), +inf of a query without keys, or NULL.
+ * lse: (batch, heads, tokens) fp32, log2 of the sum of exp2(log2(e) * score), +inf of a query without keys, or NULL; with it rest: fp16 under out's strides, what the
+ * rounding of out left, times 2^11.  Both are for cpmk_attention_backward.
  * workspace: cpmk_attention_forward_workspace() bytes on the device, 4-byte aligned, the call's own until it has finished; NULL if that is 0. */
 int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length,
                            const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
@@ -537,10 +538,10 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
                            int32_t num_buckets, int32_t max_distance, int bidirectional,
                            const void* mask /* bool or NULL */, int64_t mask_batch, int64_t mask_token,
                            void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit,
-                           void* lse, void* workspace, void* stream);
+                           void* lse, void* rest, void* workspace, void* stream);
 int64_t cpmk_attention_forward_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length);
 /* The gradients of q, k, v (dq, dk, dv: fp16, written whole, zeros where nothing was seen) and, unless dbias is NULL, of the table (heads, num_buckets) of biases, from that of
- * the result (dout) and the forward call's arguments, out and lse.  No atomics on sums: the same call gives the same bits.
+ * the result (dout) and the forward call's arguments, out, lse and rest.  No atomics on sums: the same call gives the same bits.
  * workspace: cpmk_attention_backward_workspace() bytes, 4-byte aligned (max_distance: 0 without dbias), the call's own until it has finished. */
 int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length,
                             const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
@@ -548,7 +549,7 @@ int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int3
                             const void* v /* fp16 */, int64_t v_batch, int64_t v_head, int64_t v_token, int64_t v_unit,
                             const void* lens_each, int32_t len, const void* pos_each, int32_t pos, int causal, float scale, const void* bias, const void* mapping,
                             int32_t num_buckets, int32_t max_distance, int bidirectional, const void* mask, int64_t mask_batch, int64_t mask_token,
-                            const void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit, const void* lse,
+                            const void* out /* fp16 */, int64_t out_batch, int64_t out_head, int64_t out_token, int64_t out_unit, const void* lse, const void* rest,
                             const void* dout /* fp16 */, int64_t dout_batch, int64_t dout_head, int64_t dout_token, int64_t dout_unit,
                             void* dq /* fp16 */, int64_t dq_batch, int64_t dq_head, int64_t dq_token, int64_t dq_unit,
                             void* dk /* fp16 */, int64_t dk_batch, int64_t dk_head, int64_t dk_token, int64_t dk_unit,

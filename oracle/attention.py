@@ -31,8 +31,8 @@ def attention(q, k, v, lens, first, scale, causal, mask=None, table=None, mappin
     """q (batch, heads, n, dim), k, v (batch, held, length, dim), lens and first (batch) integers, mask (batch, rows, length) or None.
     Without dout (out, bound); with it lists of (out, dq, dk, dv[, dtable]) and of their bounds.
 
-    Roundings: scores are fp32 sums of dim products; exponents and exponentials fp32; probabilities and the scores' gradients rounded to fp16, the first beside a power of two that keeps
-    them above 2^-8 of their row's largest... times 2^-24 absolutely, the second beside one that brings 2 |dout| max |v| to 2^15; sums fp32; results, the one that D is made of too, fp16."""
+    Roundings: scores are fp32 sums of dim products; exponents and exponentials fp32; probabilities and the scores' gradients rounded to fp16, the first beside a power of two that makes
+    their row's largest 2^7 at least, the second beside one that brings 2 |dout| max |v| to 2^15; sums fp32; results fp16, D from what their rounding left too."""
     q, k, v = (np.asarray(x, f64) for x in (q, k, v))
     batch, heads, n, dim = q.shape
     length, group = k.shape[2], heads // max(k.shape[1], 1)
@@ -74,11 +74,13 @@ def attention(q, k, v, lens, first, scale, causal, mask=None, table=None, mappin
                 continue
             G = np.where(empty, 0, dout[b, h])
             dp = np.where(seen, G @ np.where(seen.any(0)[:, None], V, 0).T, 0)
-            D = (G * o).sum(1, keepdims=True)
+            D = (G * o).sum(1, keepdims=True)           # of a result whose roundings were kept: fp32, but for 2^-11 of 2^-11
+            least = count * 2.0 ** -32 * p.max(1, initial=0, keepdims=True) * np.abs(Vs).max(0, initial=0)[None]
+            bD = weight * (2 * off + 2.0 ** -21 + 2 * (count + 64) * E32) + least + np.abs(o) * 2.0 ** -21 + 2.0 ** -36
             ds = p * (dp - D)
             e_p = p * (2 * off + 2.0 ** -21)                        # of a probability before it is rounded
             e_dp = (np.abs(G) @ np.abs(Vs).T) * (dim + 8) * E32
-            e_D = (np.abs(G) * bo).sum(1, keepdims=True) + (np.abs(G) * np.abs(o)).sum(1, keepdims=True) * (dim + 8) * E32
+            e_D = (np.abs(G) * bD).sum(1, keepdims=True) + (np.abs(G) * np.abs(o)).sum(1, keepdims=True) * (dim + 8) * E32
             e_ds = np.where(seen, e_p * np.abs(dp - D) + p * (e_dp + e_D), 0)
             norms = np.sqrt((G ** 2).sum(1, keepdims=True))
             vtop = np.sqrt((v[b, h // group] ** 2).sum(1)).max(initial=0) if np.isfinite(v[b, h // group]).all() else np.sqrt((Vs ** 2).sum(1)).max(initial=0)
