@@ -45,6 +45,27 @@ __device__ __forceinline__ AttnRange attn_range(const Attention& a, int64_t b) {
     return r;
 }
 
+// The keys that a tile of rows looks at, and the parts they are cut into (the same here and where the parts are joined): `least` tiles each at least.
+struct AttnParts {
+    int32_t keys, tiles, per_part, parts;
+};
+__device__ __forceinline__ AttnParts attn_parts(const Attention& a, const AttnRange& r, int32_t last_query, int least, int tile) {
+    AttnParts p;
+    p.keys = a.causal ? max(0, min(r.len, r.pos + last_query + 1)) : r.len;
+    p.tiles = (p.keys + tile - 1) / tile;
+    p.per_part = max((p.tiles + a.splits - 1) / a.splits, min(least, max(p.tiles, 1)));
+    p.parts = max(1, (p.tiles + p.per_part - 1) / p.per_part);
+    return p;
+}
+
+// How a call is divided: rows of a workgroup, workgroups of rows, parts of the keys (of `least` tiles of `tile` keys at least), waves of a workgroup; few: attention_few.hip.
+struct AttnPlan {
+    int rows, row_tiles, splits, tile, least, waves;
+    bool few;
+};
+AttnPlan attn_few_plan(int64_t batch, int64_t held, int64_t of_head, int32_t dim, int64_t length);
+int attn_few_launch(const Attention& a, const AttnPlan& p, int32_t batch, hipStream_t st);
+
 // The bucket of a distance (query - key) first_distance .. distances - 1; others are as those at the ends.  With biases for both signs first_distance is -1 at least: a key behind
 // the query takes the upper half of the buckets however short the table is.  Numbers of buckets that the table does not have count as the nearest that it has.
 __device__ __forceinline__ int32_t attn_bucket(const Attention& a, int32_t rel) {

@@ -19,19 +19,6 @@ constexpr int kAttnRows = 128, kAttnLeast = 4;       // queries of a workgroup; 
 constexpr int kLazy = 8;            // log2 of how far the running maximum may lie below the true one
 constexpr float kLift = 7.0f;       // log2 of the largest probability's size right behind a change of the maximum
 
-// The keys that a tile of rows looks at, and the parts they are cut into (the same here and where the parts are joined).
-struct AttnParts {
-    int32_t keys, tiles, per_part, parts;
-};
-__device__ __forceinline__ AttnParts attn_parts(const Attention& a, const AttnRange& r, int32_t last_query, int least) {
-    AttnParts p;
-    p.keys = a.causal ? max(0, min(r.len, r.pos + last_query + 1)) : r.len;
-    p.tiles = (p.keys + kAttnTile - 1) / kAttnTile;
-    p.per_part = max((p.tiles + a.splits - 1) / a.splits, min(least, max(p.tiles, 1)));
-    p.parts = max(1, (p.tiles + p.per_part - 1) / p.per_part);
-    return p;
-}
-
 template <int NT, bool PLAIN, int LAY, bool TRAIN>
 __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
@@ -51,7 +38,7 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
     const int32_t qt = a.row_tiles - 1 - (int32_t)(w % (uint32_t)a.row_tiles);
     const int32_t h = kvh * a.group + w / (uint32_t)a.row_tiles;
     const AttnRange range = attn_range(a, b);
-    const AttnParts parts = attn_parts(a, range, min(qt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast);
+    const AttnParts parts = attn_parts(a, range, min(qt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast, kAttnTile);
     if (split >= parts.parts) return;
 
     const int32_t q_first = qt * kAttnRows + wave * 32;
@@ -211,21 +198,21 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
     if (half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
 }
 
-// Parts joined under the largest of their maxima: a wave a row, its lanes along the units.
-__global__ __launch_bounds__(256) void k_attn_join(Attention a, uint32_t total_rows) {
-    const int lane = threadIdx.x & 63;
+// Parts joined under the largest of their maxima: a wave a row, its lanes along the units.  `rows` of them lie together: queries of a head, or (few) rows of a head of keys.
+__global__ __launch_bounds__(256) void k_attn_join(Attention a, AttnPlan plan, uint32_t total_rows) {
+    const int lane = threadIdx.x & 63, rows = plan.rows;
     const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= total_rows) return;
-    const int32_t query = id % (uint32_t)a.tokens;
-    const uint32_t bh = id / (uint32_t)a.tokens;
-    const int64_t b = bh / (uint32_t)a.heads;
-    const int32_t h = bh - (uint32_t)b * a.heads;
-    const int32_t rt = query / kAttnRows, r = query - rt * kAttnRows;
+    const int32_t group = plan.few ? a.group : 1, heads = plan.few ? a.held : a.heads, of_head = a.tokens * group;
+    const int32_t in_head = id % (uint32_t)of_head;
+    const uint32_t bh = id / (uint32_t)of_head;
+    const int64_t b = bh / (uint32_t)heads;
+    const int32_t rt = in_head / rows, r = in_head - rt * rows, query = in_head / group, h = (bh - (uint32_t)b * heads) * group + in_head - query * group;
     const AttnRange range = attn_range(a, b);
-    const AttnParts p = attn_parts(a, range, min(rt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast);
-    const int64_t size = (int64_t)kAttnRows * (a.dim + 2);
+    const AttnParts p = attn_parts(a, range, min(rt * rows + rows - 1, of_head - 1) / group, plan.least, plan.tile);
+    const int64_t size = (int64_t)rows * (a.dim + 2);
     const float* const part = a.parts + ((int64_t)bh * a.row_tiles + rt) * a.splits * size;
-    const float* const tops = part + kAttnRows * a.dim + r;
+    const float* const tops = part + rows * a.dim + r;
     float m = -__builtin_inff();
     for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, tops[i * size]);
     m = wave_max(m);
@@ -236,7 +223,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Attention a, uint32_t total_r
         const bool real = first + lane < p.parts;
         const float* const mine = tops + (first + (real ? lane : 0)) * size;
         const float weight = real ? __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
-        total = __builtin_fmaf(real ? mine[kAttnRows] : 0.0f, weight, total);
+        total = __builtin_fmaf(real ? mine[rows] : 0.0f, weight, total);
         const int n = min(64, p.parts - first);
         for (int i = 0; i < n; i += 8) {
             float x[8][4];
@@ -265,15 +252,19 @@ __global__ __launch_bounds__(256) void k_attn_join(Attention a, uint32_t total_r
             out[at] = r;
             if (a.lse) a.rest[out - a.out.p + at] = (half_t)((x - (float)r) * kRest);
         }
-    if (a.lse && lane == 0) a.lse[id] = total == 0.0f ? __builtin_inff() : base - kLift + __builtin_amdgcn_logf(total);
+    if (a.lse && lane == 0) a.lse[(b * a.heads + h) * a.tokens + query] = total == 0.0f ? __builtin_inff() : base - kLift + __builtin_amdgcn_logf(total);
 }
 
-// Into how many parts the keys are cut: as many as let the device's compute units each have a workgroup, of four tiles at least; none where rows are many.
-struct AttnPlan {
-    int row_tiles, splits;
-};
-static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t tokens, int64_t length) {
+// Which kernel a call takes, and how it is divided.  Keys are cut into as many parts as let the device's compute units each have a workgroup, of four tiles at least.
+static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length, bool rows_of_keys, bool train) {
+    const int64_t of_head = tokens * (heads / held);
+    if (rows_of_keys && !train && of_head <= 32 && dim % 8 == 0 && length > 0) {
+        AttnPlan p = attn_few_plan(batch, held, of_head, dim, length);
+        p.few = true;
+        return p;
+    }
     AttnPlan p;
+    p.few = false, p.rows = kAttnRows, p.waves = 4, p.tile = kAttnTile, p.least = kAttnLeast;
     p.row_tiles = (int)ceil_div(tokens, kAttnRows);
     const int64_t base = batch * heads * p.row_tiles, tiles = ceil_div(length, kAttnTile), units = compute_units();
     p.splits = (int)std::max<int64_t>(1, std::min(2 * units / base, tiles / kAttnLeast));
@@ -309,11 +300,16 @@ using namespace cpmk;
 
 extern "C" {
 
+// (enough for either kernel: which one a call takes depends on its strides too)
 int64_t cpmk_attention_forward_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length) {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || dim <= 0 || length <= 0 || heads % kv_heads) return 0;
     if (dim > 256 || tokens > kAttnLong || length > kAttnLong || !grid_fits((int64_t)batch * heads)) return 0;
-    const AttnPlan p = attn_plan(batch, heads, tokens, length);
-    return p.splits > 1 ? (int64_t)batch * heads * p.row_tiles * p.splits * kAttnRows * (dim + 2) * (int64_t)sizeof(float) : 0;
+    int64_t most = 0;
+    for (int few = 0; few < 2; ++few) {
+        const AttnPlan p = attn_plan(batch, heads, kv_heads, tokens, dim, length, few, false);
+        if (p.splits > 1) most = std::max(most, (int64_t)batch * (p.few ? kv_heads : heads) * p.row_tiles * p.splits * p.rows * (dim + 2) * (int64_t)sizeof(float));
+    }
+    return most;
 }
 
 int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length, const void* q, int64_t q_batch, int64_t q_head, int64_t q_token,
@@ -334,16 +330,20 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty || tokens == 0) return 0;
     if (lse && !rest) return CPMK_EBADARG;
-    const AttnPlan plan = attn_plan(batch, heads, tokens, length);
+    const AttnPlan plan = attn_plan(batch, heads, kv_heads, tokens, dim, length, k_unit == 1 && v_unit == 1, lse != nullptr);
     a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;
     const int64_t grid = (int64_t)batch * heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
     if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
     hipStream_t st = (hipStream_t)stream;
     const unsigned g = (unsigned)grid;
-    const int e = dim <= 64 ? attn_launch<2>(a, g, st) : dim <= 96 ? attn_launch<3>(a, g, st) : dim <= 128 ? attn_launch<4>(a, g, st) : attn_launch<8>(a, g, st);
+    const int e = plan.few    ? attn_few_launch(a, plan, batch, st)
+                  : dim <= 64 ? attn_launch<2>(a, g, st)
+                  : dim <= 96 ? attn_launch<3>(a, g, st)
+                  : dim <= 128 ? attn_launch<4>(a, g, st)
+                               : attn_launch<8>(a, g, st);
     if (e) return e;
-    if (a.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, (uint32_t)rows);
+    if (a.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan, (uint32_t)rows);
     return launch_status();
 }
 
