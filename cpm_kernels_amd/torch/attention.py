@@ -12,12 +12,14 @@ import math
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from ..library import cpmk          # (the launchers themselves: what the kernels layer checks is checked here)
 from ._common import cur_stream, current_device
 from .kv_cache import _each
 
 MAX_DIM, MAX_DISTANCES = 256, 1024
+_NO_MASK, _NO_TABLE = (None, 0, 0), (None, None, 0, 0, 0)
 
 
 @lru_cache(maxsize=1024)
@@ -25,8 +27,15 @@ def _workspace(device, *sizes):         # (how keys are divided depends on the d
     return cpmk.attention_forward_workspace(*sizes)
 
 
-def _like(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(x, memory_format=torch.preserve_format)
+def _forward(q, k, v, table, seen, rows, sizes, keep):
+    """(result, what the backward pass needs besides it)"""
+    out = torch.empty_like(q)
+    lse, rest = (torch.empty(sizes[:2] + sizes[3:4], dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
+    size = _workspace(q.device.index, *sizes)
+    space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
+                           lse.data_ptr() if keep else None, rest.data_ptr() if keep else None, space.data_ptr() if size else None, cur_stream())
+    return out, lse, rest
 
 
 class OpAttention(torch.autograd.Function):
@@ -34,44 +43,29 @@ class OpAttention(torch.autograd.Function):
     of its sum and what its result's rounding left."""
 
     @staticmethod
-    def forward(ctx, q, k, v, bias, mapping, mask, lens, pos, scale, causal, bidirectional, keep):
-        batch, heads, tokens, dim = q.shape
-        kv_heads, length = k.size(1), k.size(2)
-        lens_each, keys = _each(lens, batch, q.device)
-        pos_each, first = _each(-1 if pos is None else pos, batch, q.device)
-        sizes = (batch, heads, kv_heads, tokens, dim, length)
-        rows = (lens_each, keys, pos_each, first, int(causal), scale)
-        table = (None, None, 0, 0, 0) if bias is None else (bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0), int(bidirectional))
-        seen = (None, 0, 0) if mask is None else (mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0)
-        out = _like(q)
-        lse, rest = (torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
-        size = _workspace(q.device.index, *sizes)
-        space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
-                               lse.data_ptr() if keep else None, rest.data_ptr() if keep else None, space.data_ptr() if size else None, cur_stream())
-        if keep:
-            each = [x if isinstance(x, torch.Tensor) else None for x in (lens, pos)]
-            ctx.save_for_backward(q, k, v, bias, mapping, mask, out, lse, rest, *each)
-            ctx.plain = (sizes, keys, first, int(causal), scale, table, seen)
+    def forward(ctx, q, k, v, bias, mapping, mask, lens, pos, table, seen, rows, sizes):
+        out, lse, rest = _forward(q, k, v, table, seen, rows, sizes, True)
+        ctx.save_for_backward(q, k, v, bias, mapping, mask, out, lse, rest, lens, pos)       # (lens and pos too: the kernels look at them again)
+        ctx.plain = (sizes, rows, table, seen)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, bias, mapping, mask, out, lse, rest, lens, pos = ctx.saved_tensors
-        (batch, heads, kv_heads, tokens, dim, length), keys, first, causal, scale, table, seen = ctx.plain
+        q, k, v, bias, mapping, _, out, lse, rest, _, _ = ctx.saved_tensors
+        sizes, rows, table, seen = ctx.plain
+        batch, heads, kv_heads, tokens, dim, length = sizes
         current_device(q.device)
         assert dout.dtype == torch.float16
-        dq, dk, dv = _like(q), _like(k), _like(v)
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
         if batch * heads * dim == 0:
             return (dq, dk, dv, None if dbias is None else dbias.zero_()) + (None,) * 8
         size = cpmk.attention_backward_workspace(batch, heads, kv_heads, tokens, length, 0 if dbias is None else mapping.size(0), table[4])
         space = torch.empty(max(size, 4), dtype=torch.uint8, device=q.device)
-        cpmk.attention_backward(batch, heads, kv_heads, tokens, dim, length, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(),
-                                None if lens is None else lens.data_ptr(), keys, None if pos is None else pos.data_ptr(), first, causal, scale, *table, *seen,
-                                out.data_ptr(), *out.stride(), lse.data_ptr(), rest.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(),
-                                dv.data_ptr(), *dv.stride(), None if dbias is None else dbias.data_ptr(), space.data_ptr(), cur_stream())
+        cpmk.attention_backward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
+                                lse.data_ptr(), rest.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(), dv.data_ptr(), *dv.stride(),
+                                None if dbias is None else dbias.data_ptr(), space.data_ptr(), cur_stream())
         return (dq, dk, dv, dbias) + (None,) * 8
 
 
@@ -87,33 +81,37 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens=None, scal
     bias, mapping, bidirectional: PositionEmbedding's weight (heads, num_buckets) and the table of position_embedding_init.
     The result has the shape of q, and its layout where q is dense; so have the gradients theirs."""
     device = current_device(q.device)
-    for x in (q, k, v):
-        assert x.ndim == 4 and x.dtype == torch.float16 and x.device == device
+    assert q.dtype == k.dtype == v.dtype == torch.float16 and k.device == device and v.device == device
     batch, heads, queries, dim = q.shape
-    assert k.shape == v.shape and k.size(0) == batch and k.size(3) == dim and dim <= MAX_DIM
-    kv_heads, length = k.size(1), k.size(2)
+    shape = k.shape
+    assert v.shape == shape and len(shape) == 4 and shape[0] == batch and shape[3] == dim and dim <= MAX_DIM
+    kv_heads, length = shape[1:3]
     assert (heads % kv_heads == 0) if kv_heads else heads == 0
-    if lens is None:
-        lens = length
-    lens_each, keys = _each(lens, batch, device)
+    lens_each, keys = (None, length) if lens is None else _each(lens, batch, device)
     assert lens_each is not None or 0 <= keys <= length, "more keys than there are"
-    if pos is not None:
-        pos_each, first = _each(pos, batch, device)
-        assert pos_each is not None or 0 <= first < 2 ** 30
+    pos_each, first = (None, -1) if pos is None else _each(pos, batch, device)
+    assert pos is None or pos_each is not None or 0 <= first < 2 ** 30
     scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
     assert math.isfinite(scale)
+    seen, table = _NO_MASK, _NO_TABLE
     if mask is not None:
         assert mask.dtype == torch.bool and mask.device == device
         if mask.ndim == 2:
             mask = mask[:, None]
         assert mask.ndim == 3 and mask.shape[::2] == (batch, length) and mask.size(1) in (1, queries)
         assert mask.stride(2) == 1 or length <= 1
+        seen = (mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0)
     if bias is not None:
         assert bias.dtype == torch.float16 and bias.ndim == 2 and bias.size(0) == heads and bias.size(1) > 0 and bias.is_contiguous() and bias.device == device
         assert mapping is not None and mapping.dtype == torch.int32 and mapping.ndim == 1 and mapping.is_contiguous() and mapping.device == device
         assert 0 < mapping.size(0) * (2 if bidirectional else 1) <= MAX_DISTANCES
-    wanted = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
-    return OpAttention.apply(q, k, v, bias, mapping, mask, lens, pos, scale, bool(causal), bool(bidirectional), wanted)
+        table = (bias.data_ptr(), mapping.data_ptr(), bias.size(1), mapping.size(0), int(bool(bidirectional)))
+    rows = (lens_each, keys, pos_each, first, int(bool(causal)), scale)
+    sizes = (batch, heads, kv_heads, queries, dim, length)
+    # (an autograd function costs 5 us of the host's time, as much as a step's kernel; one with forward-mode tangents goes through it all the same, and is refused there)
+    if getattr(forward_ad, "_current_level", 0) < 0 and not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))):
+        return _forward(q, k, v, table, seen, rows, sizes, False)[0]
+    return OpAttention.apply(q, k, v, bias, mapping, mask, lens if lens_each is not None else None, pos if pos_each is not None else None, table, seen, rows, sizes)
 
 
 def attentionTH(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens=None, scale: float = None, causal: bool = True, pos=None, mask: torch.Tensor = None,

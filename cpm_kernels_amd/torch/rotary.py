@@ -9,6 +9,7 @@ a bias to the scores; the reference has no counterpart.
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from ..library import cpmk
 from ._common import cur_stream, current_device
@@ -112,7 +113,12 @@ class RotaryEmbedding(torch.nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor = None, pos=0):
         """q (batch, heads, tokens, dim), k (batch, any heads, tokens, dim) or None: turned copies of them, in their layouts where they are dense."""
         pos = self._check(q, k, pos)
-        out = OpRotary.apply(self, pos, q, k)
+        # (an autograd function costs 5 us of the host's time, as much as a step's kernel; one with forward-mode tangents goes through it all the same, and is refused there)
+        if getattr(forward_ad, "_current_level", 0) < 0 and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+            out = torch.empty_like(q), None if k is None else torch.empty_like(k)
+            _launch(self, (q, k), out, pos, False)
+        else:
+            out = OpRotary.apply(self, pos, q, k)
         return out[0] if k is None else out
 
     @torch.no_grad()
