@@ -18,7 +18,9 @@ struct Attention {
     const int32_t* mapping;
     const uint8_t* mask;
     int64_t mask_batch, mask_token;
-    float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; or null
+    float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; behind them (batch, held, key tiles): the largest norm
+                                    // of a tile's values, squared; or null
+    int64_t rows_in_all;
     half_t* rest;                   // with lse: what the rounding of `out` left, times 2^11, under the same strides
     float* parts;
     float scale;                    // with log2(e)
@@ -175,58 +177,82 @@ struct AttnShare {
         }
     }
 
-    // Zeros where there is nothing; with `guard` numbers that are none or infinite become zeros as well, and their tokens are entered in `bad` as those of tile `stamp`
-    __device__ __forceinline__ void clean(int dim, int32_t t0, int32_t tokens, int tid, bool guard, int32_t* bad, int32_t stamp) {
+    // Into LDS, zeros where there is nothing.  With `guard` numbers that are none or infinite become zeros as well, and their tokens' bits are set in `bad`: a product with a probability
+    // of 0 would not be 0, and must not reach the tokens that do not see these.
+    __device__ __forceinline__ void store(int8_t* tile, int dim, int32_t t0, int32_t tokens, int tid, bool guard, uint32_t* bad) {
         const bool whole = t0 + kAttnTile <= tokens && D == dim;
-        if (whole && !guard) return;
-        half8_t worst = {0, 0, 0, 0, 0, 0, 0, 0};
-        const half8_t none = worst;
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+        const int run = tid % RUN, first = LAY == kColumns ? (tid & 7) * 8 : tid / RUN, u0 = (tid >> 3) * PIECES;
+        if (!whole)
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            int units, at;      // how many of the eight are real
-            if constexpr (LAY == kColumns) {
-                at = (tid & 7) * 8;
-                units = (tid >> 3) * PIECES + i < dim ? max(0, min(8, tokens - t0 - at)) : 0;
-            } else {
-                at = tid / RUN + i * STEP;
-                units = t0 + at < tokens ? max(0, min(8, dim - (tid % RUN) * 8)) : 0;
+            for (int i = 0; i < PIECES; ++i) {
+                const int units = LAY == kColumns ? (u0 + i < dim ? tokens - t0 - first : 0) : (t0 + first + i * STEP < tokens ? dim - run * 8 : 0);       // how many of the eight are real
+                r[i] = half8_fill(r[i], half8_keep(units), none);
             }
-            r[i] = half8_fill(r[i], half8_keep(units), none);
-            worst = __builtin_elementwise_fma(r[i], none, worst);
-        }
-        if (!guard) return;
         bool any = false;
+        if (guard) {
+            half8_t worst = none;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) any |= !(worst[e] == (half_t)0);
-        if (__builtin_amdgcn_ballot_w64(any) == 0) return;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(r[i][e] * (half_t)0 == (half_t)0)) {
-                    r[i][e] = (half_t)0;
-                    bad[LAY == kColumns ? (tid & 7) * 8 + e : tid / RUN + i * STEP] = stamp;
-                    bad[kAttnTile] = stamp;
-                }
-    }
-
-    __device__ __forceinline__ void store(int8_t* tile, int tid) const {
+            for (int i = 0; i < PIECES; ++i) worst = __builtin_elementwise_fma(r[i], none, worst);
+            const uint4_t w = __builtin_bit_cast(uint4_t, worst);
+            any = ((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu) != 0;
+        }
         if constexpr (LAY == kColumns) {
-            const int u0 = (tid >> 3) * PIECES;
-            struct Run { half_t u[PIECES]; };
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int t = (tid & 7) * 8 + e;
-                typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
                 run_t v;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) v[i] = r[i][e];
-                *reinterpret_cast<run_t*>(tile + attn_place<D>(t, u0 >> 3) + (u0 & 7) * 2) = v;
+                *reinterpret_cast<run_t*>(tile + attn_place<D>(first + e, u0 >> 3) + (u0 & 7) * 2) = v;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) *reinterpret_cast<half8_t*>(tile + attn_place<D>(tid / RUN + i * STEP, tid % RUN)) = r[i];
+            for (int i = 0; i < PIECES; ++i) *reinterpret_cast<half8_t*>(tile + attn_place<D>(first + i * STEP, run)) = r[i];
         }
+        if (any) {          // (rare: what the thread has just written is looked through again)
+#pragma unroll 1
+            for (int i = 0; i < (LAY == kColumns ? 8 : PIECES); ++i) {
+                const int token = LAY == kColumns ? first + i : first + i * STEP;
+                half_t* const p = reinterpret_cast<half_t*>(tile + attn_place<D>(token, LAY == kColumns ? u0 >> 3 : run)) + (LAY == kColumns ? u0 & 7 : 0);
+#pragma unroll 1
+                for (int e = 0; e < (LAY == kColumns ? PIECES : 8); ++e)
+                    if (!(p[e] * (half_t)0 == (half_t)0)) {
+                        p[e] = (half_t)0;
+                        atomicOr(bad + (token >> 5), 1u << (token & 31));
+                    }
+            }
+        }
+    }
+    typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
+};
+
+// 32 bytes of a row of a mask as bits, on their way from memory
+struct AttnMaskShare {
+    uint4_t raw[2];
+    __device__ __forceinline__ void load(const uint8_t* row, int32_t key, int32_t length) {
+        struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
+        if (length < 32) return;
+        const uint8_t* const p = row + min(key, length - 32);
+        raw[0] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(p));
+        raw[1] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(p + 16));
+    }
+    __device__ __forceinline__ uint32_t bits(const uint8_t* row, int32_t key, int32_t length) const {
+        uint32_t all = 0;
+        if (length < 32) {
+#pragma unroll 1
+            for (int i = 0; key + i < length; ++i) all |= (row[key + i] != 0 ? 1u : 0u) << i;
+            return all;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint32_t m = raw[i >> 2][i & 3];
+            m |= m >> 4;
+            m |= m >> 2;
+            m |= m >> 1;                    // the lowest bit of a byte: whether any was set
+            all |= ((m & 0x01010101u) * 0x10204080u >> 28) << (4 * i);
+        }
+        const int over = key - min(key, length - 32);
+        return over < 32 ? all >> over : 0u;
     }
 };
 

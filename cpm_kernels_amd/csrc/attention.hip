@@ -19,17 +19,50 @@ constexpr int kAttnRows = 128, kAttnLeast = 4;       // queries of a workgroup; 
 constexpr int kLazy = 8;            // log2 of how far the running maximum may lie below the true one
 constexpr float kLift = 7.0f;       // log2 of the largest probability's size right behind a change of the maximum
 
+// Norms of 64 keys' values, the largest (squared), for the backward pass.
+__device__ __forceinline__ void attn_value_top(const Attention& a, uint32_t id, int tid) {
+    __shared__ float sums[4][64];
+    const uint32_t tiles = (uint32_t)ceil_div(a.length, 64), tile = id % tiles, bh = id / tiles;
+    const int64_t b = bh / (uint32_t)a.held, h = bh % (uint32_t)a.held;
+    const int32_t keys = attn_range(a, b).len;
+    // (four threads a token, in the order in which neighbouring ones read neighbouring addresses)
+    const bool columns = a.v.token == 1;
+    const int mine = columns ? tid & 63 : tid >> 2, share = columns ? tid >> 6 : tid & 3;
+    const int32_t t = tile * 64 + mine;
+    float square = 0.0f;
+    if (t < keys) {
+        const half_t* const p = a.v.at(b, h) + t * a.v.token;
+        if (a.v.unit == 1 && a.dim % 8 == 0) {
+            for (int u = share * 8; u < a.dim; u += 32) {
+                const half8_t x = load_half8_any(p + u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) square = __builtin_fmaf((float)x[e], (float)x[e], square);
+            }
+        } else {
+#pragma unroll 8
+            for (int u = share; u < a.dim; u += 4) square = __builtin_fmaf((float)p[u * a.v.unit], (float)p[u * a.v.unit], square);
+        }
+    }
+    sums[share][mine] = square;
+    __syncthreads();
+    if (tid >= 64) return;
+    square = wave_max((sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]));
+    if (tid == 0) a.lse[a.rows_in_all + id] = square;
+}
+
 template <int NT, bool PLAIN, int LAY, bool TRAIN>
-__global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Attention a) {
+__global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint32_t blocks) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
-    extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys and values, biases
-    __shared__ int32_t bad[2][kAttnTile + 1];
-    float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
+    extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys, two of values, biases
+    __shared__ uint32_t bad[3][2];              // tokens of a tile whose values are no finite numbers; those of tile t in t % 3
+    __shared__ uint32_t mask_bits[2][kAttnRows][2];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (TRAIN && blockIdx.x >= blocks) return attn_value_top(a, blockIdx.x - blocks, tid);
+    float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const uint32_t inner = (uint32_t)a.group * a.row_tiles * a.splits;
     uint32_t unit, w;
-    attn_deal(blockIdx.x, gridDim.x / inner, inner, unit, w);
+    attn_deal(blockIdx.x, blocks / inner, inner, unit, w);
     const int64_t b = unit / (uint32_t)a.held;
     const int32_t kvh = unit - (uint32_t)b * a.held;
     const int32_t split = w % (uint32_t)a.splits;
@@ -52,9 +85,21 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
     const bool flip = a.scale < 0.0f;           // (so that the largest score is the largest product)
     const float scale = flip ? -a.scale : a.scale;
     const bool masked = !PLAIN && a.mask != nullptr, biased = !PLAIN && a.table != nullptr;
-    const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
+    const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + min(qt * kAttnRows + (tid >> 1), a.tokens - 1) * a.mask_token : nullptr;
 
+    // Keys, and the mask's bits, come a tile before the values: scores of the next tile are formed beside this one's sums.
+    const int32_t t_begin = split * parts.per_part, t_end = min(t_begin + parts.per_part, parts.tiles);
+    AttnShare<D, LAY, 256> ks, vs;
+    AttnMaskShare ms;
+    auto load = [&](int32_t t) {
+        if (t + 1 < t_end) {
+            ks.load(keys, a.k.token, a.k.unit, a.dim, (t + 1) * kAttnTile, range.len, tid);
+            if (masked) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
+        }
+        if (t >= t_begin && t < t_end) vs.load(values, a.v.token, a.v.unit, a.dim, t * kAttnTile, range.len, tid);
+    };
+    load(t_begin - 1);
     half8_t q[KS];
     attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
     if (flip)
@@ -62,70 +107,65 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
         for (int s = 0; s < KS; ++s) q[s] = -q[s];
     if (biased) attn_biases(a, h, biases, tid, 256);
     const int32_t lo_rel = a.first_distance - kBiasPad;
-    if (tid <= kAttnTile) bad[0][tid] = bad[1][tid] = -1;
-
-    const int32_t t_begin = split * parts.per_part, t_end = min(t_begin + parts.per_part, parts.tiles);
-    AttnShare<D, LAY, 256> ks, vs;
-    auto load = [&](int32_t t) {
-        ks.load(keys, a.k.token, a.k.unit, a.dim, t * kAttnTile, range.len, tid);
-        vs.load(values, a.v.token, a.v.unit, a.dim, t * kAttnTile, range.len, tid);
-    };
-    auto store = [&](int32_t t) {
-        // (a value that is no finite number must not reach the queries that do not see it)
-        ks.clean(a.dim, t * kAttnTile, range.len, tid, false, nullptr, t);
-        vs.clean(a.dim, t * kAttnTile, range.len, tid, masked || t * kAttnTile + kAttnTile > every_sees, bad[t & 1], t);
-        int8_t* const buffer = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
-        ks.store(buffer, tid);
-        vs.store(buffer + kTileBytes, tid);
-    };
-    if (t_begin < t_end) load(t_begin);
-    __syncthreads();
-    if (t_begin < t_end) {
-        store(t_begin);
-        if (t_begin + 1 < t_end) load(t_begin + 1);
-    }
+    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
     __syncthreads();
 
     const uint32_t at_rows = attn_rows_at<D>(lane), at_units = attn_units_at<D>(lane);
-    float16_tv acc[NT];
+    float16_tv acc[NT], s[2];
+    half8_t p[4], left[TRAIN ? 4 : 1];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = kZero16;
     float top = -__builtin_inff(), sum = 0.0f;
-    for (int32_t t = t_begin; t < t_end; ++t) {
+    auto scores_of = [&](int32_t t) {
+        const int8_t* const tile = lds + (t & 1) * kTileBytes;
+        s[0] = s[1] = kZero16;
+#pragma unroll
+        for (int u = 0; u < KS; ++u)
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) s[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D>(tile, at_rows, blk, u), q[u], s[blk], 0, 0, 0);
+    };
+    auto sums_of = [&](int32_t t) {
+        const int8_t* const tile = lds + (2 + (t & 1)) * kTileBytes;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const half8_t v = attn_units<D>(tile, at_units, n, e >> 1, e & 1);
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[e], acc[n], 0, 0, 0);
+                if (TRAIN) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, left[e], acc[n], 0, 0, 0);
+            }
+    };
+    for (int32_t t = t_begin - 1; t < t_end; ++t) {
         const int32_t k0 = t * kAttnTile;
-        const int8_t* const key_tile = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
-        const int8_t* const value_tile = key_tile + kTileBytes;
-        if (k0 < any_sees) {
-            float16_tv s[2] = {kZero16, kZero16};
-#pragma unroll
-            for (int u = 0; u < KS; ++u)
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk) s[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D>(key_tile, at_rows, blk, u), q[u], s[blk], 0, 0, 0);
+        const bool active = t >= t_begin && k0 < any_sees;
+        if (active) {
             float factor = scale, add = 0.0f;
             // one bias for the whole tile where all its distances lie beyond the table's end
             const int32_t rel_min = range.pos + q_first - (k0 + kAttnTile - 1), rel_max = range.pos + last - k0;
             const bool near = biased && rel_min < a.distances - 1 && rel_max > a.first_distance;
             if (biased && !near) add = biases[(rel_min >= a.distances - 1 ? a.distances - 1 : a.first_distance) - lo_rel];
-            const bool spoilt = bad[t & 1][kAttnTile] == t;
-            if (masked || near || spoilt || k0 + kAttnTile > all_see) {
+            if (near) {
+                const float* const bp = biases + (where - k0 - half * 4 - lo_rel);
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[blk][i] = __builtin_fmaf(s[blk][i], factor, bp[-(blk * 32 + (i >> 2) * 8 + (i & 3))]);
+                factor = 1.0f;
+            }
+            if (k0 + kAttnTile > all_see) {
+                const int32_t seen = limit - k0 - half * 4;
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[blk][i] = blk * 32 + (i >> 2) * 8 + (i & 3) < seen ? s[blk][i] : -__builtin_inff();
+            }
+            if (masked) {
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
+                    const uint32_t bits = mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int32_t key = k0 + blk * 32 + g * 8 + half * 4;
-                        uint32_t keep = 0x01010101u;
-                        if (masked) keep = attn_mask4(mask, key, a.length);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = __builtin_fmaf(s[blk][g * 4 + e], factor, add);
-                            if (near) x += biases[where - key - e - lo_rel];
-                            if (spoilt && bad[t & 1][key + e - k0] == t) x = __builtin_nanf("");
-                            s[blk][g * 4 + e] = key + e < limit && (keep >> (8 * e) & 0xffu) ? x : -__builtin_inff();
-                        }
-                    }
+                    for (int i = 0; i < 16; ++i) s[blk][i] = bits & (1u << ((i >> 2) * 8 + (i & 3))) ? s[blk][i] : -__builtin_inff();
                 }
-                factor = 1.0f;
-                add = 0.0f;
             }
             float m = s[0][0];
 #pragma unroll
@@ -133,7 +173,11 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
 #pragma unroll
                 for (int j = 0; j < 16; ++j) m = fmaxf(m, s[blk][j]);
             m = __builtin_fmaf(m, factor, add);
-            m = fmaxf(m, __shfl_xor(m, 32));
+            {
+                const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+                const uint32_t low = both[0], high = both[1];       // (a bit cast of a vector's element itself takes the first one's)
+                m = fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+            }
             if (__builtin_amdgcn_ballot_w64(m > top + kLazy)) {
                 const float now = fmaxf(m, top), f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
                 top = now;
@@ -143,30 +187,40 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : NT <= 4 ? 2 : 1) void k_attn(Att
             }
             const float shift = add - (top == -__builtin_inff() ? 0.0f : top) + kLift;
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk)
+            for (int e = 0; e < 4; ++e) {
+                float part = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    half8_t p, left;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][e * 8 + j], factor, shift));
-                        sum += x;
-                        p[j] = (half_t)x;
-                        if (TRAIN) left[j] = (half_t)(x - (float)p[j]);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const half8_t v = attn_units<D>(value_tile, at_units, n, blk, e);
-                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, acc[n], 0, 0, 0);
-                        if (TRAIN) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, left, acc[n], 0, 0, 0);
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][(e & 1) * 8 + j], factor, shift));
+                    part += x;
+                    p[e][j] = (half_t)x;
+                    if (TRAIN) left[e][j] = (half_t)(x - (float)p[e][j]);
                 }
+                sum += part;
+            }
         }
         if (t + 1 < t_end) {
-            store(t + 1);
-            if (t + 2 < t_end) load(t + 2);
+            ks.store(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, false, nullptr);
+            if (masked) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         }
+        if (t >= t_begin) vs.store(lds + (2 + (t & 1)) * kTileBytes, a.dim, k0, range.len, tid, masked || k0 + kAttnTile > every_sees, bad[(uint32_t)t % 3]);
+        if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;          // (last looked at two tiles ago)
+        load(t + 1);
         __syncthreads();
+        if (active) {           // (behind the last tile: scores that nobody looks at)
+            const uint32_t spoilt[2] = {bad[(uint32_t)t % 3][0], bad[(uint32_t)t % 3][1]};
+            if (spoilt[0] | spoilt[1]) {        // a query that sees such a key has no number for a result
+                bool sees = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sees |= (spoilt[e >> 1] >> (half * 4 + (e & 1) * 16 + (j >> 2) * 8 + (j & 3)) & 1) && !(p[e][j] == (half_t)0);
+                if (sees) sum = __builtin_nanf("");
+            }
+            sums_of(t);
+            scores_of(t + 1);
+        } else if ((t + 1) * kAttnTile < any_sees && t + 1 < t_end)
+            scores_of(t + 1);
     }
     sum += __shfl_xor(sum, 32);
     if (q_first + col >= a.tokens) return;
@@ -272,26 +326,26 @@ static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t to
 }
 
 template <int NT, bool PLAIN, int LAY, bool TRAIN>
-static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
     if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY, TRAIN>, 150 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid + (TRAIN ? more : 0)), dim3(256), lds, st, a, grid);
     return 0;
 }
 template <int NT, bool PLAIN, int LAY>
-static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
-    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, st);
+static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
+    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, more, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, more, st);
 }
 template <int NT, bool PLAIN>
-static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
     const int lay = attn_layout(a.k, a.v, a.dim);
-    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
+    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, more, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, more, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, more, st);
 }
 template <int NT>
-static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
-    return a.table || a.mask ? attn_launch<NT, false>(a, grid, st) : attn_launch<NT, true>(a, grid, st);
+static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
+    return a.table || a.mask ? attn_launch<NT, false>(a, grid, more, st) : attn_launch<NT, true>(a, grid, more, st);
 }
 
 }  // namespace cpmk
@@ -334,14 +388,17 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
     a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;
     const int64_t grid = (int64_t)batch * heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
-    if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
+    const int64_t key_tiles = lse ? (int64_t)batch * kv_heads * ceil_div(length, kAttnTile) : 0;
+    if (!grid_fits(grid + key_tiles) || !grid_fits(rows)) return CPMK_ETOOBIG;
+    a.rows_in_all = rows;
+    const unsigned more = (unsigned)key_tiles;
     hipStream_t st = (hipStream_t)stream;
     const unsigned g = (unsigned)grid;
     const int e = plan.few    ? attn_few_launch(a, plan, batch, st)
-                  : dim <= 64 ? attn_launch<2>(a, g, st)
-                  : dim <= 96 ? attn_launch<3>(a, g, st)
-                  : dim <= 128 ? attn_launch<4>(a, g, st)
-                               : attn_launch<8>(a, g, st);
+                  : dim <= 64 ? attn_launch<2>(a, g, more, st)
+                  : dim <= 96 ? attn_launch<3>(a, g, more, st)
+                  : dim <= 128 ? attn_launch<4>(a, g, more, st)
+                               : attn_launch<8>(a, g, more, st);
     if (e) return e;
     if (a.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan, (uint32_t)rows);
     return launch_status();

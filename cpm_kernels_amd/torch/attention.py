@@ -30,7 +30,9 @@ def _workspace(device, *sizes):         # (how keys are divided depends on the d
 def _forward(q, k, v, table, seen, rows, sizes, keep):
     """(result, what the backward pass needs besides it)"""
     out = torch.empty_like(q)
-    lse, rest = (torch.empty(sizes[:2] + sizes[3:4], dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
+    batch, heads, kv_heads, tokens, _, length = sizes
+    # (a number for each row, and one for each tile of 64 keys)
+    lse, rest = (torch.empty(batch * (heads * tokens + kv_heads * ((length + 63) // 64)), dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
     size = _workspace(q.device.index, *sizes)
     space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
