@@ -98,42 +98,48 @@ __device__ __forceinline__ void attn_deal(uint32_t x, uint32_t units, uint32_t i
 }
 
 // ---- tiles of 64 tokens in LDS -----------------------------------------------------------------------------------------------
-// A tile lies token by token, D units (64, 128 or 256) each, in pieces of eight units; piece c of token t at place c ^ swizzle(t) within its group of eight.  An operand of the matrix
-// instructions is read in one of two ways: eight units of a token a lane (16 bytes; 8 neighbouring lanes have neighbouring tokens, whose swizzles differ), or, transposed, four tokens of a
-// unit a lane (ds_read_b64_tr_b16: 16 lanes hand in the addresses of four tokens' 32 bytes, whose swizzles differ in the bits above the lowest).  Tokens 8 apart differ too: a thread that
-// brings eight tokens of a unit writes to them one after another, beside its neighbours'.
-__device__ __forceinline__ int attn_swizzle(int token) { return (((token & 3) << 1) | ((token >> 2) & 1)) ^ ((token >> 3) & 7); }
-
+// A tile lies token by token, D units (64, 128 or 256) each, in pieces of eight units; piece c of token t at place c ^ swizzle(t) within its group of 16 (8 of 64 units): the 64 banks hold one
+// token of 128 units or two of 64.  An operand of the matrix instructions is read in one of two ways, each free of conflicts: eight units of a token a lane (16 bytes; sixteen neighbouring
+// lanes have neighbouring tokens, whose places differ), or, transposed, four tokens of a unit a lane (ds_read_b64_tr_b16: 16 lanes hand in the addresses of four tokens' 32 bytes; the places
+// of 32 lanes' four tokens differ in the bits above the lowest two).  A thread that brings eight tokens of some units writes to them one after another, beside its neighbours', whose tokens
+// are 8 apart: their places differ above the lowest bit.
+template <int D>
+__device__ __forceinline__ int attn_swizzle(int t) {
+    const int r0 = t & 1, r1 = t >> 1 & 1, r2 = t >> 2 & 1, r3 = t >> 3 & 1, r4 = t >> 4 & 1, r5 = t >> 5 & 1;
+    return D == 64 ? (r1 ^ r4) << 2 | r3 << 1 | (r2 ^ r5) : (r1 ^ r4) << 3 | (r0 ^ r5) << 2 | r3 << 1 | r2;
+}
 template <int D>
 __device__ __forceinline__ int attn_place(int token, int piece) {
-    return token * D * 2 + (((piece & ~7) | ((piece ^ attn_swizzle(token)) & 7)) << 4);
+    constexpr int W = D == 64 ? 8 : 16;
+    return token * D * 2 + (((piece & ~(W - 1)) | ((piece ^ attn_swizzle<D>(token)) & (W - 1))) << 4);
 }
 
-// Lane's address for operands of rows = tokens: piece 2 s + half of token (lane & 31) + 32 blk is at (rows ^ ((2 s & 7) << 4 ^ blk << 6)) + blk * 32 rows + (s >> 2) * 128.
+// Lane's address for operands of rows = tokens, piece 2 s + half of token (lane & 31) + 32 blk
 template <int D>
 __device__ __forceinline__ uint32_t attn_rows_at(int lane) {
     const int t = lane & 31;
-    return t * D * 2 + (((lane >> 5) ^ attn_swizzle(t)) << 4);
+    return t * D * 2 + (((lane >> 5) ^ attn_swizzle<D>(t)) << 4);
 }
 template <int D>
 __device__ __forceinline__ half8_t attn_rows(const int8_t* tile, uint32_t at, int blk, int s) {
-    return *reinterpret_cast<const half8_t*>(tile + ((at ^ (((2 * s) & 7) << 4) ^ (blk << 6)) + blk * 32 * D * 2 + (s >> 2) * 128));
+    const int x = D == 64 ? (2 * s) ^ blk : ((2 * s) & 15) ^ (blk << 2);
+    return *reinterpret_cast<const half8_t*>(tile + ((at ^ (x << 4)) + blk * 32 * D * 2 + (D == 256 ? (s >> 3) * 256 : 0)));
 }
 // Lane's address for operands of rows = units: of unit block n (32 units), tokens 32 blk + 16 e + 4 half + {0..3, 8..11}: the order in which the results of a product with tokens as
 // rows lie in a lane's registers 8 e .. 8 e + 7.
 template <int D>
 __device__ __forceinline__ uint32_t attn_units_at(int lane) {
     const int half = lane >> 5, j = lane & 15, c = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1), t = 4 * half + (j >> 2);
-    return t * D * 2 + ((c ^ ((j >> 2) << 1 | half)) << 4) + (j & 1) * 8;
+    return t * D * 2 + ((c ^ attn_swizzle<D>(t)) << 4) + (j & 1) * 8;
 }
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 template <int D>
 __device__ __forceinline__ half8_t attn_units(const int8_t* tile, uint32_t at, int n, int blk, int e) {
-    const int x = ((n & 1) << 2) ^ (blk << 2) ^ (e << 1);
-    const int8_t* const p = tile + (blk * 32 + e * 16) * D * 2 + (n >> 1) * 128;
+    const int x = D == 64 ? (n << 2) ^ (e << 2) ^ blk : ((n & 3) << 2) ^ (e << 3) ^ (blk << 2);
+    const int8_t* const p = tile + (blk * 32 + e * 16) * D * 2 + (D == 256 ? (n >> 2) * 256 : 0);
     const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + (at ^ (x << 4))));
-    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + 8 * D * 2 + (at ^ ((x ^ 1) << 4))));
+    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + 8 * D * 2 + (at ^ ((x ^ 2) << 4))));
     return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 

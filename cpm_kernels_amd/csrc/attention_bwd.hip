@@ -26,6 +26,8 @@ struct AttentionGrad : Attention {
 
 constexpr int kGradRows = 128;      // queries (k_attn_dq) or keys (k_attn_dkv) of a workgroup
 constexpr float kProbScale = 15.0f;
+template <int NT>
+constexpr int kDiagonals = (NT <= 4 ? 32 : 4) * 36 + 32;         // floats of a wave's buffer for diagonals: rows of 36, read up to 31 before and behind
 
 // The largest of n numbers, for the whole wave
 __device__ __forceinline__ float attn_largest(const float* x, int64_t n, int lane) {
@@ -95,6 +97,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     if (table_wanted)
         for (int i = tid; i < 4 * entries; i += 256) biases[entries + i] = 0.0f;
     const int32_t lo_rel = a.first_distance - kBiasPad;
+    constexpr int DIAG = NT <= 4 ? 32 : 4;          // rows of a block that are summed along their diagonals at a time (256 units leave no more LDS)
+    float* const diagonals = biases + 5 * ((entries + 3) & ~3) + wave * kDiagonals<NT>;
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
 
     half8_t q[KS], g[KS];
@@ -172,6 +176,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], a.scale, add);
         const int32_t of_lane = where - k0 - half * 4 - lo_rel;
+        const int32_t rel_of_corner = range.pos + q_first - k0 - 31 - lo_rel;        // distance of the block's first query from its last key
         if (near) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] += biases[of_lane - ((i >> 2) * 8 + (i & 3))];
@@ -195,14 +200,28 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]) * __builtin_fmaf(dp[i], dscale, minus_delta);
         if (table_wanted) {
             if (near) {
-                // (32 lanes, 32 distances: no two meet, and no other wave; a wave's operations on LDS keep their order, so each sum's terms do)
-                float* const sum = sums + of_lane;
-                if (real && half == 0)
+                // Through LDS: a lane writes its 16 keys beside each other, a row a query, and then sums a diagonal, lane l that of distance l - 31 from the block's corner.  (64 float
+                // additions in LDS itself, which has an instruction for them, took ten times as long as the block's products.)  All of it is the wave's own.
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) atomicAdd(sum - (i >> 2) * 8 - (i & 3), s[i] * undo);
-                if (real && half == 1)
+                for (int pass = 0; pass < 32 / DIAG; ++pass) {
+                    if (DIAG == 32 || col / DIAG == pass) {
+                        float* const p = diagonals + (col % DIAG) * 36 + half * 4;
+                        const float f = real ? undo : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) atomicAdd(sum - (i >> 2) * 8 - (i & 3), s[i] * undo);
+                        for (int c = 0; c < 4; ++c)
+                            *reinterpret_cast<float4_t*>(p + c * 8) = float4_t{s[c * 4] * f, s[c * 4 + 1] * f, s[c * 4 + 2] * f, s[c * 4 + 3] * f};
+                    }
+                    asm volatile("" ::: "memory");
+                    float total = 0.0f;
+                    const float* const from = diagonals + pass * DIAG + 31 - lane;
+#pragma unroll
+                    for (int r = 0; r < DIAG; ++r) {
+                        const float x = from[r * 37];
+                        total += (uint32_t)(pass * DIAG + r + 31 - lane) < 32u ? x : 0.0f;
+                    }
+                    sums[rel_of_corner + lane] += total;
+                    asm volatile("" ::: "memory");
+                }
             } else {
                 float far = 0.0f;
 #pragma unroll
@@ -450,7 +469,8 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
 template <int NT, bool PLAIN, int LAY>
 static int dq_launch(const AttentionGrad& a, unsigned grid, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
-    const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 * (a.table_parts ? 5 : 1) : 0);
+    const int entries = a.table ? a.distances - a.first_distance + 2 * kBiasPad : 0;
+    const int lds = 4 * kAttnTile * D * 2 + (a.table_parts ? 5 * ((entries + 3) & ~3) + 4 * kDiagonals<NT> : entries) * 4;
     static std::atomic<bool> done[64];
     if (int e = enable_dynamic_lds((const void*)k_attn_dq<NT, PLAIN, LAY>, 156 * 1024, done)) return e;
     hipLaunchKernelGGL((k_attn_dq<NT, PLAIN, LAY>), dim3(grid), dim3(256), lds, st, a);
