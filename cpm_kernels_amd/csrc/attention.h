@@ -18,8 +18,8 @@ struct Attention {
     const int32_t* mapping;
     const uint8_t* mask;
     int64_t mask_batch, mask_token;
-    float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; behind them (batch, held, key tiles): the largest norm
-                                    // of a tile's values, squared; or null
+    float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; behind them (batch, held, parts): the largest magnitude
+                                    // of a part's values that any query sees; or null
     int64_t rows_in_all;
     half_t* rest;                   // with lse: what the rounding of `out` left, times 2^11, under the same strides
     float* parts;
@@ -65,6 +65,7 @@ struct AttnPlan {
     int rows, row_tiles, splits, tile, least, waves;
     bool few;
 };
+AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length, bool rows_of_keys, bool train);
 AttnPlan attn_few_plan(int64_t batch, int64_t held, int64_t of_head, int32_t dim, int64_t length);
 int attn_few_launch(const Attention& a, const AttnPlan& p, int32_t batch, hipStream_t st);
 
@@ -170,16 +171,22 @@ struct AttnShare {
                 for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(u0 + i, dim - 1) * unit + t0 + tb);
             } else {
 #pragma unroll
-                for (int i = 0; i < PIECES; ++i)
+                for (int i = 0; i < PIECES; ++i) {
+                    half_t y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) r[i][e] = base[min(u0 + i, dim - 1) * unit + min(t0 + tb + e, tokens - 1)];
+                    for (int e = 0; e < 8; ++e) y[e] = base[min(u0 + i, dim - 1) * unit + min(t0 + tb + e, tokens - 1)];
+                    r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+                }
             }
         } else {
             const int row = tid / RUN, u = (tid % RUN) * 8;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i)
+            for (int i = 0; i < PIECES; ++i) {
+                half_t y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) r[i][e] = base[min(t0 + row + i * STEP, tokens - 1) * token + min(u + e, dim - 1) * unit];
+                for (int e = 0; e < 8; ++e) y[e] = base[min(t0 + row + i * STEP, tokens - 1) * token + min(u + e, dim - 1) * unit];
+                r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+            }
         }
     }
 
@@ -232,6 +239,22 @@ struct AttnShare {
     typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
 };
 
+// Operands that the waves keep of tensors whose tokens are neighbours in memory, of 128 tokens from t0 on: through two tiles in LDS (`bring`, then, behind a barrier, `keep`).
+template <int D>
+__device__ __forceinline__ void attn_bring_columns(const AttnTensor& t, const half_t* base, int32_t t0, int32_t tokens, int dim, int tid, int8_t* tiles) {
+    AttnShare<D, kColumns, 256> share[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) share[i].load(base, t.token, t.unit, dim, t0 + i * kAttnTile, tokens, tid);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) share[i].store(tiles + i * kAttnTile * D * 2, dim, t0 + i * kAttnTile, tokens, tid, false, nullptr);
+}
+template <int D, int KS>
+__device__ __forceinline__ void attn_keep_columns(half8_t (&x)[KS], const int8_t* tiles, int wave, int lane) {
+    const uint32_t at = attn_rows_at<D>(lane);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) x[s] = attn_rows<D>(tiles + (wave >> 1) * kAttnTile * D * 2, at, wave & 1, s);
+}
+
 // 32 bytes of a row of a mask as bits, on their way from memory
 struct AttnMaskShare {
     uint4_t raw[2];
@@ -270,9 +293,12 @@ __device__ __forceinline__ void attn_keep(half8_t (&x)[KS], const AttnTensor& t,
         for (int s = 0; s < KS; ++s) x[s] = load_half8_any(row + min(s * 16 + half * 8, dim - 8));
     } else {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s) {
+            half_t y[8];            // (element by element into the operand itself leaves it in scratch memory)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[s][e] = row[min(s * 16 + half * 8 + e, dim - 1) * t.unit];
+            for (int e = 0; e < 8; ++e) y[e] = row[min(s * 16 + half * 8 + e, dim - 1) * t.unit];
+            x[s] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+        }
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) x[s] = half8_fill(x[s], half8_keep(dim - s * 16 - half * 8), half8_t{0, 0, 0, 0, 0, 0, 0, 0});
@@ -289,15 +315,19 @@ __device__ __forceinline__ uint32_t attn_mask4(const uint8_t* row, int32_t key, 
 
 constexpr float kRest = 2048.0f;        // fp16 has 11 bits: what a rounding leaves, times this, is as large as the number at most
 
-// A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times f, as fp16; or, REST, what that rounding leaves
+// A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times the lane's f, as fp16 to the tokens first .. first + 31 below `tokens`; or,
+// REST, what that rounding leaves.  Through LDS of the wave's own (80 D bytes), so that 16 bytes a lane go out side by side, units or tokens, whichever are neighbours in memory.
 template <int NT, bool REST = false>
-__device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, const float16_tv (&acc)[NT], float f, int dim, int half) {
+__device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* base, const float16_tv (&acc)[NT], float f, int32_t first, int32_t tokens, int dim, int lane, int8_t* lds) {
+    constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
+    const int col = lane & 31, half = lane >> 5, count = min(32, tokens - first);
+    if (count <= 0) return;
     const auto rounded = [&](float x) {
         x *= f;
         const half_t r = round_f16(x);
         return REST ? (half_t)((x - (float)r) * kRest) : r;
     };
-    if (t.unit == 1 && dim % 4 == 0) {
+    if (t.unit == 1 && dim % 8 == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -305,10 +335,37 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, con
                 half4_t v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = rounded(acc[n][c * 4 + e]);
-                const int u = n * 32 + c * 8 + half * 4;
-                if (u < dim) *reinterpret_cast<Half4Any*>(row + u) = __builtin_bit_cast(Half4Any, v);
+                *reinterpret_cast<half4_t*>(lds + attn_place<D>(col, n * 4 + c) + half * 8) = v;
             }
-    } else {
+        asm volatile("" ::: "memory");
+        const int piece = lane % (D / 8);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int token = i * (512 / D) + lane / (D / 8);
+            const half8_t v = *reinterpret_cast<const half8_t*>(lds + attn_place<D>(token, piece));
+            if (token < count && piece * 8 < dim) store_half8_any(base + (first + token) * t.token + piece * 8, v);
+        }
+    } else if (t.token == 1) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) *reinterpret_cast<half_t*>(lds + (n * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 80 + col * 2) = rounded(acc[n][i]);
+        asm volatile("" ::: "memory");
+        const int at = (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < NT * 2; ++i) {
+            const int unit = i * 16 + (lane >> 2);
+            const half8_t v = *reinterpret_cast<const half8_t*>(lds + unit * 80 + at * 2);
+            half_t* const p = base + unit * t.unit + first + at;
+            if (unit < dim && at < count) {
+                if (at + 8 <= count) store_half8_any(p, v);
+                else
+#pragma unroll 1
+                    for (int e = 0; at + e < count; ++e) p[e] = reinterpret_cast<const half_t*>(lds + unit * 80 + at * 2)[e];
+            }
+        }
+    } else if (col < count) {
+        half_t* const row = base + (first + col) * t.token;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -316,6 +373,26 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* row, con
                 const int u = n * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
                 if (u < dim) row[u * t.unit] = rounded(acc[n][i]);
             }
+    }
+    asm volatile("" ::: "memory");
+}
+
+// The order of a stretch of products whose operands come from LDS, first M1 of R1 reads, then M2 of M2: eight reads ahead, so that their latency lies behind products (the compiler by
+// itself reads an operand right before its product and waits).
+template <int M1, int R1, int M2>
+__device__ __forceinline__ void attn_pace() {
+    constexpr int kAhead = M2 >= 8 || M2 == 0 ? 8 : M2, kEach = M1 ? R1 / M1 : 1;
+    static_assert(M1 == 0 || R1 % M1 == 0, "reads of a product");
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < M1; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (M2 > 0 || i < M1 - kAhead / kEach) __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < M2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (i < M2 - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
 }
 

@@ -19,50 +19,18 @@ constexpr int kAttnRows = 128, kAttnLeast = 4;       // queries of a workgroup; 
 constexpr int kLazy = 8;            // log2 of how far the running maximum may lie below the true one
 constexpr float kLift = 7.0f;       // log2 of the largest probability's size right behind a change of the maximum
 
-// Norms of 64 keys' values, the largest (squared), for the backward pass.
-__device__ __forceinline__ void attn_value_top(const Attention& a, uint32_t id, int tid) {
-    __shared__ float sums[4][64];
-    const uint32_t tiles = (uint32_t)ceil_div(a.length, 64), tile = id % tiles, bh = id / tiles;
-    const int64_t b = bh / (uint32_t)a.held, h = bh % (uint32_t)a.held;
-    const int32_t keys = attn_range(a, b).len;
-    // (four threads a token, in the order in which neighbouring ones read neighbouring addresses)
-    const bool columns = a.v.token == 1;
-    const int mine = columns ? tid & 63 : tid >> 2, share = columns ? tid >> 6 : tid & 3;
-    const int32_t t = tile * 64 + mine;
-    float square = 0.0f;
-    if (t < keys) {
-        const half_t* const p = a.v.at(b, h) + t * a.v.token;
-        if (a.v.unit == 1 && a.dim % 8 == 0) {
-            for (int u = share * 8; u < a.dim; u += 32) {
-                const half8_t x = load_half8_any(p + u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) square = __builtin_fmaf((float)x[e], (float)x[e], square);
-            }
-        } else {
-#pragma unroll 8
-            for (int u = share; u < a.dim; u += 4) square = __builtin_fmaf((float)p[u * a.v.unit], (float)p[u * a.v.unit], square);
-        }
-    }
-    sums[share][mine] = square;
-    __syncthreads();
-    if (tid >= 64) return;
-    square = wave_max((sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]));
-    if (tid == 0) a.lse[a.rows_in_all + id] = square;
-}
-
 template <int NT, bool PLAIN, int LAY, bool TRAIN>
-__global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint32_t blocks) {
+__global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys, two of values, biases
     __shared__ uint32_t bad[3][2];              // tokens of a tile whose values are no finite numbers; those of tile t in t % 3
     __shared__ uint32_t mask_bits[2][kAttnRows][2];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (TRAIN && blockIdx.x >= blocks) return attn_value_top(a, blockIdx.x - blocks, tid);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const uint32_t inner = (uint32_t)a.group * a.row_tiles * a.splits;
     uint32_t unit, w;
-    attn_deal(blockIdx.x, blocks / inner, inner, unit, w);
+    attn_deal(blockIdx.x, gridDim.x / inner, inner, unit, w);
     const int64_t b = unit / (uint32_t)a.held;
     const int32_t kvh = unit - (uint32_t)b * a.held;
     const int32_t split = w % (uint32_t)a.splits;
@@ -72,7 +40,11 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
     const int32_t h = kvh * a.group + w / (uint32_t)a.row_tiles;
     const AttnRange range = attn_range(a, b);
     const AttnParts parts = attn_parts(a, range, min(qt * kAttnRows + kAttnRows - 1, a.tokens - 1), kAttnLeast, kAttnTile);
-    if (split >= parts.parts) return;
+    const bool looks = TRAIN && qt == a.row_tiles - 1 && h == kvh * a.group;         // for the largest magnitude of the values: the workgroup whose queries see most keys of a head
+    if (split >= parts.parts) {
+        if (looks && tid == 0) a.lse[a.rows_in_all + (b * a.held + kvh) * a.splits + split] = 0.0f;
+        return;
+    }
 
     const int32_t q_first = qt * kAttnRows + wave * 32;
     const int32_t query = min(q_first + col, a.tokens - 1);         // (queries past the end repeat the last one)
@@ -101,7 +73,12 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
     };
     load(t_begin - 1);
     half8_t q[KS];
-    attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
+    if (LAY == kColumns && a.q.token == 1) {
+        attn_bring_columns<D>(a.q, a.q.at(b, h), qt * kAttnRows, a.tokens, a.dim, tid, lds + 2 * kTileBytes);
+        __syncthreads();
+        attn_keep_columns<D, KS>(q, lds + 2 * kTileBytes, wave, lane);
+    } else
+        attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
     if (flip)
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s] = -q[s];
@@ -116,6 +93,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = kZero16;
     float top = -__builtin_inff(), sum = 0.0f;
+    ushort8_t largest = {0, 0, 0, 0, 0, 0, 0, 0};
     auto scores_of = [&](int32_t t) {
         const int8_t* const tile = lds + (t & 1) * kTileBytes;
         s[0] = s[1] = kZero16;
@@ -203,6 +181,9 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
             ks.store(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, false, nullptr);
             if (masked) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         }
+        if (TRAIN && looks && t >= t_begin)
+#pragma unroll
+            for (int i = 0; i < decltype(vs)::PIECES; ++i) largest = absbits_max(largest, vs.r[i]);
         if (t >= t_begin) vs.store(lds + (2 + (t & 1)) * kTileBytes, a.dim, k0, range.len, tid, masked || k0 + kAttnTile > every_sees, bad[(uint32_t)t % 3]);
         if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;          // (last looked at two tiles ago)
         load(t + 1);
@@ -219,13 +200,27 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
             }
             sums_of(t);
             scores_of(t + 1);
-        } else if ((t + 1) * kAttnTile < any_sees && t + 1 < t_end)
+            attn_pace<4 * NT * (TRAIN ? 2 : 1), 8 * NT, 2 * KS>();
+        } else if ((t + 1) * kAttnTile < any_sees && t + 1 < t_end) {
             scores_of(t + 1);
+            attn_pace<0, 0, 2 * KS>();
+        }
     }
     sum += __shfl_xor(sum, 32);
-    if (q_first + col >= a.tokens) return;
+    __syncthreads();            // (the tiles are done with)
+    if (looks) {
+        // (numbers that are none or infinite count as the largest one: the keys past the end among them are zeros or copies)
+        const uint32_t m = wave_max_u32(min(absbits_max_of(largest), 0x7bffu));
+        if (lane == 0) bad[0][0] = 0;
+        __syncthreads();
+        if (lane == 0) atomicMax(&bad[0][0], m);
+        __syncthreads();
+        if (tid == 0) a.lse[a.rows_in_all + (b * a.held + kvh) * a.splits + split] = (float)__builtin_bit_cast(half_t, (uint16_t)bad[0][0]);
+    }
+    const bool real = q_first + col < a.tokens;
     const int64_t row = (b * a.heads + h) * a.tokens + query;
     if (a.splits > 1) {
+        if (!real) return;
         struct __attribute__((packed, aligned(4))) Float4Any { float x, y, z, w; };         // (a workspace is aligned to 4 bytes)
         float* const part = a.parts + (((b * a.heads + h) * a.row_tiles + qt) * a.splits + split) * kAttnRows * (a.dim + 2);
         const int r = wave * 32 + col;
@@ -246,10 +241,11 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a, uint
         return;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    attn_write<NT>(a.out, a.out.at(b, h) + query * a.out.token, acc, inv, a.dim, half);
+    int8_t* const own = lds + wave * D * 80;
+    attn_write<NT>(a.out, a.out.at(b, h), acc, inv, q_first, a.tokens, a.dim, lane, own);
     if (!TRAIN) return;
-    attn_write<NT, true>(a.out, a.rest + b * a.out.batch + h * a.out.head + query * a.out.token, acc, inv, a.dim, half);
-    if (half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
+    attn_write<NT, true>(a.out, a.rest + (a.out.at(b, h) - a.out.p), acc, inv, q_first, a.tokens, a.dim, lane, own);
+    if (real && half == 0) a.lse[row] = sum == 0.0f ? __builtin_inff() : top - kLift + __builtin_amdgcn_logf(sum);
 }
 
 // Parts joined under the largest of their maxima: a wave a row, its lanes along the units.  `rows` of them lie together: queries of a head, or (few) rows of a head of keys.
@@ -310,7 +306,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Attention a, AttnPlan plan, u
 }
 
 // Which kernel a call takes, and how it is divided.  Keys are cut into as many parts as let the device's compute units each have a workgroup, of four tiles at least.
-static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length, bool rows_of_keys, bool train) {
+AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length, bool rows_of_keys, bool train) {
     const int64_t of_head = tokens * (heads / held);
     if (rows_of_keys && !train && of_head <= 32 && dim % 8 == 0 && length > 0) {
         AttnPlan p = attn_few_plan(batch, held, of_head, dim, length);
@@ -326,26 +322,26 @@ static AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t to
 }
 
 template <int NT, bool PLAIN, int LAY, bool TRAIN>
-static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
     if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY, TRAIN>, 150 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid + (TRAIN ? more : 0)), dim3(256), lds, st, a, grid);
+    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid), dim3(256), lds, st, a);
     return 0;
 }
 template <int NT, bool PLAIN, int LAY>
-static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
-    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, more, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, more, st);
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, st);
 }
 template <int NT, bool PLAIN>
-static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     const int lay = attn_layout(a.k, a.v, a.dim);
-    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, more, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, more, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, more, st);
+    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
 }
 template <int NT>
-static int attn_launch(const Attention& a, unsigned grid, unsigned more, hipStream_t st) {
-    return a.table || a.mask ? attn_launch<NT, false>(a, grid, more, st) : attn_launch<NT, true>(a, grid, more, st);
+static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
+    return a.table || a.mask ? attn_launch<NT, false>(a, grid, st) : attn_launch<NT, true>(a, grid, st);
 }
 
 }  // namespace cpmk
@@ -388,17 +384,15 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
     a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;
     const int64_t grid = (int64_t)batch * heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;
-    const int64_t key_tiles = lse ? (int64_t)batch * kv_heads * ceil_div(length, kAttnTile) : 0;
-    if (!grid_fits(grid + key_tiles) || !grid_fits(rows)) return CPMK_ETOOBIG;
+    if (!grid_fits(grid) || !grid_fits(rows)) return CPMK_ETOOBIG;
     a.rows_in_all = rows;
-    const unsigned more = (unsigned)key_tiles;
     hipStream_t st = (hipStream_t)stream;
     const unsigned g = (unsigned)grid;
     const int e = plan.few    ? attn_few_launch(a, plan, batch, st)
-                  : dim <= 64 ? attn_launch<2>(a, g, more, st)
-                  : dim <= 96 ? attn_launch<3>(a, g, more, st)
-                  : dim <= 128 ? attn_launch<4>(a, g, more, st)
-                               : attn_launch<8>(a, g, more, st);
+                  : dim <= 64 ? attn_launch<2>(a, g, st)
+                  : dim <= 96 ? attn_launch<3>(a, g, st)
+                  : dim <= 128 ? attn_launch<4>(a, g, st)
+                               : attn_launch<8>(a, g, st);
     if (e) return e;
     if (a.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, plan, (uint32_t)rows);
     return launch_status();

@@ -8,7 +8,7 @@
 //
 // ds and p are rounded to fp16 for the last products.  p is taken times 2^15 (exact, in the exponent).  |dp_ij - D_i| is at most 2 |do_i| max |v_j|: ds is taken times the power of two that
 // brings this bound to 2^15 (a row's own in k_attn_dq, the largest row's in k_attn_dkv), so that it neither overflows beside a loss scale nor vanishes without one.
-// The forward pass has left the values' norms, k_attn_dq, which comes first, leaves D and the gradients'.
+// The forward pass has left the values' largest magnitude, k_attn_dq, which comes first, leaves D and the gradients'.
 #include <algorithm>
 #include "attention.h"
 
@@ -21,7 +21,7 @@ struct AttentionGrad : Attention {
     half_t* dtable;
     float natural_scale;
     int64_t batch;
-    int32_t query_tiles, key_tiles;
+    int32_t query_tiles;
 };
 
 constexpr int kGradRows = 128;      // queries (k_attn_dq) or keys (k_attn_dkv) of a workgroup
@@ -34,6 +34,11 @@ __device__ __forceinline__ float attn_largest(const float* x, int64_t n, int lan
     float m = 0.0f;
     for (int64_t i = lane; i < n; i += 64) m = fmaxf(m, x[i]);
     return wave_max(m);
+}
+// A bound of the norms of a head's values, squared, from their largest magnitude
+__device__ __forceinline__ float attn_value_norm(const AttentionGrad& a, int64_t b, int64_t kvh, int lane) {
+    const float m = attn_largest(a.lse + a.rows_in_all + (b * a.held + kvh) * a.splits, a.splits, lane);
+    return m * m * (float)a.dim;
 }
 // log2 of the factor that brings 2 sqrt(squares) to at most 1: with a probability of at most 2^15, ds to at most 2^15
 __device__ __forceinline__ int attn_exponent(float dout_square, float value_square) {
@@ -105,38 +110,60 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     float minus_delta, minus_lse, dscale, undo;
     {
         // D from the result and what its rounding left; the factor of ds from the norms
-        const half_t* const at_out = a.out.at(b, h) + query * a.out.token;
-        AttnTensor of_rest = a.out;
-        attn_keep<KS>(g, a.dout, a.dout.at(b, h) + query * a.dout.token, a.dim, half);
-        attn_keep<KS>(q, of_rest, at_out, a.dim, half);
-        float square = 0.0f, delta = 0.0f;
+        float square = 0.0f, delta = 0.0f, little = 0.0f;
+        auto first = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                square = __builtin_fmaf((float)g[s][e], (float)g[s][e], square);
-                delta = __builtin_fmaf((float)g[s][e], (float)q[s][e], delta);
-            }
-        attn_keep<KS>(q, of_rest, a.rest + (at_out - a.out.p), a.dim, half);
-        float little = 0.0f;
+                for (int e = 0; e < 8; ++e) {
+                    square = __builtin_fmaf((float)g[s][e], (float)g[s][e], square);
+                    delta = __builtin_fmaf((float)g[s][e], (float)q[s][e], delta);
+                }
+        };
+        auto second = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) little = __builtin_fmaf((float)g[s][e], (float)q[s][e], little);
+                for (int e = 0; e < 8; ++e) little = __builtin_fmaf((float)g[s][e], (float)q[s][e], little);
+        };
+        const half_t *const of_out = a.out.at(b, h), *const of_rest = a.rest + (of_out - a.out.p);
+        if (LAY == kColumns && a.q.token == 1 && a.out.token == 1 && a.dout.token == 1) {
+            const auto bring = [&](const AttnTensor& x, const half_t* base, int at) __attribute__((always_inline)) {
+                attn_bring_columns<D>(x, base, qt * kGradRows, a.tokens, a.dim, tid, lds + at * kTileBytes);
+            };
+            bring(a.dout, a.dout.at(b, h), 0);
+            bring(a.out, of_out, 2);
+            __syncthreads();
+            attn_keep_columns<D, KS>(g, lds, wave, lane);
+            attn_keep_columns<D, KS>(q, lds + 2 * kTileBytes, wave, lane);
+            first();
+            __syncthreads();
+            bring(a.out, of_rest, 0);
+            bring(a.q, a.q.at(b, h), 2);
+            __syncthreads();
+            attn_keep_columns<D, KS>(q, lds, wave, lane);
+            second();
+            attn_keep_columns<D, KS>(q, lds + 2 * kTileBytes, wave, lane);
+        } else {
+            attn_keep<KS>(g, a.dout, a.dout.at(b, h) + query * a.dout.token, a.dim, half);
+            attn_keep<KS>(q, a.out, of_out + query * a.out.token, a.dim, half);
+            first();
+            attn_keep<KS>(q, a.out, of_rest + query * a.out.token, a.dim, half);
+            second();
+            attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
+        }
         delta = __builtin_fmaf(little, 1.0f / kRest, delta);
         square += __shfl_xor(square, 32);
         delta += __shfl_xor(delta, 32);
         if (real && half == 0) a.delta[row] = delta;
         const float largest = wave_max(real ? square : 0.0f);
         if (lane == 0) tops[wave] = largest;
-        const float value_top = attn_largest(a.lse + a.rows_in_all + (b * a.held + kvh) * a.key_tiles, a.key_tiles, lane);
-        const int exponent = attn_exponent(square, value_top);
+        const int exponent = attn_exponent(square, attn_value_norm(a, b, kvh, lane));
         dscale = ldexpf(1.0f, exponent);
         undo = ldexpf(1.0f, -exponent - (int)kProbScale);
         const float lse = real ? a.lse[row] : __builtin_inff();
         minus_lse = kProbScale - lse;
         minus_delta = lse == __builtin_inff() ? 0.0f : -delta * dscale;
-        attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
     }
     __syncthreads();
     if (tid == 0) a.dout_top[(b * a.heads + h) * a.row_tiles + qt] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -233,22 +260,30 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
 #pragma unroll
         for (int i = 0; i < 16; ++i) d[i >> 3][i & 7] = (half_t)s[i];
     };
-    if (0 < any_sees) scores_of(0, 0);
+    if (0 < any_sees) {
+        scores_of(0, 0);
+        attn_pace<0, 0, 2 * KS>();
+    }
     for (int32_t t = 0; t < tiles; ++t) {
         const bool one = t * kAttnTile < any_sees;          // (the second block of the tile: scores that nobody sees, or zeros)
         if (one) {
             gradients_of(t, 0);
             sums_of(t, 0);
             scores_of(t, 1);
+            attn_pace<2 * NT, 4 * NT, 2 * KS>();
             gradients_of(t, 1);
             sums_of(t, 1);
+            attn_pace<2 * NT, 4 * NT, 0>();
         }
         store(t + 1);
         load(t + 2);
         __syncthreads();
-        if ((t + 1) * kAttnTile < any_sees) scores_of(t + 1, 0);
+        if ((t + 1) * kAttnTile < any_sees) {
+            scores_of(t + 1, 0);
+            attn_pace<0, 0, 2 * KS>();
+        }
     }
-    if (real) attn_write<NT>(a.dq, a.dq.at(b, h) + query * a.dq.token, acc, undo * a.natural_scale, a.dim, half);
+    attn_write<NT>(a.dq, a.dq.at(b, h), acc, undo * a.natural_scale, q_first, a.tokens, a.dim, lane, lds + wave * D * 80);
     if (!table_wanted) return;
     far_before = wave_sum(real ? far_before * undo : 0.0f);
     far_behind = wave_sum(real ? far_behind * undo : 0.0f);
@@ -313,14 +348,19 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     const int32_t of_head = k_first_of_all < range.len && first_query < a.tokens ? a.query_tiles - first_tile : 0;
 
     half8_t k[KS], v[KS];
-    {
+    if (LAY == kColumns && a.k.token == 1 && a.v.token == 1) {
+        attn_bring_columns<D>(a.k, a.k.at(b, kvh), k_first_of_all, a.length, a.dim, tid, lds);
+        attn_bring_columns<D>(a.v, a.v.at(b, kvh), k_first_of_all, a.length, a.dim, tid, lds + 2 * kTileBytes);
+        __syncthreads();
+        attn_keep_columns<D, KS>(k, lds, wave, lane);
+        attn_keep_columns<D, KS>(v, lds + 2 * kTileBytes, wave, lane);
+    } else {
         const int32_t mine = min(key, a.length - 1);
         attn_keep<KS>(k, a.k, a.k.at(b, kvh) + mine * a.k.token, a.dim, half);
         attn_keep<KS>(v, a.v, a.v.at(b, kvh) + mine * a.v.token, a.dim, half);
     }
-    const float value_top = attn_largest(a.lse + a.rows_in_all + (b * a.held + kvh) * a.key_tiles, a.key_tiles, lane);
     const float dout_top = attn_largest(a.dout_top + (b * a.heads + kvh * a.group) * a.row_tiles, (int64_t)a.group * a.row_tiles, lane);
-    const int exponent = attn_exponent(dout_top, value_top);
+    const int exponent = attn_exponent(dout_top, attn_value_norm(a, b, kvh, lane));
     const float dscale = ldexpf(1.0f, exponent);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int32_t lo_rel = a.first_distance - kBiasPad;
@@ -448,11 +488,14 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
             const int8_t* const tile = lds + buffer * 2 * kTileBytes;
             if (k_first < range.len && (!a.causal || range.pos + q0 + kAttnTile - 1 >= k_first)) {
                 scores_of(tile, 0);
+                attn_pace<0, 0, 2 * KS>();
                 gradients_of(buffer, turn, q0, 0);
                 sums_of(tile, 0);
                 scores_of(tile, 1);
+                attn_pace<4 * NT, 8 * NT, 2 * KS>();
                 gradients_of(buffer, turn, q0, 1);
                 sums_of(tile, 1);
+                attn_pace<4 * NT, 8 * NT, 0>();
             }
             if (t + 1 < of_head || g + 1 < a.group) store(buffer ^ 1);
             load();
@@ -461,9 +504,9 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
             __syncthreads();
         }
     }
-    if (key >= a.length) return;
-    attn_write<NT>(a.dk, a.dk.at(b, kvh) + key * a.dk.token, dk, ldexpf(a.natural_scale, -exponent - (int)kProbScale), a.dim, half);
-    attn_write<NT>(a.dv, a.dv.at(b, kvh) + key * a.dv.token, dv, ldexpf(1.0f, -(int)kProbScale), a.dim, half);
+    int8_t* const own = lds + wave * D * 80;
+    attn_write<NT>(a.dk, a.dk.at(b, kvh), dk, ldexpf(a.natural_scale, -exponent - (int)kProbScale), k_first, a.length, a.dim, lane, own);
+    attn_write<NT>(a.dv, a.dv.at(b, kvh), dv, ldexpf(1.0f, -(int)kProbScale), k_first, a.length, a.dim, lane, own);
 }
 
 template <int NT, bool PLAIN, int LAY>
@@ -542,12 +585,13 @@ int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int3
     a.table = (const half_t*)bias, a.mapping = (const int32_t*)mapping, a.buckets = num_buckets, a.distances = max_distance, a.dtable = (half_t*)dbias;
     a.mask = (const uint8_t*)mask, a.mask_batch = mask_batch, a.mask_token = mask_token;
     a.lse = (float*)lse, a.rest = (half_t*)rest, a.scale = scale * kLog2e, a.natural_scale = scale, a.causal = causal != 0;
-    a.tokens = tokens, a.dim = dim, a.length = length, a.splits = 1, a.parts = nullptr;
+    a.tokens = tokens, a.dim = dim, a.length = length, a.parts = nullptr;
     bool empty;
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty) return 0;
     if ((tokens > 0 && any_null(lse, rest, dout, dq)) || (length > 0 && any_null(dk, dv)) || !workspace || (dbias && !bias)) return CPMK_EBADARG;
-    a.row_tiles = (int32_t)ceil_div(tokens, kGradRows), a.query_tiles = (int32_t)ceil_div(tokens, kAttnTile), a.key_tiles = (int32_t)ceil_div(length, kAttnTile);
+    a.row_tiles = (int32_t)ceil_div(tokens, kGradRows), a.query_tiles = (int32_t)ceil_div(tokens, kAttnTile);
+    a.splits = tokens > 0 ? attn_plan(batch, heads, kv_heads, tokens, dim, length, false, true).splits : 0;        // (the forward pass's: where it has left the values' magnitudes)
     const int64_t dkv_blocks = (int64_t)batch * kv_heads * ceil_div(length, kGradRows);
     if (!grid_fits((int64_t)batch * heads * a.row_tiles) || !grid_fits(dkv_blocks + heads)) return CPMK_ETOOBIG;
     int64_t at[3];

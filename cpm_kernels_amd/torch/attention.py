@@ -13,7 +13,6 @@ from functools import lru_cache
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 from ..library import cpmk          # (the launchers themselves: what the kernels layer checks is checked here)
 from ._common import cur_stream, current_device
 from .kv_cache import _each
@@ -31,8 +30,8 @@ def _forward(q, k, v, table, seen, rows, sizes, keep):
     """(result, what the backward pass needs besides it)"""
     out = torch.empty_like(q)
     batch, heads, kv_heads, tokens, _, length = sizes
-    # (a number for each row, and one for each tile of 64 keys)
-    lse, rest = (torch.empty(batch * (heads * tokens + kv_heads * ((length + 63) // 64)), dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
+    # (a number for each row, and one for each part of the keys, which are 256 at least)
+    lse, rest = (torch.empty(batch * (heads * tokens + kv_heads * (length // 256 + 1)), dtype=torch.float32, device=q.device), torch.empty_like(out)) if keep else (None, None)
     size = _workspace(q.device.index, *sizes)
     space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     cpmk.attention_forward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
@@ -52,8 +51,8 @@ class OpAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        assert not torch.is_grad_enabled(), "the gradients have no gradients"       # (create_graph; a wrapper that refuses it costs 10 us)
         q, k, v, bias, mapping, _, out, lse, rest, _, _ = ctx.saved_tensors
         sizes, rows, table, seen = ctx.plain
         batch, heads, kv_heads, tokens, dim, length = sizes

@@ -526,8 +526,9 @@ int64_t cpmk_kv_attention_int8_workspace(int32_t batch, int32_t heads, int32_t k
  * mask_token of 0 for one row a sequence).  A query that no key is left for gives zeros.  What lies in keys and values that a query does not see, numbers or
  * not, does not reach its result.  bias: the table of cpmk_position_embedding_forward, buckets as there (mapping of cpmk_position_embedding_init; a bucket
  * number outside of the table counts as the nearest in it), at most 1024 distances (both signs counted if bidirectional); NULL for none.
- * lse: (batch, heads, tokens) fp32, log2 of the sum of exp2(log2(e) * score), +inf of a query without keys, or NULL; with it rest: fp16 under out's strides, what the
- * rounding of out left, times 2^11.  Both are for cpmk_attention_backward.
+ * lse: fp32, batch * heads * tokens numbers, log2 of the sum of exp2(log2(e) * score), +inf of a query without keys, and behind them room for batch * kv_heads *
+ * (length / 256 + 1) others (largest magnitudes of v); or NULL.  With it rest: fp16 under out's strides, what the rounding of out left, times 2^11.  Both are for
+ * cpmk_attention_backward.
  * workspace: cpmk_attention_forward_workspace() bytes on the device, 4-byte aligned, the call's own until it has finished; NULL if that is 0. */
 int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens, int32_t dim, int32_t length,
                            const void* q /* fp16 */, int64_t q_batch, int64_t q_head, int64_t q_token, int64_t q_unit,
