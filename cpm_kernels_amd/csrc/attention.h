@@ -35,7 +35,7 @@ constexpr int kAttnTile = 64;       // tokens a workgroup stages at a time
 constexpr int32_t kAttnFar = 1 << 30, kAttnLong = 1 << 29;       // positions stay below the one, numbers of tokens and keys up to the other: distances fit 32 bits
 constexpr int kBiasPad = 96;        // distances beyond the table's ends that a tile of 64 tokens and the 32 of a wave can reach into
 
-enum { kRows = 0, kColumns = 1, kAnyLayout = 2 };
+enum { kDirect = 0, kColumns = 1, kAnyLayout = 2, kRows = 3 };           // (kRows: rotary.hip)
 
 struct AttnRange {
     int32_t len, pos;
@@ -144,8 +144,8 @@ __device__ __forceinline__ half8_t attn_units(const int8_t* tile, uint32_t at, i
     return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// A thread's share of a tile on its way from memory to LDS.  kRows: pieces of eight units as they lie.  kColumns: eight tokens of PIECES neighbouring units, turned in registers.
-// kAnyLayout: unit by unit.  Tokens past the last one and units past the head's are zeros.
+// A thread's share of a tile on its way from memory to LDS through registers.  kColumns: eight tokens of PIECES neighbouring units, turned there.  Else pieces of eight units, unit by unit
+// where they are not neighbours.  Tokens past the last one and units past the head's are zeros.
 template <int D, int LAY, int THREADS>
 struct AttnShare {
     static constexpr int PIECES = 64 * D / 8 / THREADS, RUN = D / 8, STEP = THREADS / RUN;      // (rows: a pass of the workgroup brings STEP tokens)
@@ -154,17 +154,7 @@ struct AttnShare {
 
     __device__ __forceinline__ void load(const half_t* base, int64_t token, int64_t unit, int dim, int32_t t0, int32_t tokens, int tid) {
         const bool whole = t0 + kAttnTile <= tokens;
-        if constexpr (LAY == kRows) {
-            const int row = tid / RUN, u = min((tid % RUN) * 8, dim - 8);
-            if (whole) {
-                const half_t* p = base + (t0 + row) * token + u;
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(p + i * STEP * token);
-            } else {
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(t0 + row + i * STEP, tokens - 1) * token + u);
-            }
-        } else if constexpr (LAY == kColumns) {
+        if constexpr (LAY == kColumns) {
             const int tb = (tid & 7) * 8, u0 = (tid >> 3) * PIECES;
             if (whole) {
 #pragma unroll
@@ -178,6 +168,10 @@ struct AttnShare {
                     r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
                 }
             }
+        } else if (unit == 1 && dim % 8 == 0) {
+            const int row = tid / RUN, u = min((tid % RUN) * 8, dim - 8);
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(t0 + row + i * STEP, tokens - 1) * token + u);
         } else {
             const int row = tid / RUN, u = (tid % RUN) * 8;
 #pragma unroll
@@ -236,7 +230,101 @@ struct AttnShare {
             }
         }
     }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m) const {        // of the magnitudes, as bits
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, r[i]);
+        return m;
+    }
     typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
+};
+
+// The same without registers, 16 bytes a lane straight into LDS: tensors whose units are neighbours, every token on a 16-byte boundary.  A wave brings sixteen tokens, 1 KB an
+// instruction; which piece a lane fetches makes up for LDS being written in the order of the lanes.  Tokens past the last one are copies of it, places of units past the head's are left
+// alone (attn_clear has made them zeros).
+template <int D>
+struct AttnDirect {
+    static constexpr int PIECES = D / 32, EACH = 512 / D;       // instructions a wave and tile, tokens of one
+    uint32_t off[PIECES];
+
+    __device__ __forceinline__ void init(int64_t token, int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) off[i] = (uint32_t)((wave * 16 + i * EACH + lane / (D / 8)) * (int32_t)token + piece(i, wave, lane) * 8) * 2;
+    }
+    static __device__ __forceinline__ int piece(int i, int wave, int lane) {
+        constexpr int W = D == 64 ? 8 : 16;
+        const int place = lane % (D / 8);
+        return (place & ~(W - 1)) | ((place ^ attn_swizzle<D>(wave * 16 + i * EACH + lane / (D / 8))) & (W - 1));
+    }
+    __device__ __forceinline__ void issue(const half_t* tile, int64_t token, int32_t count, int8_t* lds, int dim, int wave, int lane) const {
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds + wave * 16 * D * 2;
+        if (dim == D && count >= kAttnTile) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) lds_dma16(off[i], reinterpret_cast<const int8_t*>(tile), to + i * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int over = max(0, wave * 16 + i * EACH + lane / (D / 8) - (count - 1));
+                if (piece(i, wave, lane) * 8 < dim) lds_dma16(off[i] - (uint32_t)(over * (int32_t)token) * 2, reinterpret_cast<const int8_t*>(tile), to + i * 1024);
+            }
+        }
+    }
+    // Numbers that are none or infinite among what the wave has brought become zeros, their tokens' bits are set
+    static __device__ __forceinline__ void guard(int8_t* lds, int wave, int lane, uint32_t* bad) {
+        half_t* const p = reinterpret_cast<half_t*>(lds + wave * 16 * D * 2 + lane * 16);
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+        half8_t worst = none;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) worst = __builtin_elementwise_fma(*reinterpret_cast<const half8_t*>(p + i * 512), none, worst);
+        const uint4_t w = __builtin_bit_cast(uint4_t, worst);
+        if ((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu) {
+#pragma unroll 1
+            for (int i = 0; i < PIECES * 8; ++i) {
+                half_t* const x = p + (i >> 3) * 512 + (i & 7);
+                const int t = wave * 16 + (i >> 3) * EACH + lane / (D / 8);
+                if (!(*x * (half_t)0 == (half_t)0)) {
+                    *x = (half_t)0;
+                    atomicOr(bad + (t >> 5), 1u << (t & 31));
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, *reinterpret_cast<const half8_t*>(lds + wave * 16 * D * 2 + i * 1024 + lane * 16));
+        return m;
+    }
+};
+// Zeros in tiles' buffers, where a head has fewer units than they have room for
+__device__ __forceinline__ void attn_clear(int8_t* lds, int bytes, int tid, int threads) {
+    for (int i = tid; i < bytes / 16; i += threads) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
+}
+
+// A tensor's tiles, one after another: `fetch` asks for one, `place`, when it has arrived, puts it into LDS (kDirect: it is there, behind wait_vmcnt); bad: to be guarded (AttnShare::store),
+// or null.  kDirect writes the buffer from `fetch` on.
+template <int D, int LAY>
+struct AttnTiles {
+    const half_t* base;
+    int64_t token, unit;
+    AttnShare<D, LAY, 256> share;
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int) { base = b, token = t.token, unit = t.unit; }
+    __device__ __forceinline__ void fetch(int8_t*, int dim, int32_t t0, int32_t tokens, int tid, int, int) { share.load(base, token, unit, dim, t0, tokens, tid); }
+    __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t t0, int32_t tokens, int tid, int, int, uint32_t* bad) { share.store(lds, dim, t0, tokens, tid, bad != nullptr, bad); }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int, int) const { return share.largest(m); }
+};
+template <int D>
+struct AttnTiles<D, kDirect> {
+    const half_t* base;
+    int64_t token;
+    AttnDirect<D> direct;
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int wave, int lane) {
+        base = b, token = t.token;
+        direct.init(token, wave, lane);
+    }
+    __device__ __forceinline__ void fetch(int8_t* lds, int dim, int32_t t0, int32_t tokens, int, int wave, int lane) { direct.issue(base + t0 * token, token, tokens - t0, lds, dim, wave, lane); }
+    __device__ __forceinline__ void place(int8_t* lds, int, int32_t, int32_t, int, int wave, int lane, uint32_t* bad) {
+        if (bad != nullptr) AttnDirect<D>::guard(lds, wave, lane, bad);
+    }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int wave, int lane) const { return AttnDirect<D>::largest(m, lds, wave, lane); }
 };
 
 // Operands that the waves keep of tensors whose tokens are neighbours in memory, of 128 tokens from t0 on: through two tiles in LDS (`bring`, then, behind a barrier, `keep`).
@@ -399,8 +487,11 @@ __device__ __forceinline__ void attn_pace() {
 constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
 // The layout by which tiles of two tensors are brought
+inline bool attn_direct(const AttnTensor& x, int32_t dim) {
+    return x.unit == 1 && dim % 8 == 0 && aligned16(x.p) && x.batch % 8 == 0 && x.head % 8 == 0 && x.token % 8 == 0 && x.token >= 0 && x.token < (1 << 23);        // (64 tokens: offsets of 32 bits)
+}
 inline int attn_layout(const AttnTensor& x, const AttnTensor& y, int32_t dim) {
-    if (x.unit == 1 && y.unit == 1 && dim % 8 == 0) return kRows;
+    if (attn_direct(x, dim) && attn_direct(y, dim)) return kDirect;
     return x.token == 1 && y.token == 1 ? kColumns : kAnyLayout;
 }
 

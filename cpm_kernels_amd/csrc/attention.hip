@@ -62,16 +62,25 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
 
     // Keys, and the mask's bits, come a tile before the values: scores of the next tile are formed beside this one's sums.
     const int32_t t_begin = split * parts.per_part, t_end = min(t_begin + parts.per_part, parts.tiles);
-    AttnShare<D, LAY, 256> ks, vs;
+    AttnTiles<D, LAY> ks, vs;
+    ks.init(keys, a.k, wave, lane);
+    vs.init(values, a.v, wave, lane);
     AttnMaskShare ms;
-    auto load = [&](int32_t t) {
+    ushort8_t largest = {0, 0, 0, 0, 0, 0, 0, 0};
+    const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a value that is no finite number must not reach the queries that do not see it)
+    auto fetch = [&](int32_t t) __attribute__((always_inline)) {
         if (t + 1 < t_end) {
-            ks.load(keys, a.k.token, a.k.unit, a.dim, (t + 1) * kAttnTile, range.len, tid);
+            ks.fetch(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane);
             if (masked) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         }
-        if (t >= t_begin && t < t_end) vs.load(values, a.v.token, a.v.unit, a.dim, t * kAttnTile, range.len, tid);
+        if (t >= t_begin && t < t_end) vs.fetch(lds + (2 + (t & 1)) * kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
     };
-    load(t_begin - 1);
+    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
+    if (LAY == kDirect && a.dim < D) {
+        attn_clear(lds, 4 * kTileBytes, tid, 256);
+        __syncthreads();
+    }
+    if (LAY != kDirect) fetch(t_begin - 1);
     half8_t q[KS];
     if (LAY == kColumns && a.q.token == 1) {
         attn_bring_columns<D>(a.q, a.q.at(b, h), qt * kAttnRows, a.tokens, a.dim, tid, lds + 2 * kTileBytes);
@@ -84,8 +93,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
         for (int s = 0; s < KS; ++s) q[s] = -q[s];
     if (biased) attn_biases(a, h, biases, tid, 256);
     const int32_t lo_rel = a.first_distance - kBiasPad;
-    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
     __syncthreads();
+    if (LAY == kDirect) fetch(t_begin - 1);
 
     const uint32_t at_rows = attn_rows_at<D>(lane), at_units = attn_units_at<D>(lane);
     float16_tv acc[NT], s[2];
@@ -93,7 +102,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = kZero16;
     float top = -__builtin_inff(), sum = 0.0f;
-    ushort8_t largest = {0, 0, 0, 0, 0, 0, 0, 0};
     auto scores_of = [&](int32_t t) {
         const int8_t* const tile = lds + (t & 1) * kTileBytes;
         s[0] = s[1] = kZero16;
@@ -177,17 +185,20 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
                 sum += part;
             }
         }
+        if (LAY == kDirect) wait_vmcnt<0>();
         if (t + 1 < t_end) {
-            ks.store(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, false, nullptr);
+            ks.place(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane, nullptr);
             if (masked) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         }
-        if (TRAIN && looks && t >= t_begin)
-#pragma unroll
-            for (int i = 0; i < decltype(vs)::PIECES; ++i) largest = absbits_max(largest, vs.r[i]);
-        if (t >= t_begin) vs.store(lds + (2 + (t & 1)) * kTileBytes, a.dim, k0, range.len, tid, masked || k0 + kAttnTile > every_sees, bad[(uint32_t)t % 3]);
+        if (t >= t_begin) {
+            int8_t* const tile = lds + (2 + (t & 1)) * kTileBytes;
+            if (looks) largest = vs.largest(largest, tile, wave, lane);
+            vs.place(tile, a.dim, k0, range.len, tid, wave, lane, guarded(t) ? bad[(uint32_t)t % 3] : nullptr);
+        }
         if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;          // (last looked at two tiles ago)
-        load(t + 1);
+        if (LAY != kDirect) fetch(t + 1);
         __syncthreads();
+        if (LAY == kDirect) fetch(t + 1);
         if (active) {           // (behind the last tile: scores that nobody looks at)
             const uint32_t spoilt[2] = {bad[(uint32_t)t % 3][0], bad[(uint32_t)t % 3][1]};
             if (spoilt[0] | spoilt[1]) {        // a query that sees such a key has no number for a result
@@ -337,7 +348,7 @@ static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
 template <int NT, bool PLAIN>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     const int lay = attn_layout(a.k, a.v, a.dim);
-    return lay == kRows ? attn_launch<NT, PLAIN, kRows>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
+    return lay == kDirect ? attn_launch<NT, PLAIN, kDirect>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
 }
 template <int NT>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {

@@ -78,23 +78,31 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
     const int64_t row = (b * a.heads + h) * a.tokens + query;
 
-    AttnShare<D, LAY, 256> ks, vs;
+    AttnTiles<D, LAY> ks, vs;
+    ks.init(keys, a.k, wave, lane);
+    vs.init(values, a.v, wave, lane);
     AttnMaskShare ms;
-    auto load = [&](int32_t t) {
-        if (t >= tiles) return;
-        ks.load(keys, a.k.token, a.k.unit, a.dim, t * kAttnTile, range.len, tid);
-        vs.load(values, a.v.token, a.v.unit, a.dim, t * kAttnTile, range.len, tid);
-        if (masked) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
-    };
-    auto store = [&](int32_t t) {
+    const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a key that is no finite number must not reach the queries that do not see it)
+    auto fetch = [&](int32_t t) __attribute__((always_inline)) {
         if (t >= tiles) return;
         int8_t* const buffer = lds + (t & 1) * 2 * kTileBytes;
-        ks.store(buffer, a.dim, t * kAttnTile, range.len, tid, masked || t * kAttnTile + kAttnTile > every_sees, bad[(uint32_t)t % 3]);
-        vs.store(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, false, nullptr);
+        ks.fetch(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane);
+        vs.fetch(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
+        if (masked) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
+    };
+    auto place = [&](int32_t t) __attribute__((always_inline)) {
+        if (t >= tiles) return;
+        int8_t* const buffer = lds + (t & 1) * 2 * kTileBytes;
+        if (LAY == kDirect) wait_vmcnt<0>();
+        ks.place(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane, guarded(t) ? bad[(uint32_t)t % 3] : nullptr);
+        vs.place(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane, nullptr);
         if (masked) mask_bits[t & 1][tid >> 1][tid & 1] = ms.bits(mask, t * kAttnTile + (tid & 1) * 32, a.length);
         if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;
     };
-    load(0);
+    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
+    if (LAY == kDirect && a.dim < D) attn_clear(lds, 4 * kTileBytes, tid, 256);
+    if (LAY == kDirect) __syncthreads();
+    fetch(0);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int entries = biased ? attn_bias_entries(a) : 0;
     float* const sums = biases + entries + wave * entries;
@@ -104,7 +112,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     const int32_t lo_rel = a.first_distance - kBiasPad;
     constexpr int DIAG = NT <= 4 ? 32 : 4;          // rows of a block that are summed along their diagonals at a time (256 units leave no more LDS)
     float* const diagonals = biases + 5 * ((entries + 3) & ~3) + wave * kDiagonals<NT>;
-    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
 
     half8_t q[KS], g[KS];
     float minus_delta, minus_lse, dscale, undo;
@@ -167,9 +174,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     }
     __syncthreads();
     if (tid == 0) a.dout_top[(b * a.heads + h) * a.row_tiles + qt] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    store(0);
-    load(1);
+    place(0);
+    if (LAY != kDirect) fetch(1);
     __syncthreads();
+    if (LAY == kDirect) fetch(1);
 
     const uint32_t at_rows = attn_rows_at<D>(lane), at_units = attn_units_at<D>(lane);
     float16_tv acc[NT], s, dp;
@@ -275,9 +283,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
             sums_of(t, 1);
             attn_pace<2 * NT, 4 * NT, 0>();
         }
-        store(t + 1);
-        load(t + 2);
+        place(t + 1);
+        if (LAY != kDirect) fetch(t + 2);
         __syncthreads();
+        if (LAY == kDirect) fetch(t + 2);
         if ((t + 1) * kAttnTile < any_sees) {
             scores_of(t + 1, 0);
             attn_pace<0, 0, 2 * KS>();
@@ -365,40 +374,50 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int32_t lo_rel = a.first_distance - kBiasPad;
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
+    if (LAY == kDirect && a.dim < D) attn_clear(lds, 4 * kTileBytes, tid, 256);
+    if (LAY == kDirect) __syncthreads();
 
-    AttnShare<D, LAY, 256> qs, gs;
+    AttnTiles<D, LAY> qs, gs;
+    qs.init(a.q.at(b, kvh * a.group), a.q, wave, lane);
+    gs.init(a.dout.at(b, kvh * a.group), a.dout, wave, lane);
     AttnMaskShare ms;
     float fact = 0.0f;
-    int32_t h_load = kvh * a.group, t_load = 0, t_store = 0;         // head and tile of the head to be loaded next, the tile to be stored next
-    int32_t left = of_head * a.group;           // tiles still to be loaded
-    uint32_t phase = 0;         // of `bad`
-    auto load = [&]() __attribute__((always_inline)) {
+    int32_t h_fetch = kvh * a.group, t_fetch = 0, t_place = 0;       // head and tile of the head to be fetched next, the tile to be placed next
+    int32_t left = of_head * a.group;           // tiles still to be fetched
+    uint32_t phase_place = 0;          // of `bad`
+    const auto guarded = [&](int32_t q0) { return masked || q0 + kAttnTile > a.tokens || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1); };
+    auto fetch = [&](int buffer) __attribute__((always_inline)) {
         if (left == 0) return;
-        const int32_t q0 = (first_tile + t_load) * kAttnTile;
-        qs.load(a.q.at(b, h_load), a.q.token, a.q.unit, a.dim, q0, a.tokens, tid);
-        gs.load(a.dout.at(b, h_load), a.dout.token, a.dout.unit, a.dim, q0, a.tokens, tid);
+        const int32_t q0 = (first_tile + t_fetch) * kAttnTile;
+        int8_t* const at = lds + buffer * 2 * kTileBytes;
+        qs.fetch(at, a.dim, q0, a.tokens, tid, wave, lane);
+        gs.fetch(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane);
         if (masked) ms.load(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
         if (tid < 128) {
             const int32_t query = q0 + (tid & 63);
-            const int64_t row = (b * a.heads + h_load) * a.tokens + min(query, a.tokens - 1);
+            const int64_t row = (b * a.heads + h_fetch) * a.tokens + min(query, a.tokens - 1);
             const float lse = query < a.tokens ? a.lse[row] : __builtin_inff();
             fact = tid < 64 ? kProbScale - lse : lse == __builtin_inff() ? 0.0f : -a.delta[row] * dscale;
         }
-        if (++t_load == of_head) t_load = 0, ++h_load;
+        if (++t_fetch == of_head) {
+            t_fetch = 0, ++h_fetch;
+            qs.base += a.q.head;
+            gs.base += a.dout.head;
+        }
         --left;
     };
-    auto store = [&](int buffer) __attribute__((always_inline)) {
-        const int32_t q0 = (first_tile + t_store) * kAttnTile;
-        const bool guard = masked || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1);
-        uint32_t* const spoilt = bad[phase];
+    auto place = [&](int buffer) __attribute__((always_inline)) {
+        const int32_t q0 = (first_tile + t_place) * kAttnTile;
+        uint32_t* const spoilt = guarded(q0) ? bad[phase_place] : nullptr;
         int8_t* const at = lds + buffer * 2 * kTileBytes;
-        qs.store(at, a.dim, q0, a.tokens, tid, guard, spoilt);
-        gs.store(at + kTileBytes, a.dim, q0, a.tokens, tid, guard, spoilt);
+        if (LAY == kDirect) wait_vmcnt<0>();
+        qs.place(at, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
+        gs.place(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
         if (masked) mask_bits[buffer][tid & 3][tid >> 2] = ms.bits(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
         if (tid < 128) facts[buffer][tid >> 6][tid & 63] = fact;
-        if (++t_store == of_head) t_store = 0;
-        phase = phase == 2 ? 0 : phase + 1;
-        if (tid < 2) bad[phase][tid] = 0;
+        if (++t_place == of_head) t_place = 0;
+        phase_place = phase_place == 2 ? 0 : phase_place + 1;
+        if (tid < 2) bad[phase_place][tid] = 0;
     };
     const uint32_t at_rows = attn_rows_at<D>(lane), at_units = attn_units_at<D>(lane);
     float16_tv dk[NT], dv[NT], s, dp;
@@ -442,8 +461,9 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
             for (int i = 0; i < 16; ++i) s[i] += bp[(i >> 2) * 8 + (i & 3)];
         }
         const uint32_t spoilt = bad[turn][blk];
-        if (masked || spoilt || k_first + 32 > range.len || (a.causal && rel_min < 0)) {
-            // query j of the block is seen from j >= least on
+        if (masked || spoilt || k_first + 32 > range.len || q0 + 32 > a.tokens || (a.causal && rel_min < 0)) {
+            // of the block's queries (from the lane's first on) those from `least` on see the key, up to the last one
+            const int32_t end = a.tokens - q0 - half * 4;
             const int32_t least = key >= range.len ? 64 : a.causal ? -rel : -64;
             const uint32_t none = spoilt >> (half * 4);        // (a key that such a query sees has no number for a gradient)
 #pragma unroll
@@ -453,7 +473,7 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = c * 4 + e, j = c * 8 + e;
-                    const bool sees = j >= least && (bits[e] & (1u << col));
+                    const bool sees = j >= least && j < end && (bits[e] & (1u << col));
                     s[i] = none & (1u << j) ? __builtin_nanf("") : s[i];
                     s[i] = sees ? s[i] : -__builtin_inff();
                     dp[i] = sees ? dp[i] : 0.0f;
@@ -471,11 +491,12 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
             }
         }
     };
-    load();
+    fetch(0);
     __syncthreads();
-    if (of_head > 0) store(0);
-    load();
+    if (of_head > 0) place(0);
+    if (LAY != kDirect) fetch(1);
     __syncthreads();
+    if (LAY == kDirect) fetch(1);
     int buffer = 0;
     uint32_t turn = 0;
     for (int32_t g = 0; g < a.group; ++g) {
@@ -497,11 +518,12 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
                 sums_of(tile, 1);
                 attn_pace<4 * NT, 8 * NT, 0>();
             }
-            if (t + 1 < of_head || g + 1 < a.group) store(buffer ^ 1);
-            load();
+            if (t + 1 < of_head || g + 1 < a.group) place(buffer ^ 1);
+            if (LAY != kDirect) fetch(buffer);
+            __syncthreads();
+            if (LAY == kDirect) fetch(buffer);
             buffer ^= 1;
             turn = turn == 2 ? 0 : turn + 1;
-            __syncthreads();
         }
     }
     int8_t* const own = lds + wave * D * 80;
@@ -532,12 +554,12 @@ template <int NT, bool PLAIN>
 static int grad_launch(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_grid, hipStream_t st) {
     if (dq_grid) {
         const int lay = attn_layout(a.k, a.v, a.dim);
-        if (int e = lay == kRows ? dq_launch<NT, PLAIN, kRows>(a, dq_grid, st) : lay == kColumns ? dq_launch<NT, PLAIN, kColumns>(a, dq_grid, st) : dq_launch<NT, PLAIN, kAnyLayout>(a, dq_grid, st)) return e;
+        if (int e = lay == kDirect ? dq_launch<NT, PLAIN, kDirect>(a, dq_grid, st) : lay == kColumns ? dq_launch<NT, PLAIN, kColumns>(a, dq_grid, st) : dq_launch<NT, PLAIN, kAnyLayout>(a, dq_grid, st)) return e;
     }
     const unsigned more = a.dtable ? a.heads : 0;
     if (dkv_grid + more == 0) return 0;
     const int lay = attn_layout(a.q, a.dout, a.dim);
-    return lay == kRows      ? dkv_launch<NT, PLAIN, kRows>(a, dkv_grid, more, st)
+    return lay == kDirect    ? dkv_launch<NT, PLAIN, kDirect>(a, dkv_grid, more, st)
            : lay == kColumns ? dkv_launch<NT, PLAIN, kColumns>(a, dkv_grid, more, st)
                              : dkv_launch<NT, PLAIN, kAnyLayout>(a, dkv_grid, more, st);
 }
