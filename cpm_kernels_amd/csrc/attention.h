@@ -76,12 +76,13 @@ __device__ __forceinline__ int32_t attn_bucket(const Attention& a, int32_t rel) 
     return max(0, min(bucket, a.buckets - 1));
 }
 
-// The biases of a head by distance, times log2(e), in LDS: entry i is that of the distance i + first_distance - kBiasPad, clamped to the table's ends.
+// The biases of a head by distance over the scores' scale, in LDS: where a product's sums begin.  Entry i is that of the distance i + first_distance - kBiasPad, clamped to the table's ends.
 __device__ __forceinline__ int attn_bias_entries(const Attention& a) { return a.distances - a.first_distance + 2 * kBiasPad; }
-__device__ __forceinline__ void attn_biases(const Attention& a, int32_t head, float* biases, int tid, int threads) {
+__device__ __forceinline__ void attn_biases(const Attention& a, int32_t head, float scale, float* biases, int tid, int threads) {
+    const float factor = kLog2e / scale;
     const half_t* const row = a.table + (int64_t)head * a.buckets;
     for (int i = tid; i < attn_bias_entries(a); i += threads)
-        biases[i] = (float)row[attn_bucket(a, max(a.first_distance, min(i + a.first_distance - kBiasPad, a.distances - 1)))] * kLog2e;
+        biases[i] = (float)row[attn_bucket(a, max(a.first_distance, min(i + a.first_distance - kBiasPad, a.distances - 1)))] * factor;
 }
 
 // Workgroup x of units * inner ones: the `inner` workgroups of a unit, which read the same keys, follow one another on one XCD, and units are dealt to the XCDs in turn.
@@ -153,21 +154,12 @@ struct AttnShare {
     half8_t r[PIECES];
 
     __device__ __forceinline__ void load(const half_t* base, int64_t token, int64_t unit, int dim, int32_t t0, int32_t tokens, int tid) {
-        const bool whole = t0 + kAttnTile <= tokens;
         if constexpr (LAY == kColumns) {
             const int tb = (tid & 7) * 8, u0 = (tid >> 3) * PIECES;
-            if (whole) {
+            const half_t* p[PIECES];
 #pragma unroll
-                for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(base + min(u0 + i, dim - 1) * unit + t0 + tb);
-            } else {
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    half_t y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = base[min(u0 + i, dim - 1) * unit + min(t0 + tb + e, tokens - 1)];
-                    r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
-                }
-            }
+            for (int i = 0; i < PIECES; ++i) p[i] = base + min(u0 + i, dim - 1) * unit + tb;
+            load_columns(p, t0, tokens, tb);
         } else if (unit == 1 && dim % 8 == 0) {
             const int row = tid / RUN, u = min((tid % RUN) * 8, dim - 8);
 #pragma unroll
@@ -176,9 +168,24 @@ struct AttnShare {
             const int row = tid / RUN, u = (tid % RUN) * 8;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                half_t y[8];
+                half_t y[8];            // (element by element into the vector itself leaves it in scratch memory)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] = base[min(t0 + row + i * STEP, tokens - 1) * token + min(u + e, dim - 1) * unit];
+                r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+            }
+        }
+    }
+    // p: the thread's units at its first token of the tensor's first tile, the tb-th
+    __device__ __forceinline__ void load_columns(const half_t* const (&p)[PIECES], int32_t t0, int32_t tokens, int tb) {
+        if (t0 + kAttnTile <= tokens) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(p[i] + t0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                half_t y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = p[i][min(t0 + tb + e, tokens - 1) - tb];
                 r[i] = half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
             }
         }
@@ -306,8 +313,26 @@ struct AttnTiles {
     const half_t* base;
     int64_t token, unit;
     AttnShare<D, LAY, 256> share;
-    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int) { base = b, token = t.token, unit = t.unit; }
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int, int, int) { base = b, token = t.token, unit = t.unit; }
+    __device__ __forceinline__ void advance(int64_t by) { base += by; }
     __device__ __forceinline__ void fetch(int8_t*, int dim, int32_t t0, int32_t tokens, int tid, int, int) { share.load(base, token, unit, dim, t0, tokens, tid); }
+    __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t t0, int32_t tokens, int tid, int, int, uint32_t* bad) { share.store(lds, dim, t0, tokens, tid, bad != nullptr, bad); }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int, int) const { return share.largest(m); }
+};
+template <int D>
+struct AttnTiles<D, kColumns> {
+    static constexpr int PIECES = AttnShare<D, kColumns, 256>::PIECES;
+    const half_t* p[PIECES];
+    AttnShare<D, kColumns, 256> share;
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int dim, int tid, int, int) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) p[i] = b + min((tid >> 3) * PIECES + i, dim - 1) * t.unit + (tid & 7) * 8;
+    }
+    __device__ __forceinline__ void advance(int64_t by) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) p[i] += by;
+    }
+    __device__ __forceinline__ void fetch(int8_t*, int, int32_t t0, int32_t tokens, int tid, int, int) { share.load_columns(p, t0, tokens, (tid & 7) * 8); }
     __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t t0, int32_t tokens, int tid, int, int, uint32_t* bad) { share.store(lds, dim, t0, tokens, tid, bad != nullptr, bad); }
     __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int, int) const { return share.largest(m); }
 };
@@ -316,10 +341,11 @@ struct AttnTiles<D, kDirect> {
     const half_t* base;
     int64_t token;
     AttnDirect<D> direct;
-    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int wave, int lane) {
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int, int wave, int lane) {
         base = b, token = t.token;
         direct.init(token, wave, lane);
     }
+    __device__ __forceinline__ void advance(int64_t by) { base += by; }
     __device__ __forceinline__ void fetch(int8_t* lds, int dim, int32_t t0, int32_t tokens, int, int wave, int lane) { direct.issue(base + t0 * token, token, tokens - t0, lds, dim, wave, lane); }
     __device__ __forceinline__ void place(int8_t* lds, int, int32_t, int32_t, int, int wave, int lane, uint32_t* bad) {
         if (bad != nullptr) AttnDirect<D>::guard(lds, wave, lane, bad);
@@ -343,9 +369,10 @@ __device__ __forceinline__ void attn_keep_columns(half8_t (&x)[KS], const int8_t
     for (int s = 0; s < KS; ++s) x[s] = attn_rows<D>(tiles + (wave >> 1) * kAttnTile * D * 2, at, wave & 1, s);
 }
 
-// 32 bytes of a row of a mask as bits, on their way from memory
+// 32 bytes of a row of a mask as bits, or one byte, on their way from memory
 struct AttnMaskShare {
     uint4_t raw[2];
+    uint8_t byte;
     __device__ __forceinline__ void load(const uint8_t* row, int32_t key, int32_t length) {
         struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
         if (length < 32) return;
@@ -467,9 +494,11 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* base, co
 
 // The order of a stretch of products whose operands come from LDS, first M1 of R1 reads, then M2 of M2: eight reads ahead, so that their latency lies behind products (the compiler by
 // itself reads an operand right before its product and waits).
-template <int M1, int R1, int M2>
+// With B: before M2, B other reads (where its sums begin).
+template <int M1, int R1, int M2, int B = 0>
 __device__ __forceinline__ void attn_pace() {
     constexpr int kAhead = M2 >= 8 || M2 == 0 ? 8 : M2, kEach = M1 ? R1 / M1 : 1;
+    if (B) __builtin_amdgcn_sched_group_barrier(0x100, B, 0);
     static_assert(M1 == 0 || R1 % M1 == 0, "reads of a product");
     __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
@@ -482,6 +511,29 @@ __device__ __forceinline__ void attn_pace() {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         if (i < M2 - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+}
+
+// Where the sums of a tile's scores begin, for a wave with keys as rows: the biases' entries from `first` on downwards
+__device__ __forceinline__ void attn_begin(float16_tv& s, int blk, const float* first) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = first[-(blk * 32 + (i >> 2) * 8 + (i & 3))];
+}
+// The lane's entry for key 0 of a tile of 64 (or 32) keys, its query being `rel` behind it: windows beyond the table's ends are moved into the entries of the end that they are beyond
+__device__ __forceinline__ const float* attn_window(const Attention& a, const float* biases, int32_t rel, int half) {
+    return biases + max(63, min(rel - half * 4 - (a.first_distance - kBiasPad), attn_bias_entries(a) - 1));
+}
+// Scores of keys that a mask leaves out: -inf.  caps: +inf or -inf by key (the smaller of a number that is none and -inf is -inf); bits: a query's, the half's first key lowest
+__device__ __forceinline__ void attn_cap(float16_tv& s, int blk, int half, const float* caps) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const float4_t x = *reinterpret_cast<const float4_t*>(caps + blk * 32 + c * 8 + half * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[c * 4 + e] = fminf(s[c * 4 + e], x[e]);
+    }
+}
+__device__ __forceinline__ void attn_cap_each(float16_tv& s, uint32_t bits) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = bits & (1u << ((i >> 2) * 8 + (i & 3))) ? s[i] : -__builtin_inff();
 }
 
 constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};

@@ -19,12 +19,13 @@ constexpr int kAttnRows = 128, kAttnLeast = 4;       // queries of a workgroup; 
 constexpr int kLazy = 8;            // log2 of how far the running maximum may lie below the true one
 constexpr float kLift = 7.0f;       // log2 of the largest probability's size right behind a change of the maximum
 
-template <int NT, bool PLAIN, int LAY, bool TRAIN>
+template <int NT, bool BIAS, int LAY, bool TRAIN>
 __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys, two of values, biases
     __shared__ uint32_t bad[3][2];              // tokens of a tile whose values are no finite numbers; those of tile t in t % 3
     __shared__ uint32_t mask_bits[2][kAttnRows][2];
+    __shared__ __attribute__((aligned(16))) float mask_caps[2][kAttnTile];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
@@ -54,24 +55,25 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     const int32_t all_see = a.causal ? min(range.len, range.pos + min(q_first, a.tokens - 1) + 1) : range.len;
     const int32_t any_sees = q_first >= a.tokens ? 0 : a.causal ? min(range.len, range.pos + last + 1) : range.len;
     const int32_t every_sees = a.causal ? min(range.len, range.pos + qt * kAttnRows + 1) : range.len;
-    const bool flip = a.scale < 0.0f;           // (so that the largest score is the largest product)
-    const float scale = flip ? -a.scale : a.scale;
-    const bool masked = !PLAIN && a.mask != nullptr, biased = !PLAIN && a.table != nullptr;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);         // (of queries times its sign: the largest score is the largest product)
+    const bool masked = a.mask != nullptr;
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
+    const bool each = masked && a.mask_token != 0;          // a row of the mask for each query, or one for all
     const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + min(qt * kAttnRows + (tid >> 1), a.tokens - 1) * a.mask_token : nullptr;
 
     // Keys, and the mask's bits, come a tile before the values: scores of the next tile are formed beside this one's sums.
     const int32_t t_begin = split * parts.per_part, t_end = min(t_begin + parts.per_part, parts.tiles);
     AttnTiles<D, LAY> ks, vs;
-    ks.init(keys, a.k, wave, lane);
-    vs.init(values, a.v, wave, lane);
+    ks.init(keys, a.k, a.dim, tid, wave, lane);
+    vs.init(values, a.v, a.dim, tid, wave, lane);
     AttnMaskShare ms;
     ushort8_t largest = {0, 0, 0, 0, 0, 0, 0, 0};
     const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a value that is no finite number must not reach the queries that do not see it)
     auto fetch = [&](int32_t t) __attribute__((always_inline)) {
         if (t + 1 < t_end) {
             ks.fetch(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane);
-            if (masked) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
+            if (each) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
+            else if (masked && tid < kAttnTile) ms.byte = mask[min((t + 1) * kAttnTile + tid, a.length - 1)];
         }
         if (t >= t_begin && t < t_end) vs.fetch(lds + (2 + (t & 1)) * kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
     };
@@ -88,11 +90,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
         attn_keep_columns<D, KS>(q, lds + 2 * kTileBytes, wave, lane);
     } else
         attn_keep<KS>(q, a.q, a.q.at(b, h) + query * a.q.token, a.dim, half);
-    if (flip)
+    if (!(a.scale > 0.0f))
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = -q[s];
-    if (biased) attn_biases(a, h, biases, tid, 256);
-    const int32_t lo_rel = a.first_distance - kBiasPad;
+        for (int s = 0; s < KS; ++s) q[s] *= (half_t)(a.scale < 0.0f ? -1.0f : 0.0f);
+    if (BIAS) attn_biases(a, h, scale, biases, tid, 256);
     __syncthreads();
     if (LAY == kDirect) fetch(t_begin - 1);
 
@@ -104,7 +105,12 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     float top = -__builtin_inff(), sum = 0.0f;
     auto scores_of = [&](int32_t t) {
         const int8_t* const tile = lds + (t & 1) * kTileBytes;
-        s[0] = s[1] = kZero16;
+        if (BIAS) {
+            const float* const first = attn_window(a, biases, where - t * kAttnTile, half);
+            attn_begin(s[0], 0, first);
+            attn_begin(s[1], 1, first);
+        } else
+            s[0] = s[1] = kZero16;
 #pragma unroll
         for (int u = 0; u < KS; ++u)
 #pragma unroll
@@ -125,19 +131,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
         const int32_t k0 = t * kAttnTile;
         const bool active = t >= t_begin && k0 < any_sees;
         if (active) {
-            float factor = scale, add = 0.0f;
-            // one bias for the whole tile where all its distances lie beyond the table's end
-            const int32_t rel_min = range.pos + q_first - (k0 + kAttnTile - 1), rel_max = range.pos + last - k0;
-            const bool near = biased && rel_min < a.distances - 1 && rel_max > a.first_distance;
-            if (biased && !near) add = biases[(rel_min >= a.distances - 1 ? a.distances - 1 : a.first_distance) - lo_rel];
-            if (near) {
-                const float* const bp = biases + (where - k0 - half * 4 - lo_rel);
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[blk][i] = __builtin_fmaf(s[blk][i], factor, bp[-(blk * 32 + (i >> 2) * 8 + (i & 3))]);
-                factor = 1.0f;
-            }
             if (k0 + kAttnTile > all_see) {
                 const int32_t seen = limit - k0 - half * 4;
 #pragma unroll
@@ -148,9 +141,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
             if (masked) {
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
-                    const uint32_t bits = mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[blk][i] = bits & (1u << ((i >> 2) * 8 + (i & 3))) ? s[blk][i] : -__builtin_inff();
+                    if (each) attn_cap_each(s[blk], mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4));
+                    else attn_cap(s[blk], blk, half, mask_caps[t & 1]);
                 }
             }
             float m = s[0][0];
@@ -158,7 +150,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) m = fmaxf(m, s[blk][j]);
-            m = __builtin_fmaf(m, factor, add);
+            m *= scale;
             {
                 const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
                 const uint32_t low = both[0], high = both[1];       // (a bit cast of a vector's element itself takes the first one's)
@@ -171,13 +163,13 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[n] *= f;
             }
-            const float shift = add - (top == -__builtin_inff() ? 0.0f : top) + kLift;
+            const float shift = kLift - (top == -__builtin_inff() ? 0.0f : top);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float part = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][(e & 1) * 8 + j], factor, shift));
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][(e & 1) * 8 + j], scale, shift));
                     part += x;
                     p[e][j] = (half_t)x;
                     if (TRAIN) left[e][j] = (half_t)(x - (float)p[e][j]);
@@ -188,7 +180,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
         if (LAY == kDirect) wait_vmcnt<0>();
         if (t + 1 < t_end) {
             ks.place(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane, nullptr);
-            if (masked) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
+            if (each) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
+            else if (masked && tid < kAttnTile) mask_caps[(t + 1) & 1][tid] = ms.byte ? __builtin_inff() : -__builtin_inff();
         }
         if (t >= t_begin) {
             int8_t* const tile = lds + (2 + (t & 1)) * kTileBytes;
@@ -211,10 +204,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
             }
             sums_of(t);
             scores_of(t + 1);
-            attn_pace<4 * NT * (TRAIN ? 2 : 1), 8 * NT, 2 * KS>();
+            attn_pace<4 * NT * (TRAIN ? 2 : 1), 8 * NT, 2 * KS, BIAS ? 16 : 0>();
         } else if ((t + 1) * kAttnTile < any_sees && t + 1 < t_end) {
             scores_of(t + 1);
-            attn_pace<0, 0, 2 * KS>();
+            attn_pace<0, 0, 2 * KS, BIAS ? 16 : 0>();
         }
     }
     sum += __shfl_xor(sum, 32);
@@ -332,27 +325,27 @@ AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, i
     return p;
 }
 
-template <int NT, bool PLAIN, int LAY, bool TRAIN>
+template <int NT, bool BIAS, int LAY, bool TRAIN>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_attn<NT, PLAIN, LAY, TRAIN>, 150 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn<NT, PLAIN, LAY, TRAIN>), dim3(grid), dim3(256), lds, st, a);
+    if (int e = enable_dynamic_lds((const void*)k_attn<NT, BIAS, LAY, TRAIN>, 150 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_attn<NT, BIAS, LAY, TRAIN>), dim3(grid), dim3(256), lds, st, a);
     return 0;
 }
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool BIAS, int LAY>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
-    return a.lse ? attn_launch<NT, PLAIN, LAY, true>(a, grid, st) : attn_launch<NT, PLAIN, LAY, false>(a, grid, st);
+    return a.lse ? attn_launch<NT, BIAS, LAY, true>(a, grid, st) : attn_launch<NT, BIAS, LAY, false>(a, grid, st);
 }
-template <int NT, bool PLAIN>
+template <int NT, bool BIAS>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     const int lay = attn_layout(a.k, a.v, a.dim);
-    return lay == kDirect ? attn_launch<NT, PLAIN, kDirect>(a, grid, st) : lay == kColumns ? attn_launch<NT, PLAIN, kColumns>(a, grid, st) : attn_launch<NT, PLAIN, kAnyLayout>(a, grid, st);
+    return lay == kDirect ? attn_launch<NT, BIAS, kDirect>(a, grid, st) : lay == kColumns ? attn_launch<NT, BIAS, kColumns>(a, grid, st) : attn_launch<NT, BIAS, kAnyLayout>(a, grid, st);
 }
 template <int NT>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
-    return a.table || a.mask ? attn_launch<NT, false>(a, grid, st) : attn_launch<NT, true>(a, grid, st);
+    return a.table ? attn_launch<NT, true>(a, grid, st) : attn_launch<NT, false>(a, grid, st);
 }
 
 }  // namespace cpmk

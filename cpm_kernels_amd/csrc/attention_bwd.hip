@@ -46,12 +46,13 @@ __device__ __forceinline__ int attn_exponent(float dout_square, float value_squa
     return bound > 0.0f && bound < __builtin_inff() ? -max(-100, min(__builtin_amdgcn_frexp_expf(bound), 100)) : 0;
 }
 
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool BIAS, int LAY>
 __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad a) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys and values; biases; sums of ds by distance, of each wave
-    __shared__ uint32_t bad[3][2];              // tokens of a tile whose keys are no finite numbers; those of tile t in t % 3
+    __shared__ uint32_t bad[3][2];              // tokens of a tile whose keys (and, masked, values) are no finite numbers; those of tile t in t % 3
     __shared__ uint32_t mask_bits[2][kGradRows][2];
+    __shared__ __attribute__((aligned(16))) float mask_caps[2][kAttnTile];
     __shared__ float tops[4];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -73,14 +74,16 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     const int32_t every_sees = a.causal ? min(range.len, range.pos + qt * kGradRows + 1) : range.len;
     const int32_t keys_seen = a.causal ? max(0, min(range.len, range.pos + q_last_of_all + 1)) : range.len;
     const int32_t tiles = (keys_seen + kAttnTile - 1) / kAttnTile;
-    const bool masked = !PLAIN && a.mask != nullptr, biased = !PLAIN && a.table != nullptr, table_wanted = !PLAIN && a.table_parts != nullptr;
+    const bool masked = a.mask != nullptr, table_wanted = BIAS && a.table_parts != nullptr;
+    const bool each = masked && a.mask_token != 0;          // a row of the mask for each query, or one for all
+    const float scale = a.scale == 0.0f ? 1.0f : a.scale;
     const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + min(qt * kGradRows + (tid >> 1), a.tokens - 1) * a.mask_token : nullptr;
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
     const int64_t row = (b * a.heads + h) * a.tokens + query;
 
     AttnTiles<D, LAY> ks, vs;
-    ks.init(keys, a.k, wave, lane);
-    vs.init(values, a.v, wave, lane);
+    ks.init(keys, a.k, a.dim, tid, wave, lane);
+    vs.init(values, a.v, a.dim, tid, wave, lane);
     AttnMaskShare ms;
     const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a key that is no finite number must not reach the queries that do not see it)
     auto fetch = [&](int32_t t) __attribute__((always_inline)) {
@@ -88,15 +91,17 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         int8_t* const buffer = lds + (t & 1) * 2 * kTileBytes;
         ks.fetch(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane);
         vs.fetch(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
-        if (masked) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
+        if (each) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
+        else if (masked && tid < kAttnTile) ms.byte = mask[min(t * kAttnTile + tid, a.length - 1)];
     };
     auto place = [&](int32_t t) __attribute__((always_inline)) {
         if (t >= tiles) return;
         int8_t* const buffer = lds + (t & 1) * 2 * kTileBytes;
         if (LAY == kDirect) wait_vmcnt<0>();
         ks.place(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane, guarded(t) ? bad[(uint32_t)t % 3] : nullptr);
-        vs.place(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane, nullptr);
-        if (masked) mask_bits[t & 1][tid >> 1][tid & 1] = ms.bits(mask, t * kAttnTile + (tid & 1) * 32, a.length);
+        vs.place(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane, masked ? bad[(uint32_t)t % 3] : nullptr);        // (0 times no number is none)
+        if (each) mask_bits[t & 1][tid >> 1][tid & 1] = ms.bits(mask, t * kAttnTile + (tid & 1) * 32, a.length);
+        else if (masked && tid < kAttnTile) mask_caps[t & 1][tid] = ms.byte ? __builtin_inff() : -__builtin_inff();
         if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;
     };
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
@@ -104,9 +109,9 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     if (LAY == kDirect) __syncthreads();
     fetch(0);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
-    const int entries = biased ? attn_bias_entries(a) : 0;
+    const int entries = BIAS ? attn_bias_entries(a) : 0;
     float* const sums = biases + entries + wave * entries;
-    if (biased) attn_biases(a, h, biases, tid, 256);
+    if (BIAS) attn_biases(a, h, scale, biases, tid, 256);
     if (table_wanted)
         for (int i = tid; i < 4 * entries; i += 256) biases[entries + i] = 0.0f;
     const int32_t lo_rel = a.first_distance - kBiasPad;
@@ -172,6 +177,9 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         minus_lse = kProbScale - lse;
         minus_delta = lse == __builtin_inff() ? 0.0f : -delta * dscale;
     }
+    if (a.scale == 0.0f)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] *= (half_t)0;
     __syncthreads();
     if (tid == 0) a.dout_top[(b * a.heads + h) * a.row_tiles + qt] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     place(0);
@@ -188,6 +196,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     auto scores_of = [&](int32_t t, int blk) __attribute__((always_inline)) {
         const int8_t* const tile = lds + (t & 1) * 2 * kTileBytes;
         s = dp = kZero16;
+        if (BIAS) attn_begin(s, 0, attn_window(a, biases, where - t * kAttnTile - blk * 32, half));
 #pragma unroll
         for (int u = 0; u < KS; ++u) {
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D>(tile, at_rows, blk, u), q[u], s, 0, 0, 0);
@@ -204,28 +213,20 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     // ds of a block of 32 keys, as fp16
     auto gradients_of = [&](int32_t t, int blk) __attribute__((always_inline)) {
         const int32_t k0 = t * kAttnTile + blk * 32;
-        const int32_t rel_min = range.pos + q_first - (k0 + 31), rel_max = range.pos + last - k0;
-        const bool near = biased && rel_min < a.distances - 1 && rel_max > a.first_distance, before = rel_min >= a.distances - 1;
-        float add = minus_lse;
-        if (biased && !near) add += biases[(before ? a.distances - 1 : a.first_distance) - lo_rel];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], a.scale, add);
-        const int32_t of_lane = where - k0 - half * 4 - lo_rel;
-        const int32_t rel_of_corner = range.pos + q_first - k0 - 31 - lo_rel;        // distance of the block's first query from its last key
-        if (near) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] += biases[of_lane - ((i >> 2) * 8 + (i & 3))];
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], scale, minus_lse);
+        if (masked) {
+            if (each) attn_cap_each(s, mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4));
+            else attn_cap(s, blk, half, mask_caps[t & 1]);
         }
         const uint32_t spoilt = bad[(uint32_t)t % 3][blk];
-        if (k0 + 32 > all_see || masked || spoilt) {
+        if (k0 + 32 > all_see || spoilt) {
             const int32_t seen = limit - k0 - half * 4;
-            uint32_t bits = 0xffffffffu, none = 0;
-            if (masked) bits = mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4);
-            none = spoilt >> (half * 4);        // (a query that sees such a key has no number for a gradient)
+            const uint32_t none = spoilt >> (half * 4);        // (a query that sees such a key has no number for a gradient)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int j = (i >> 2) * 8 + (i & 3);
-                const bool sees = j < seen && (bits & (1u << j));
+                const bool sees = j < seen && s[i] != -__builtin_inff();
                 s[i] = none & (1u << j) ? __builtin_nanf("") : s[i];
                 s[i] = sees ? s[i] : -__builtin_inff();
                 dp[i] = sees ? dp[i] : 0.0f;
@@ -234,7 +235,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]) * __builtin_fmaf(dp[i], dscale, minus_delta);
         if (table_wanted) {
-            if (near) {
+            const int32_t rel_min = range.pos + q_first - (k0 + 31), rel_max = range.pos + last - k0;
+            const int32_t rel_of_corner = rel_min - lo_rel;         // of the block's first query from its last key
+            const bool before = rel_min >= a.distances - 1;
+            if (!before && rel_max > a.first_distance) {
                 // Through LDS: a lane writes its 16 keys beside each other, a row a query, and then sums a diagonal, lane l that of distance l - 31 from the block's corner.  (64 float
                 // additions in LDS itself, which has an instruction for them, took ten times as long as the block's products.)  All of it is the wave's own.
 #pragma unroll
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     };
     if (0 < any_sees) {
         scores_of(0, 0);
-        attn_pace<0, 0, 2 * KS>();
+        attn_pace<0, 0, 2 * KS, BIAS ? 8 : 0>();
     }
     for (int32_t t = 0; t < tiles; ++t) {
         const bool one = t * kAttnTile < any_sees;          // (the second block of the tile: scores that nobody sees, or zeros)
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
             gradients_of(t, 0);
             sums_of(t, 0);
             scores_of(t, 1);
-            attn_pace<2 * NT, 4 * NT, 2 * KS>();
+            attn_pace<2 * NT, 4 * NT, 2 * KS, BIAS ? 8 : 0>();
             gradients_of(t, 1);
             sums_of(t, 1);
             attn_pace<2 * NT, 4 * NT, 0>();
@@ -289,7 +293,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         if (LAY == kDirect) fetch(t + 2);
         if ((t + 1) * kAttnTile < any_sees) {
             scores_of(t + 1, 0);
-            attn_pace<0, 0, 2 * KS>();
+            attn_pace<0, 0, 2 * KS, BIAS ? 8 : 0>();
         }
     }
     attn_write<NT>(a.dq, a.dq.at(b, h), acc, undo * a.natural_scale, q_first, a.tokens, a.dim, lane, lds + wave * D * 80);
@@ -333,7 +337,7 @@ __device__ __forceinline__ void attn_dtable(const AttentionGrad& a, int64_t h, f
     }
 }
 
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool BIAS, int LAY>
 __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad a, uint32_t blocks) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of queries and their results' gradients; biases of the heads in turn
@@ -342,7 +346,7 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     __shared__ __attribute__((aligned(16))) uint32_t mask_bits[2][4][kAttnTile];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (!PLAIN && blockIdx.x >= blocks) return attn_dtable(a, blockIdx.x - blocks, reinterpret_cast<float*>(lds), tid);
+    if (BIAS && blockIdx.x >= blocks) return attn_dtable(a, blockIdx.x - blocks, reinterpret_cast<float*>(lds), tid);
     const uint32_t inner = (uint32_t)ceil_div(a.length, kGradRows);
     uint32_t unit, kt;
     attn_deal(blockIdx.x, blocks / inner, inner, unit, kt);         // (of causal keys the first are seen by most queries)
@@ -350,7 +354,8 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     const int32_t kvh = unit - (uint32_t)b * a.held;
     const AttnRange range = attn_range(a, b);
     const int32_t k_first_of_all = kt * kGradRows, k_first = k_first_of_all + wave * 32, key = k_first + col;
-    const bool masked = !PLAIN && a.mask != nullptr, biased = !PLAIN && a.table != nullptr;
+    const bool masked = a.mask != nullptr && a.mask_token != 0;         // (by a row for each query)
+    const float scale = a.scale == 0.0f ? 1.0f : a.scale;
     // tiles of queries that see any key of the workgroup
     const int32_t first_query = a.causal ? max(0, k_first_of_all - range.pos) : 0;
     const int32_t first_tile = min(first_query / kAttnTile, a.query_tiles);
@@ -368,6 +373,15 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         attn_keep<KS>(k, a.k, a.k.at(b, kvh) + mine * a.k.token, a.dim, half);
         attn_keep<KS>(v, a.v, a.v.at(b, kvh) + mine * a.v.token, a.dim, half);
     }
+    // Keys past the end, and keys that one mask for all queries leaves out: zeros, their scores -inf
+    const bool out_of_all = key >= range.len || (a.mask != nullptr && a.mask_token == 0 && a.mask[b * a.mask_batch + min(key, a.length - 1)] == 0);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        if (out_of_all) k[s] = v[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        if (a.scale == 0.0f) k[s] *= (half_t)0;
+    }
+    const float of_lane = out_of_all ? -__builtin_inff() : 0.0f;
+    const bool some_out = k_first_of_all + kGradRows > range.len || (a.mask != nullptr && a.mask_token == 0);       // (the same for the whole workgroup)
     const float dout_top = attn_largest(a.dout_top + (b * a.heads + kvh * a.group) * a.row_tiles, (int64_t)a.group * a.row_tiles, lane);
     const int exponent = attn_exponent(dout_top, attn_value_norm(a, b, kvh, lane));
     const float dscale = ldexpf(1.0f, exponent);
@@ -378,14 +392,14 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     if (LAY == kDirect) __syncthreads();
 
     AttnTiles<D, LAY> qs, gs;
-    qs.init(a.q.at(b, kvh * a.group), a.q, wave, lane);
-    gs.init(a.dout.at(b, kvh * a.group), a.dout, wave, lane);
+    qs.init(a.q.at(b, kvh * a.group), a.q, a.dim, tid, wave, lane);
+    gs.init(a.dout.at(b, kvh * a.group), a.dout, a.dim, tid, wave, lane);
     AttnMaskShare ms;
     float fact = 0.0f;
     int32_t h_fetch = kvh * a.group, t_fetch = 0, t_place = 0;       // head and tile of the head to be fetched next, the tile to be placed next
     int32_t left = of_head * a.group;           // tiles still to be fetched
     uint32_t phase_place = 0;          // of `bad`
-    const auto guarded = [&](int32_t q0) { return masked || q0 + kAttnTile > a.tokens || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1); };
+    const auto guarded = [&](int32_t q0) { return masked || q0 + kAttnTile > a.tokens || some_out || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1); };
     auto fetch = [&](int buffer) __attribute__((always_inline)) {
         if (left == 0) return;
         const int32_t q0 = (first_tile + t_fetch) * kAttnTile;
@@ -401,8 +415,8 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         }
         if (++t_fetch == of_head) {
             t_fetch = 0, ++h_fetch;
-            qs.base += a.q.head;
-            gs.base += a.dout.head;
+            qs.advance(a.q.head);
+            gs.advance(a.dout.head);
         }
         --left;
     };
@@ -414,7 +428,13 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         qs.place(at, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
         gs.place(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
         if (masked) mask_bits[buffer][tid & 3][tid >> 2] = ms.bits(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
-        if (tid < 128) facts[buffer][tid >> 6][tid & 63] = fact;
+        if (tid < 128) {
+            // (a query whose statistics are no numbers, like one that is none itself, must not reach the keys that it does not see)
+            const float none = tid < 64 ? -__builtin_inff() : 0.0f;
+            const bool spoils = fact != none && !(fabsf(fact) < __builtin_inff());
+            facts[buffer][tid >> 6][tid & 63] = spoils ? none : fact;
+            if (spoils) atomicOr(&bad[phase_place][(tid & 63) >> 5], 1u << (tid & 31));
+        }
         if (++t_place == of_head) t_place = 0;
         phase_place = phase_place == 2 ? 0 : phase_place + 1;
         if (tid < 2) bad[phase_place][tid] = 0;
@@ -424,8 +444,13 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
 #pragma unroll
     for (int n = 0; n < NT; ++n) dk[n] = dv[n] = kZero16;
     half8_t p[2], d[2];
-    auto scores_of = [&](const int8_t* tile, int blk) __attribute__((always_inline)) {
+    auto scores_of = [&](const int8_t* tile, int32_t q0, int blk) __attribute__((always_inline)) {
         s = dp = kZero16;
+        if (BIAS) {         // (windows beyond the table's ends are moved into the entries of the end that they are beyond)
+            const float* const bp = biases + max(0, min(range.pos + q0 + blk * 32 + half * 4 - key - lo_rel, attn_bias_entries(a) - 32));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = bp[(i >> 2) * 8 + (i & 3)];
+        }
 #pragma unroll
         for (int u = 0; u < KS; ++u) {
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D>(tile, at_rows, blk, u), k[u], s, 0, 0, 0);
@@ -444,27 +469,19 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     // p and ds of a block of 32 queries, as fp16
     auto gradients_of = [&](int buffer, uint32_t turn, int32_t q0, int blk) __attribute__((always_inline)) {
         q0 += blk * 32;
-        const int32_t rel_min = range.pos + q0 - (k_first + 31), rel_max = range.pos + q0 + 31 - k_first;
-        const bool near = biased && rel_min < a.distances - 1 && rel_max > a.first_distance;
-        float add = 0.0f;
-        if (biased && !near) add = biases[(rel_min >= a.distances - 1 ? a.distances - 1 : a.first_distance) - lo_rel];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float4_t minus_lse = *reinterpret_cast<const float4_t*>(&facts[buffer][0][blk * 32 + c * 8 + half * 4]);
+            float4_t minus_lse = *reinterpret_cast<const float4_t*>(&facts[buffer][0][blk * 32 + c * 8 + half * 4]);
+            if (some_out) minus_lse += of_lane;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[c * 4 + e] = __builtin_fmaf(s[c * 4 + e], a.scale, minus_lse[e] + add);
+            for (int e = 0; e < 4; ++e) s[c * 4 + e] = __builtin_fmaf(s[c * 4 + e], scale, minus_lse[e]);
         }
         const int32_t rel = range.pos + q0 + half * 4 - key;         // of the first of the lane's queries
-        if (near) {
-            const float* const bp = biases + (rel - lo_rel);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] += bp[(i >> 2) * 8 + (i & 3)];
-        }
         const uint32_t spoilt = bad[turn][blk];
-        if (masked || spoilt || k_first + 32 > range.len || q0 + 32 > a.tokens || (a.causal && rel_min < 0)) {
+        if (masked || spoilt || q0 + 32 > a.tokens || (a.causal && range.pos + q0 - (k_first + 31) < 0)) {
             // of the block's queries (from the lane's first on) those from `least` on see the key, up to the last one
             const int32_t end = a.tokens - q0 - half * 4;
-            const int32_t least = key >= range.len ? 64 : a.causal ? -rel : -64;
+            const int32_t least = out_of_all ? 64 : a.causal ? -rel : -64;
             const uint32_t none = spoilt >> (half * 4);        // (a key that such a query sees has no number for a gradient)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -500,20 +517,20 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     int buffer = 0;
     uint32_t turn = 0;
     for (int32_t g = 0; g < a.group; ++g) {
-        if (biased && of_head > 0) {
-            attn_biases(a, kvh * a.group + g, biases, tid, 256);
+        if (BIAS && of_head > 0) {
+            attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
             __syncthreads();
         }
         for (int32_t t = 0; t < of_head; ++t) {
             const int32_t q0 = (first_tile + t) * kAttnTile;
             const int8_t* const tile = lds + buffer * 2 * kTileBytes;
             if (k_first < range.len && (!a.causal || range.pos + q0 + kAttnTile - 1 >= k_first)) {
-                scores_of(tile, 0);
-                attn_pace<0, 0, 2 * KS>();
+                scores_of(tile, q0, 0);
+                attn_pace<0, 0, 2 * KS, BIAS ? 8 : 0>();
                 gradients_of(buffer, turn, q0, 0);
                 sums_of(tile, 0);
-                scores_of(tile, 1);
-                attn_pace<4 * NT, 8 * NT, 2 * KS>();
+                scores_of(tile, q0, 1);
+                attn_pace<4 * NT, 8 * NT, 2 * KS, BIAS ? 8 : 0>();
                 gradients_of(buffer, turn, q0, 1);
                 sums_of(tile, 1);
                 attn_pace<4 * NT, 8 * NT, 0>();
@@ -531,41 +548,41 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     attn_write<NT>(a.dv, a.dv.at(b, kvh), dv, ldexpf(1.0f, -(int)kProbScale), k_first, a.length, a.dim, lane, own);
 }
 
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool BIAS, int LAY>
 static int dq_launch(const AttentionGrad& a, unsigned grid, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int entries = a.table ? a.distances - a.first_distance + 2 * kBiasPad : 0;
     const int lds = 4 * kAttnTile * D * 2 + (a.table_parts ? 5 * ((entries + 3) & ~3) + 4 * kDiagonals<NT> : entries) * 4;
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_attn_dq<NT, PLAIN, LAY>, 156 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn_dq<NT, PLAIN, LAY>), dim3(grid), dim3(256), lds, st, a);
+    if (int e = enable_dynamic_lds((const void*)k_attn_dq<NT, BIAS, LAY>, 156 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_attn_dq<NT, BIAS, LAY>), dim3(grid), dim3(256), lds, st, a);
     return 0;
 }
-template <int NT, bool PLAIN, int LAY>
+template <int NT, bool BIAS, int LAY>
 static int dkv_launch(const AttentionGrad& a, unsigned grid, unsigned more, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
     const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
-    if (int e = enable_dynamic_lds((const void*)k_attn_dkv<NT, PLAIN, LAY>, 150 * 1024, done)) return e;
-    hipLaunchKernelGGL((k_attn_dkv<NT, PLAIN, LAY>), dim3(grid + more), dim3(256), lds, st, a, grid);
+    if (int e = enable_dynamic_lds((const void*)k_attn_dkv<NT, BIAS, LAY>, 150 * 1024, done)) return e;
+    hipLaunchKernelGGL((k_attn_dkv<NT, BIAS, LAY>), dim3(grid + more), dim3(256), lds, st, a, grid);
     return 0;
 }
-template <int NT, bool PLAIN>
+template <int NT, bool BIAS>
 static int grad_launch(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_grid, hipStream_t st) {
     if (dq_grid) {
         const int lay = attn_layout(a.k, a.v, a.dim);
-        if (int e = lay == kDirect ? dq_launch<NT, PLAIN, kDirect>(a, dq_grid, st) : lay == kColumns ? dq_launch<NT, PLAIN, kColumns>(a, dq_grid, st) : dq_launch<NT, PLAIN, kAnyLayout>(a, dq_grid, st)) return e;
+        if (int e = lay == kDirect ? dq_launch<NT, BIAS, kDirect>(a, dq_grid, st) : lay == kColumns ? dq_launch<NT, BIAS, kColumns>(a, dq_grid, st) : dq_launch<NT, BIAS, kAnyLayout>(a, dq_grid, st)) return e;
     }
     const unsigned more = a.dtable ? a.heads : 0;
     if (dkv_grid + more == 0) return 0;
     const int lay = attn_layout(a.q, a.dout, a.dim);
-    return lay == kDirect    ? dkv_launch<NT, PLAIN, kDirect>(a, dkv_grid, more, st)
-           : lay == kColumns ? dkv_launch<NT, PLAIN, kColumns>(a, dkv_grid, more, st)
-                             : dkv_launch<NT, PLAIN, kAnyLayout>(a, dkv_grid, more, st);
+    return lay == kDirect    ? dkv_launch<NT, BIAS, kDirect>(a, dkv_grid, more, st)
+           : lay == kColumns ? dkv_launch<NT, BIAS, kColumns>(a, dkv_grid, more, st)
+                             : dkv_launch<NT, BIAS, kAnyLayout>(a, dkv_grid, more, st);
 }
 template <int NT>
 static int grad_launch(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_grid, hipStream_t st) {
-    return a.table || a.mask ? grad_launch<NT, false>(a, dq_grid, dkv_grid, st) : grad_launch<NT, true>(a, dq_grid, dkv_grid, st);
+    return a.table ? grad_launch<NT, true>(a, dq_grid, dkv_grid, st) : grad_launch<NT, false>(a, dq_grid, dkv_grid, st);
 }
 
 }  // namespace cpmk
