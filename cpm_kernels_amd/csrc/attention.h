@@ -35,7 +35,8 @@ constexpr int kAttnTile = 64;       // tokens a workgroup stages at a time
 constexpr int32_t kAttnFar = 1 << 30, kAttnLong = 1 << 29;       // positions stay below the one, numbers of tokens and keys up to the other: distances fit 32 bits
 constexpr int kBiasPad = 96;        // distances beyond the table's ends that a tile of 64 tokens and the 32 of a wave can reach into
 
-enum { kDirect = 0, kColumns = 1, kAnyLayout = 2, kRows = 3 };           // (kRows: rotary.hip)
+// How tiles come: units beside each other or tokens beside each other, straight into LDS (kDirect, kTurned) or through registers (kAnyLayout, kColumns); rotary.hip: kRows
+enum { kDirect = 0, kColumns = 1, kAnyLayout = 2, kTurned = 3, kRows = 4 };
 
 struct AttnRange {
     int32_t len, pos;
@@ -116,33 +117,54 @@ __device__ __forceinline__ int attn_place(int token, int piece) {
     return token * D * 2 + (((piece & ~(W - 1)) | ((piece ^ attn_swizzle<D>(token)) & (W - 1))) << 4);
 }
 
-// Lane's address for operands of rows = tokens, piece 2 s + half of token (lane & 31) + 32 blk
-template <int D>
+// Tiles of tensors whose tokens are neighbours lie unit by unit instead, as in memory, 64 tokens each, piece c of eight tokens of unit u at place c ^ turned(u).  The two ways of reading change
+// places: tokens of the lanes through the transposing read, units of the lanes as they lie (8 bytes; u and u + 16 share banks).
+__device__ __forceinline__ int attn_turned(int u) { return (u >> 1 & 1) << 2 | (u >> 3 & 1) << 1 | (u >> 2 & 1); }
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ half8_t attn_join(short4_t lo, short4_t hi) { return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)); }
+__device__ __forceinline__ short4_t attn_read_turning(const int8_t* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)p); }
+
+template <int LAY>
+constexpr bool kByUnit = LAY == kTurned || LAY == kColumns;
+
+// Lane's address for operands of rows = tokens, units 16 s + 8 half + {0..7} of token (lane & 31) + 32 blk
+template <int D, bool BY_UNIT = false>
 __device__ __forceinline__ uint32_t attn_rows_at(int lane) {
-    const int t = lane & 31;
-    return t * D * 2 + (((lane >> 5) ^ attn_swizzle<D>(t)) << 4);
+    const int t = lane & 31, half = lane >> 5;
+    if (BY_UNIT) {
+        const int j = lane & 15, u = 8 * half + (j >> 2);
+        return u * 128 + (((((lane >> 4) & 1) * 2 + ((j & 3) >> 1)) ^ attn_turned(u)) << 4) + (j & 1) * 8;
+    }
+    return t * D * 2 + ((half ^ attn_swizzle<D>(t)) << 4);
 }
-template <int D>
+template <int D, bool BY_UNIT = false>
 __device__ __forceinline__ half8_t attn_rows(const int8_t* tile, uint32_t at, int blk, int s) {
+    if (BY_UNIT) {
+        const int8_t* const p = tile + s * 16 * 128;
+        return attn_join(attn_read_turning(p + (at ^ (blk << 6))), attn_read_turning(p + 4 * 128 + (at ^ (blk << 6) ^ 16)));
+    }
     const int x = D == 64 ? (2 * s) ^ blk : ((2 * s) & 15) ^ (blk << 2);
     return *reinterpret_cast<const half8_t*>(tile + ((at ^ (x << 4)) + blk * 32 * D * 2 + (D == 256 ? (s >> 3) * 256 : 0)));
 }
 // Lane's address for operands of rows = units: of unit block n (32 units), tokens 32 blk + 16 e + 4 half + {0..3, 8..11}: the order in which the results of a product with tokens as
 // rows lie in a lane's registers 8 e .. 8 e + 7.
-template <int D>
+template <int D, bool BY_UNIT = false>
 __device__ __forceinline__ uint32_t attn_units_at(int lane) {
     const int half = lane >> 5, j = lane & 15, c = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1), t = 4 * half + (j >> 2);
+    if (BY_UNIT) return (lane & 31) * 128 + (attn_turned(lane & 31) << 4) + half * 8;
     return t * D * 2 + ((c ^ attn_swizzle<D>(t)) << 4) + (j & 1) * 8;
 }
-typedef short short4_t __attribute__((ext_vector_type(4)));
-typedef short short8_t __attribute__((ext_vector_type(8)));
-template <int D>
+template <int D, bool BY_UNIT = false>
 __device__ __forceinline__ half8_t attn_units(const int8_t* tile, uint32_t at, int n, int blk, int e) {
+    if (BY_UNIT) {
+        const int8_t* const p = tile + n * 32 * 128;
+        const int x = blk * 4 + e * 2;
+        return attn_join(*reinterpret_cast<const short4_t*>(p + (at ^ (x << 4))), *reinterpret_cast<const short4_t*>(p + (at ^ ((x + 1) << 4))));
+    }
     const int x = D == 64 ? (n << 2) ^ (e << 2) ^ blk : ((n & 3) << 2) ^ (e << 3) ^ (blk << 2);
     const int8_t* const p = tile + (blk * 32 + e * 16) * D * 2 + (D == 256 ? (n >> 2) * 256 : 0);
-    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + (at ^ (x << 4))));
-    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(p + 8 * D * 2 + (at ^ ((x ^ 2) << 4))));
-    return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return attn_join(attn_read_turning(p + (at ^ (x << 4))), attn_read_turning(p + 8 * D * 2 + (at ^ ((x ^ 2) << 4))));
 }
 
 // A thread's share of a tile on its way from memory to LDS through registers.  kColumns: eight tokens of PIECES neighbouring units, turned there.  Else pieces of eight units, unit by unit
@@ -306,42 +328,131 @@ __device__ __forceinline__ void attn_clear(int8_t* lds, int bytes, int tid, int 
     for (int i = tid; i < bytes / 16; i += threads) reinterpret_cast<uint4_t*>(lds)[i] = uint4_t{0, 0, 0, 0};
 }
 
-// A tensor's tiles, one after another: `fetch` asks for one, `place`, when it has arrived, puts it into LDS (kDirect: it is there, behind wait_vmcnt); bad: to be guarded (AttnShare::store),
+// Pieces of eight tokens from `token` on, `step` bytes apart: numbers that are none or infinite become zeros, their tokens' bits are set
+__device__ __forceinline__ void attn_clean_turned(int8_t* p, int step, int pieces, int token, uint32_t* bad) {
+#pragma unroll 1
+    for (int i = 0; i < pieces * 8; ++i) {
+        half_t* const x = reinterpret_cast<half_t*>(p + (i >> 3) * step) + (i & 7);
+        const int t = token + (i & 7);
+        if (!(*x * (half_t)0 == (half_t)0)) {
+            *x = (half_t)0;
+            atomicOr(bad + (t >> 5), 1u << (t & 31));
+        }
+    }
+}
+
+// A tensor's tiles, one after another (largest: of the magnitudes of a tile's first `count` tokens, or copies of them): `fetch` asks for one, `place`, when it has arrived, puts it into LDS (kDirect: it is there, behind wait_vmcnt); bad: to be guarded (AttnShare::store),
 // or null.  kDirect writes the buffer from `fetch` on.
 template <int D, int LAY>
 struct AttnTiles {
     const half_t* base;
     int64_t token, unit;
     AttnShare<D, LAY, 256> share;
-    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int, int, int) { base = b, token = t.token, unit = t.unit; }
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int32_t, int, int, int, int) { base = b, token = t.token, unit = t.unit; }
     __device__ __forceinline__ void advance(int64_t by) { base += by; }
     __device__ __forceinline__ void fetch(int8_t*, int dim, int32_t t0, int32_t tokens, int tid, int, int) { share.load(base, token, unit, dim, t0, tokens, tid); }
     __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t t0, int32_t tokens, int tid, int, int, uint32_t* bad) { share.store(lds, dim, t0, tokens, tid, bad != nullptr, bad); }
-    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int, int) const { return share.largest(m); }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int32_t, int, int) const { return share.largest(m); }
 };
+// (pieces of eight tokens of a unit, beside each other in memory: PIECES units of a thread, 32 apart)
 template <int D>
 struct AttnTiles<D, kColumns> {
-    static constexpr int PIECES = AttnShare<D, kColumns, 256>::PIECES;
-    const half_t* p[PIECES];
-    AttnShare<D, kColumns, 256> share;
-    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int dim, int tid, int, int) {
+    static constexpr int PIECES = D / 32;
+    const half_t* p;
+    int64_t unit;
+    half8_t r[PIECES];
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int32_t, int dim, int tid, int, int) { p = b + min(tid >> 3, dim - 1) * t.unit + (tid & 7) * 8, unit = t.unit; }
+    __device__ __forceinline__ void advance(int64_t by) { p += by; }
+    __device__ __forceinline__ void fetch(int8_t*, int dim, int32_t t0, int32_t tokens, int tid, int, int) {
+        const int tb = (tid & 7) * 8, u = tid >> 3;
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (t0 + kAttnTile <= tokens) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) p[i] = b + min((tid >> 3) * PIECES + i, dim - 1) * t.unit + (tid & 7) * 8;
-    }
-    __device__ __forceinline__ void advance(int64_t by) {
+            for (int i = 0; i < PIECES; ++i) r[i] = load_half8_any(p + (u + i * 32 < dim ? i * 32 : 0) * unit + t0);
+        } else {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) p[i] += by;
+            for (int i = 0; i < PIECES; ++i) {
+                half_t y[8];
+                const half_t* const q = p + (u + i * 32 < dim ? i * 32 : 0) * unit - tb;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = q[min(t0 + tb + e, tokens - 1)];
+                r[i] = half8_fill(half8_t{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]}, half8_keep(tokens - t0 - tb), none);
+            }
+        }
     }
-    __device__ __forceinline__ void fetch(int8_t*, int, int32_t t0, int32_t tokens, int tid, int, int) { share.load_columns(p, t0, tokens, (tid & 7) * 8); }
-    __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t t0, int32_t tokens, int tid, int, int, uint32_t* bad) { share.store(lds, dim, t0, tokens, tid, bad != nullptr, bad); }
-    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int, int) const { return share.largest(m); }
+    __device__ __forceinline__ void place(int8_t* lds, int dim, int32_t, int32_t, int tid, int, int, uint32_t* bad) {
+        const int u = tid >> 3, c = tid & 7;
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (dim < D)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                if (u + i * 32 >= dim) r[i] = none;
+        half8_t worst = none;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            *reinterpret_cast<half8_t*>(lds + (u + i * 32) * 128 + ((c ^ attn_turned(u)) << 4)) = r[i];
+            worst = __builtin_elementwise_fma(r[i], none, worst);
+        }
+        if (bad == nullptr) return;
+        const uint4_t w = __builtin_bit_cast(uint4_t, worst);
+        if ((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu) attn_clean_turned(lds + u * 128 + ((c ^ attn_turned(u)) << 4), 32 * 128, PIECES, c * 8, bad);
+    }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int32_t, int, int) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, r[i]);
+        return m;
+    }
+};
+// Straight into LDS: a wave brings D / 4 units, eight an instruction.  Whole pieces of tokens: their number is a multiple of eight, and pieces past the end are copies of the last one.
+template <int D>
+struct AttnTiles<D, kTurned> {
+    static constexpr int PIECES = D / 32;
+    const half_t* base;
+    int64_t unit;
+    int32_t all;            // tokens of the tensor
+    uint32_t off;           // (units 8 apart have the same places but for bit 1)
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int32_t tokens, int, int, int wave, int lane) {
+        base = b, unit = t.unit, all = tokens;
+        off = (uint32_t)((lane >> 3) * (int32_t)unit) * 2;
+    }
+    __device__ __forceinline__ void advance(int64_t by) { base += by; }
+    __device__ __forceinline__ void fetch(int8_t* lds, int dim, int32_t t0, int32_t, int, int wave, int lane) {
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds + wave * (D / 4) * 128;
+        const int most = min(7, ((all - t0) >> 3) - 1);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int u = wave * (D / 4) + i * 8 + (lane >> 3), c = (lane & 7) ^ attn_turned(u);
+            if (dim == D || u < dim) lds_dma16(off + min(c, most) * 16, reinterpret_cast<const int8_t*>(base + (int64_t)(wave * (D / 4) + i * 8) * unit + t0), to + i * 1024);
+        }
+    }
+    __device__ __forceinline__ void place(int8_t* lds, int, int32_t, int32_t, int, int wave, int lane, uint32_t* bad) {
+        if (bad == nullptr) return;
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+        half8_t worst = none;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) worst = __builtin_elementwise_fma(*reinterpret_cast<const half8_t*>(lds + wave * (D / 4) * 128 + i * 1024 + lane * 16), none, worst);
+        const uint4_t w = __builtin_bit_cast(uint4_t, worst);
+        if ((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu)
+#pragma unroll 1
+            for (int i = 0; i < PIECES; ++i) attn_clean_turned(lds + wave * (D / 4) * 128 + i * 1024 + lane * 16, 0, 1, ((lane & 7) ^ attn_turned(wave * (D / 4) + i * 8 + (lane >> 3))) * 8, bad);
+    }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int32_t count, int wave, int lane) const {
+        const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = (lane & 7) ^ attn_turned(wave * (D / 4) + i * 8 + (lane >> 3));
+            const half8_t x = *reinterpret_cast<const half8_t*>(lds + wave * (D / 4) * 128 + i * 1024 + lane * 16);
+            m = absbits_max(m, count < kAttnTile ? half8_fill(x, half8_keep(count - c * 8), none) : x);
+        }
+        return m;
+    }
 };
 template <int D>
 struct AttnTiles<D, kDirect> {
     const half_t* base;
     int64_t token;
     AttnDirect<D> direct;
-    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int, int, int wave, int lane) {
+    __device__ __forceinline__ void init(const half_t* b, const AttnTensor& t, int32_t, int, int, int wave, int lane) {
         base = b, token = t.token;
         direct.init(token, wave, lane);
     }
@@ -350,7 +461,7 @@ struct AttnTiles<D, kDirect> {
     __device__ __forceinline__ void place(int8_t* lds, int, int32_t, int32_t, int, int wave, int lane, uint32_t* bad) {
         if (bad != nullptr) AttnDirect<D>::guard(lds, wave, lane, bad);
     }
-    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int wave, int lane) const { return AttnDirect<D>::largest(m, lds, wave, lane); }
+    __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int32_t, int wave, int lane) const { return AttnDirect<D>::largest(m, lds, wave, lane); }
 };
 
 // Operands that the waves keep of tensors whose tokens are neighbours in memory, of 128 tokens from t0 on: through two tiles in LDS (`bring`, then, behind a barrier, `keep`).
@@ -495,21 +606,21 @@ __device__ __forceinline__ void attn_write(const AttnTensor& t, half_t* base, co
 // The order of a stretch of products whose operands come from LDS, first M1 of R1 reads, then M2 of M2: eight reads ahead, so that their latency lies behind products (the compiler by
 // itself reads an operand right before its product and waits).
 // With B: before M2, B other reads (where its sums begin).
-template <int M1, int R1, int M2, int B = 0>
+template <int M1, int R1, int M2, int R2, int B = 0>
 __device__ __forceinline__ void attn_pace() {
-    constexpr int kAhead = M2 >= 8 || M2 == 0 ? 8 : M2, kEach = M1 ? R1 / M1 : 1;
+    constexpr int kEach1 = M1 ? R1 / M1 : 1, kEach2 = M2 ? R2 / M2 : 1, kAhead = M2 == 0 || R2 >= 8 ? 8 : R2;
+    static_assert((M1 == 0 || R1 % M1 == 0) && (M2 == 0 || R2 % M2 == 0), "reads of a product");
     if (B) __builtin_amdgcn_sched_group_barrier(0x100, B, 0);
-    static_assert(M1 == 0 || R1 % M1 == 0, "reads of a product");
     __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
     for (int i = 0; i < M1; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (M2 > 0 || i < M1 - kAhead / kEach) __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+        if (M2 > 0 || i < M1 - kAhead / kEach1) __builtin_amdgcn_sched_group_barrier(0x100, kEach1, 0);
     }
 #pragma unroll
     for (int i = 0; i < M2; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (i < M2 - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (i < M2 - kAhead / kEach2) __builtin_amdgcn_sched_group_barrier(0x100, kEach2, 0);
     }
 }
 
@@ -542,8 +653,12 @@ constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 inline bool attn_direct(const AttnTensor& x, int32_t dim) {
     return x.unit == 1 && dim % 8 == 0 && aligned16(x.p) && x.batch % 8 == 0 && x.head % 8 == 0 && x.token % 8 == 0 && x.token >= 0 && x.token < (1 << 23);        // (64 tokens: offsets of 32 bits)
 }
-inline int attn_layout(const AttnTensor& x, const AttnTensor& y, int32_t dim) {
+inline bool attn_turnable(const AttnTensor& x, int32_t tokens) {
+    return x.token == 1 && tokens % 8 == 0 && aligned16(x.p) && x.batch % 8 == 0 && x.head % 8 == 0 && x.unit % 8 == 0 && x.unit >= 0 && x.unit < (1 << 26);         // (eight units: the same)
+}
+inline int attn_layout(const AttnTensor& x, const AttnTensor& y, int32_t dim, int32_t tokens) {
     if (attn_direct(x, dim) && attn_direct(y, dim)) return kDirect;
+    if (attn_turnable(x, tokens) && attn_turnable(y, tokens)) return kTurned;
     return x.token == 1 && y.token == 1 ? kColumns : kAnyLayout;
 }
 

@@ -1,0 +1,8 @@
+// Heads of 97 to 128 units (attention_bwd.hip).
+#include "attention_grad.h"
+
+namespace cpmk {
+
+int attn_grad_launch_128(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_grid, hipStream_t st) { return grad_launch<4>(a, dq_grid, dkv_grid, st); }
+
+}  // namespace cpmk
