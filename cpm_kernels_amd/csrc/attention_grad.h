@@ -17,6 +17,8 @@ struct AttentionGrad : Attention {
 constexpr int kGradRows = 128;      // queries (k_attn_dq) or keys (k_attn_dkv) of a workgroup
 constexpr float kProbScale = 15.0f;
 template <int NT>
+constexpr int kGradBuffers = NT <= 4 ? 3 : 2;         // tiles of k_attn_dkv in LDS: three take one barrier a tile (of 256 units two fit)
+template <int NT>
 constexpr int kDiagonals = (NT <= 4 ? 32 : 4) * 36 + 32;         // floats of a wave's buffer for diagonals: rows of 36, read up to 31 before and behind
 
 // The largest of n numbers, for the whole wave
@@ -339,10 +341,11 @@ __device__ __forceinline__ void attn_dtable(const AttentionGrad& a, int64_t h, f
 template <int NT, bool BIAS, bool MASK, int LAY>
 __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad a, uint32_t blocks) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256, KS = NT * 2, kTileBytes = kAttnTile * D * 2;
-    extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of queries and their results' gradients; biases of the heads in turn
-    __shared__ uint32_t bad[3][2];              // queries of a tile that are no finite numbers, or their gradients; those of tile t in t % 3
-    __shared__ __attribute__((aligned(16))) float facts[2][2][kAttnTile];        // 15 - lse and -D of a tile's queries
-    __shared__ __attribute__((aligned(16))) uint32_t mask_bits[2][4][kAttnTile];
+    constexpr int BUFS = kGradBuffers<NT>;
+    extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // BUFS buffers of queries and their results' gradients; biases of the heads in turn
+    __shared__ uint32_t bad[4][2];              // queries of a tile that are no finite numbers, or their gradients; those of tile t in t % 4
+    __shared__ __attribute__((aligned(16))) float facts[BUFS][2][kAttnTile];        // 15 - lse and -D of a tile's queries
+    __shared__ __attribute__((aligned(16))) uint32_t mask_bits[BUFS][4][kAttnTile];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (BIAS && blockIdx.x >= blocks) return attn_dtable(a, blockIdx.x - blocks, reinterpret_cast<float*>(lds), tid);
@@ -355,7 +358,7 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     const int32_t k_first_of_all = kt * kGradRows, k_first = k_first_of_all + wave * 32, key = k_first + col;
     constexpr bool BY_UNIT = kByUnit<LAY>, ARRIVES = LAY == kDirect || LAY == kTurned;
     const bool masked = MASK && a.mask != nullptr && a.mask_token != 0;         // (by a row for each query)
-    const float scale = a.scale == 0.0f ? 1.0f : a.scale;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);         // (of keys times its sign: a score of -inf stays one)
     // tiles of queries that see any key of the workgroup
     const int32_t first_query = a.causal ? max(0, k_first_of_all - range.pos) : 0;
     const int32_t first_tile = min(first_query / kAttnTile, a.query_tiles);
@@ -378,19 +381,19 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         if (out_of_all) k[s] = v[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-        if (a.scale == 0.0f) k[s] *= (half_t)0;
+        if (!(a.scale > 0.0f)) k[s] *= (half_t)(a.scale < 0.0f ? -1.0f : 0.0f);
     }
     const float of_lane = out_of_all ? -__builtin_inff() : 0.0f;
     const bool some_out = k_first_of_all + kGradRows > range.len || (MASK && a.mask != nullptr && a.mask_token == 0);       // (the same for the whole workgroup)
     const float dout_top = attn_largest(a.dout_top + (b * a.heads + kvh * a.group) * a.row_tiles, (int64_t)a.group * a.row_tiles, lane);
     const int exponent = attn_exponent(dout_top, attn_value_norm(a, b, kvh, lane));
     const float dscale = ldexpf(1.0f, exponent);
-    float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
+    float* const biases = reinterpret_cast<float*>(lds + 2 * BUFS * kTileBytes);
     const int32_t lo_rel = a.first_distance - kBiasPad;
-    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
+    if (tid < 8) bad[tid >> 1][tid & 1] = 0;
     if (ARRIVES) __syncthreads();
     if (ARRIVES && a.dim < D) {
-        attn_clear(lds, 4 * kTileBytes, tid, 256);
+        attn_clear(lds, 2 * BUFS * kTileBytes, tid, 256);
         __syncthreads();
     }
 
@@ -398,10 +401,10 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     qs.init(a.q.at(b, kvh * a.group), a.q, a.tokens, a.dim, tid, wave, lane);
     gs.init(a.dout.at(b, kvh * a.group), a.dout, a.tokens, a.dim, tid, wave, lane);
     AttnMaskShare ms;
-    float fact = 0.0f;
+    float lse = 0.0f, delta = 0.0f;
     int32_t h_fetch = kvh * a.group, t_fetch = 0, t_place = 0;       // head and tile of the head to be fetched next, the tile to be placed next
     int32_t left = of_head * a.group;           // tiles still to be fetched
-    uint32_t phase_place = 0;          // of `bad`
+    uint32_t phase_place = 0;           // of `bad`
     const auto guarded = [&](int32_t q0) { return masked || q0 + kAttnTile > a.tokens || some_out || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1); };
     auto fetch = [&](int buffer) __attribute__((always_inline)) {
         if (left == 0) return;
@@ -411,10 +414,10 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         gs.fetch(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane);
         if (masked) ms.load(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
         if (tid < 128) {
-            const int32_t query = q0 + (tid & 63);
-            const int64_t row = (b * a.heads + h_fetch) * a.tokens + min(query, a.tokens - 1);
-            const float lse = query < a.tokens ? a.lse[row] : __builtin_inff();
-            fact = tid < 64 ? kProbScale - lse : lse == __builtin_inff() ? 0.0f : -a.delta[row] * dscale;
+            // (as they are: to look at them here would be to wait for the tile)
+            const int64_t row = (b * a.heads + h_fetch) * a.tokens + min(q0 + (tid & 63), a.tokens - 1);
+            lse = a.lse[row];
+            delta = a.delta[row];
         }
         if (++t_fetch == of_head) {
             t_fetch = 0, ++h_fetch;
@@ -434,118 +437,163 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         if (tid < 128) {
             // (a query whose statistics are no numbers, like one that is none itself, must not reach the keys that it does not see)
             const float none = tid < 64 ? -__builtin_inff() : 0.0f;
+            const float fact = q0 + (tid & 63) >= a.tokens || lse == __builtin_inff() ? none : tid < 64 ? kProbScale - lse : -delta * dscale;
             const bool spoils = fact != none && !(fabsf(fact) < __builtin_inff());
             facts[buffer][tid >> 6][tid & 63] = spoils ? none : fact;
             if (spoils) atomicOr(&bad[phase_place][(tid & 63) >> 5], 1u << (tid & 31));
         }
         if (++t_place == of_head) t_place = 0;
-        phase_place = phase_place == 2 ? 0 : phase_place + 1;
-        if (tid < 2) bad[phase_place][tid] = 0;
+        phase_place = (phase_place + 1) & 3;
+        if (tid < 2) bad[phase_place][tid] = 0;         // (last looked at before the barrier of the tile before)
     };
     const uint32_t at_rows = attn_rows_at<D, BY_UNIT>(lane), at_units = attn_units_at<D, BY_UNIT>(lane);
-    float16_tv dk[NT], dv[NT], s, dp;
+    constexpr bool ROOM = NT == 3 || NT == 4;         // for registers: one wave a SIMD
+    constexpr bool AHEAD = NT <= 4;         // scores of a block beside the one before (256 units leave no registers for that)
+    float16_tv dk[NT], dv[NT], s[AHEAD ? 2 : 1], dp[AHEAD ? 2 : 1];
 #pragma unroll
     for (int n = 0; n < NT; ++n) dk[n] = dv[n] = kZero16;
     half8_t p[2], d[2];
-    auto scores_of = [&](const int8_t* tile, int32_t q0, int blk) __attribute__((always_inline)) {
-        s = dp = kZero16;
+    auto begin_of = [&](int32_t q0, int blk) __attribute__((always_inline)) {
+        s[blk & AHEAD] = dp[blk & AHEAD] = kZero16;
         if (BIAS) {         // (windows beyond the table's ends are moved into the entries of the end that they are beyond)
             const float* const bp = biases + max(0, min(range.pos + q0 + blk * 32 + half * 4 - key - lo_rel, attn_bias_entries(a) - 32));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = bp[(i >> 2) * 8 + (i & 3)];
+            for (int i = 0; i < 16; ++i) s[blk & AHEAD][i] = bp[(i >> 2) * 8 + (i & 3)];
         }
+    };
+    auto scores_of = [&](const int8_t* tile, int32_t q0, int blk) __attribute__((always_inline)) {
+        begin_of(q0, blk);
 #pragma unroll
         for (int u = 0; u < KS; ++u) {
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D, BY_UNIT>(tile, at_rows, blk, u), k[u], s, 0, 0, 0);
-            dp = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D, BY_UNIT>(tile + kTileBytes, at_rows, blk, u), v[u], dp, 0, 0, 0);
+            s[blk & AHEAD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D, BY_UNIT>(tile, at_rows, blk, u), k[u], s[blk & AHEAD], 0, 0, 0);
+            dp[blk & AHEAD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_rows<D, BY_UNIT>(tile + kTileBytes, at_rows, blk, u), v[u], dp[blk & AHEAD], 0, 0, 0);
         }
     };
-    auto sums_of = [&](const int8_t* tile, int blk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                dv[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_units<D, BY_UNIT>(tile + kTileBytes, at_units, n, blk, e), p[e], dv[n], 0, 0, 0);
-                dk[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(attn_units<D, BY_UNIT>(tile, at_units, n, blk, e), d[e], dk[n], 0, 0, 0);
-            }
-    };
-    // p and ds of a block of 32 queries, as fp16
-    auto gradients_of = [&](int buffer, uint32_t turn, int32_t q0, int blk) __attribute__((always_inline)) {
+    // Scores of pairs that do not count become -inf
+    auto mask_of = [&](int buffer, uint32_t turn, int32_t q0, int blk) __attribute__((always_inline)) {
         q0 += blk * 32;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            float4_t minus_lse = *reinterpret_cast<const float4_t*>(&facts[buffer][0][blk * 32 + c * 8 + half * 4]);
-            if (some_out) minus_lse += of_lane;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[c * 4 + e] = __builtin_fmaf(s[c * 4 + e], scale, minus_lse[e]);
-        }
-        const int32_t rel = range.pos + q0 + half * 4 - key;         // of the first of the lane's queries
         const uint32_t spoilt = bad[turn][blk];
-        if (masked || spoilt || q0 + 32 > a.tokens || (a.causal && range.pos + q0 - (k_first + 31) < 0)) {
-            // of the block's queries (from the lane's first on) those from `least` on see the key, up to the last one
-            const int32_t end = a.tokens - q0 - half * 4;
-            const int32_t least = out_of_all ? 64 : a.causal ? -rel : -64;
-            const uint32_t none = spoilt >> (half * 4);        // (a key that such a query sees has no number for a gradient)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint4_t bits = {~0u, ~0u, ~0u, ~0u};
-                if (masked) bits = *reinterpret_cast<const uint4_t*>(&mask_bits[buffer][wave][blk * 32 + c * 8 + half * 4]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = c * 4 + e, j = c * 8 + e;
-                    const bool sees = j >= least && j < end && (bits[e] & (1u << col));
-                    s[i] = none & (1u << j) ? __builtin_nanf("") : s[i];
-                    s[i] = sees ? s[i] : -__builtin_inff();
-                    dp[i] = sees ? dp[i] : 0.0f;
-                }
-            }
-        }
+        if (!(masked || spoilt || q0 + 32 > a.tokens || (a.causal && range.pos + q0 - (k_first + 31) < 0))) return;
+        // of the block's queries (from the lane's first on) those from `least` on see the key, up to the last one
+        const int32_t end = a.tokens - q0 - half * 4;
+        const int32_t least = out_of_all ? 64 : a.causal ? key - (range.pos + q0 + half * 4) : -64;
+        const uint32_t none = spoilt >> (half * 4);        // (a key that such a query sees has no number for a gradient)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float4_t minus_delta = *reinterpret_cast<const float4_t*>(&facts[buffer][1][blk * 32 + c * 8 + half * 4]);
+            uint4_t bits = {~0u, ~0u, ~0u, ~0u};
+            if (masked) bits = *reinterpret_cast<const uint4_t*>(&mask_bits[buffer][wave][blk * 32 + c * 8 + half * 4]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = __builtin_amdgcn_exp2f(s[c * 4 + e]);
-                p[c >> 1][(c & 1) * 4 + e] = (half_t)x;
-                d[c >> 1][(c & 1) * 4 + e] = (half_t)(x * __builtin_fmaf(dp[c * 4 + e], dscale, minus_delta[e]));
+                const int i = c * 4 + e, j = c * 8 + e;
+                const bool sees = j >= least && j < end && (bits[e] & (1u << col));
+                s[blk & AHEAD][i] = none & (1u << j) ? __builtin_nanf("") : s[blk & AHEAD][i];
+                s[blk & AHEAD][i] = sees ? s[blk & AHEAD][i] : -__builtin_inff();
+                dp[blk & AHEAD][i] = sees ? dp[blk & AHEAD][i] : 0.0f;
             }
         }
     };
+    // A block's p and ds, as fp16, beside the products of the next one's scores, then its sums.  One wave a SIMD is all that 128 units leave registers for, so the order is written out:
+    // operands are read kAhead products before theirs (the compiler by itself reads each right before its product and waits), and numbers are dealt out among the products.
+    auto block = [&](int buffer, uint32_t turn, int32_t q0, int blk, const int8_t* next, int32_t next_q0) __attribute__((always_inline)) {
+        constexpr int kAhead = ROOM ? 6 : 4, kFacts = ROOM ? 4 : 2, kScores = 2 * KS, kSums = 4 * NT, kPairs = 8;
+        const int8_t* const tile = lds + buffer * 2 * kTileBytes;
+        float4_t minus_lse[kFacts], minus_delta[kFacts];         // of four queries, and of the next ones
+        const auto facts_of = [&](int c) __attribute__((always_inline)) {
+            minus_lse[c % kFacts] = *reinterpret_cast<const float4_t*>(&facts[buffer][0][blk * 32 + c * 8 + half * 4]);
+            minus_delta[c % kFacts] = *reinterpret_cast<const float4_t*>(&facts[buffer][1][blk * 32 + c * 8 + half * 4]);
+        };
+        if (!AHEAD) {
+            scores_of(tile, q0, blk);
+            attn_pace<0, 0, kScores, kScores * (BY_UNIT ? 2 : 1), BIAS ? 8 : 0>();
+        }
+        mask_of(buffer, turn, q0, blk);
+#pragma unroll
+        for (int c = 0; c < kFacts - 1; ++c) facts_of(c);
+        const int now = blk & AHEAD, then = now ^ AHEAD;
+        const auto operand = [&](int i) __attribute__((always_inline)) {
+            if (i < kScores) return attn_rows<D, BY_UNIT>(next + (i & 1) * kTileBytes, at_rows, blk ^ 1, i >> 1);
+            i -= kScores;
+            return attn_units<D, BY_UNIT>(tile + (i & 1 ? 0 : kTileBytes), at_units, (i % (2 * NT)) >> 1, blk, i / (2 * NT));
+        };
+        const auto numbers = [&](int i) __attribute__((always_inline)) {
+            const int c = i >> 1;
+            if (i % 2 == 0 && c + kFacts - 1 < 4) facts_of(c + kFacts - 1);
+#pragma unroll
+            for (int e = 2 * i; e < 2 * i + 2; ++e) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[now][e], scale, minus_lse[c % kFacts][e & 3] + of_lane));
+                p[e >> 3][e & 7] = (half_t)x;
+                d[e >> 3][e & 7] = (half_t)(x * __builtin_fmaf(dp[now][e], dscale, minus_delta[c % kFacts][e & 3]));
+            }
+        };
+        constexpr int kFrom = AHEAD ? 0 : kScores;
+        if (AHEAD && BIAS) begin_of(next_q0, blk ^ 1);
+        half8_t ring[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = operand(kFrom + i);
+        if (!AHEAD)
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) numbers(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = kFrom; i < kScores + kSums; ++i) {
+            half8_t& x = ring[(i - kFrom) % kAhead];
+            if (i < kScores) {
+                float16_tv& sum = i & 1 ? dp[then] : s[then];
+                sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, (i & 1 ? v : k)[i >> 1], i == 1 || (i == 0 && !BIAS) ? kZero16 : sum, 0, 0, 0);
+            } else {
+                const int j = i - kScores, e = j / (2 * NT), n = (j % (2 * NT)) >> 1;
+                float16_tv& sum = j & 1 ? dk[n] : dv[n];
+                sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, (j & 1 ? d : p)[e], sum, 0, 0, 0);
+            }
+            if (i + kAhead < kScores + kSums) x = operand(i + kAhead);
+            if (i < kScores)
+#pragma unroll
+                for (int j = kPairs * i / kScores; j < kPairs * (i + 1) / kScores; ++j) numbers(j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const int32_t total = of_head * a.group;
     fetch(0);
+    if (BIAS && total > 0) attn_biases(a, kvh * a.group, scale, biases, tid, 256);
     __syncthreads();
-    if (of_head > 0) place(0);
+    if (total > 0) place(0);
     if (!ARRIVES) fetch(1);
     __syncthreads();
     if (ARRIVES) fetch(1);
+    const auto looked_at = [&](int32_t q0) { return k_first < range.len && (!a.causal || range.pos + q0 + kAttnTile - 1 >= k_first); };
     int buffer = 0;
-    uint32_t turn = 0;
-    for (int32_t g = 0; g < a.group; ++g) {
-        if (BIAS && of_head > 0) {
-            attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
-            __syncthreads();
-        }
-        for (int32_t t = 0; t < of_head; ++t) {
-            const int32_t q0 = (first_tile + t) * kAttnTile;
-            const int8_t* const tile = lds + buffer * 2 * kTileBytes;
-            if (k_first < range.len && (!a.causal || range.pos + q0 + kAttnTile - 1 >= k_first)) {
-                scores_of(tile, q0, 0);
-                attn_pace<0, 0, 2 * KS, 2 * KS * (BY_UNIT ? 2 : 1), BIAS ? 8 : 0>();
-                gradients_of(buffer, turn, q0, 0);
-                sums_of(tile, 0);
-                scores_of(tile, q0, 1);
-                attn_pace<4 * NT, 8 * NT, 2 * KS, 2 * KS * (BY_UNIT ? 2 : 1), BIAS ? 8 : 0>();
-                gradients_of(buffer, turn, q0, 1);
-                sums_of(tile, 1);
-                attn_pace<4 * NT, 8 * NT, 0, 0>();
+    int32_t t = 0, g = 0;
+    bool active = total > 0 && looked_at(first_tile * kAttnTile);
+    if (AHEAD && active) scores_of(lds, first_tile * kAttnTile, 0);
+    for (int32_t i = 0; i < total; ++i) {
+        const int32_t q0 = (first_tile + t) * kAttnTile;
+        if (active) block(buffer, i & 3, q0, 0, lds + buffer * 2 * kTileBytes, q0);
+        const int next = buffer + 1 == BUFS ? 0 : buffer + 1;
+        if (++t == of_head) {
+            t = 0, ++g;
+            if (BIAS && i + 1 < total) {
+                __syncthreads();
+                attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
             }
-            if (t + 1 < of_head || g + 1 < a.group) place(buffer ^ 1);
-            if (!ARRIVES) fetch(buffer);
+        }
+        // (with three buffers the one that is fetched into was last read before this barrier; scores behind the last tile are of what the buffer held, and nobody looks at them)
+        const int32_t next_q0 = (first_tile + t) * kAttnTile;
+        if (i + 1 < total) place(next);
+        if (BUFS == 3 && !ARRIVES) fetch(0);
+        __syncthreads();
+        if (BUFS == 3 && ARRIVES) fetch(next + 1 == BUFS ? 0 : next + 1);
+        if (active) block(buffer, i & 3, q0, 1, lds + next * 2 * kTileBytes, next_q0);
+        const bool was = active;
+        active = i + 1 < total && looked_at(next_q0);
+        if (AHEAD && active && !was) scores_of(lds + next * 2 * kTileBytes, next_q0, 0);
+        if (BUFS == 2) {
+            if (!ARRIVES) fetch(0);
             __syncthreads();
             if (ARRIVES) fetch(buffer);
-            buffer ^= 1;
-            turn = turn == 2 ? 0 : turn + 1;
         }
+        buffer = next;
     }
+    __syncthreads();
     int8_t* const own = lds + wave * D * 80;
     attn_write<NT>(a.dk, a.dk.at(b, kvh), dk, ldexpf(a.natural_scale, -exponent - (int)kProbScale), k_first, a.length, a.dim, lane, own);
     attn_write<NT>(a.dv, a.dv.at(b, kvh), dv, ldexpf(1.0f, -(int)kProbScale), k_first, a.length, a.dim, lane, own);
@@ -564,7 +612,7 @@ static int dq_launch(const AttentionGrad& a, unsigned grid, hipStream_t st) {
 template <int NT, bool BIAS, bool MASK, int LAY>
 static int dkv_launch(const AttentionGrad& a, unsigned grid, unsigned more, hipStream_t st) {
     constexpr int D = NT <= 2 ? 64 : NT <= 4 ? 128 : 256;
-    const int lds = 4 * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
+    const int lds = 2 * kGradBuffers<NT> * kAttnTile * D * 2 + (a.table ? (a.distances - a.first_distance + 2 * kBiasPad) * 4 : 0);
     static std::atomic<bool> done[64];
     if (int e = enable_dynamic_lds((const void*)k_attn_dkv<NT, BIAS, MASK, LAY>, 150 * 1024, done)) return e;
     hipLaunchKernelGGL((k_attn_dkv<NT, BIAS, MASK, LAY>), dim3(grid + more), dim3(256), lds, st, a, grid);
