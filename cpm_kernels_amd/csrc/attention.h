@@ -480,20 +480,20 @@ __device__ __forceinline__ void attn_keep_columns(half8_t (&x)[KS], const int8_t
     for (int s = 0; s < KS; ++s) x[s] = attn_rows<D>(tiles + (wave >> 1) * kAttnTile * D * 2, at, wave & 1, s);
 }
 
-// 32 bytes of a row of a mask as bits, or one byte, on their way from memory
+// 32 bytes of a row of a mask, on their way from memory, as bits.  LONG: rows of 32 at least
+template <bool LONG>
 struct AttnMaskShare {
     uint4_t raw[2];
-    uint8_t byte;
     __device__ __forceinline__ void load(const uint8_t* row, int32_t key, int32_t length) {
         struct __attribute__((packed, aligned(1))) Byte16Any { uint32_t w[4]; };
-        if (length < 32) return;
+        if (!LONG && length < 32) return;
         const uint8_t* const p = row + min(key, length - 32);
         raw[0] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(p));
         raw[1] = __builtin_bit_cast(uint4_t, *reinterpret_cast<const Byte16Any*>(p + 16));
     }
     __device__ __forceinline__ uint32_t bits(const uint8_t* row, int32_t key, int32_t length) const {
         uint32_t all = 0;
-        if (length < 32) {
+        if (!LONG && length < 32) {
 #pragma unroll 1
             for (int i = 0; key + i < length; ++i) all |= (row[key + i] != 0 ? 1u : 0u) << i;
             return all;
@@ -633,18 +633,14 @@ __device__ __forceinline__ void attn_begin(float16_tv& s, int blk, const float* 
 __device__ __forceinline__ const float* attn_window(const Attention& a, const float* biases, int32_t rel, int half) {
     return biases + max(63, min(rel - half * 4 - (a.first_distance - kBiasPad), attn_bias_entries(a) - 1));
 }
-// Scores of keys that a mask leaves out: -inf.  caps: +inf or -inf by key (the smaller of a number that is none and -inf is -inf); bits: a query's, the half's first key lowest
-__device__ __forceinline__ void attn_cap(float16_tv& s, int blk, int half, const float* caps) {
+// Scores of keys that a query's mask leaves out: -inf (whatever they are).  bits: the half's first key lowest
+__device__ __forceinline__ void attn_cap(float16_tv& s, uint32_t bits) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const float4_t x = *reinterpret_cast<const float4_t*>(caps + blk * 32 + c * 8 + half * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[c * 4 + e] = fminf(s[c * 4 + e], x[e]);
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t keep = (int32_t)(bits << (31 - ((i >> 2) * 8 + (i & 3)))) >> 31;
+        const float x = s[i];           // (a bit cast of a vector's element itself takes the first one's)
+        s[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
     }
-}
-__device__ __forceinline__ void attn_cap_each(float16_tv& s, uint32_t bits) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = bits & (1u << ((i >> 2) * 8 + (i & 3))) ? s[i] : -__builtin_inff();
 }
 
 constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};

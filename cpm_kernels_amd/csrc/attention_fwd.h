@@ -14,7 +14,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys, two of values, biases
     __shared__ uint32_t bad[3][2];              // tokens of a tile whose values are no finite numbers; those of tile t in t % 3
     __shared__ uint32_t mask_bits[2][kAttnRows][2];
-    __shared__ __attribute__((aligned(16))) float mask_caps[2][kAttnTile];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* const biases = reinterpret_cast<float*>(lds + 4 * kTileBytes);
@@ -46,9 +45,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     const int32_t every_sees = a.causal ? min(range.len, range.pos + qt * kAttnRows + 1) : range.len;
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);         // (of queries times its sign: the largest score is the largest product)
     constexpr bool BY_UNIT = kByUnit<LAY>, ARRIVES = LAY == kDirect || LAY == kTurned;
-    const bool masked = MASK && a.mask != nullptr;
+    const bool masked = MASK && (ARRIVES || a.mask != nullptr);
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
-    const bool each = masked && a.mask_token != 0;          // a row of the mask for each query, or one for all
     const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + min(qt * kAttnRows + (tid >> 1), a.tokens - 1) * a.mask_token : nullptr;
 
     // Keys, and the mask's bits, come a tile before the values: scores of the next tile are formed beside this one's sums.
@@ -56,15 +54,13 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     AttnTiles<D, LAY> ks, vs;
     ks.init(keys, a.k, a.length, a.dim, tid, wave, lane);
     vs.init(values, a.v, a.length, a.dim, tid, wave, lane);
-    AttnMaskShare ms;
+    AttnMaskShare<ARRIVES> ms;
     ushort8_t largest = {0, 0, 0, 0, 0, 0, 0, 0};
     const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a value that is no finite number must not reach the queries that do not see it)
     auto fetch = [&](int32_t t) __attribute__((always_inline)) {
-        if (t + 1 < t_end) {
-            ks.fetch(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane);
-            if (each) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
-            else if (masked && tid < kAttnTile) ms.byte = mask[min((t + 1) * kAttnTile + tid, a.length - 1)];
-        }
+        if (t + 1 < t_end) ks.fetch(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane);
+        // (without a branch: where paths meet, the compiler waits for what either loads, and for the tiles with it)
+        if (masked) ms.load(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         if (t >= t_begin && t < t_end) vs.fetch(lds + (2 + (t & 1)) * kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
     };
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
@@ -131,8 +127,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
             if (masked) {
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
-                    if (each) attn_cap_each(s[blk], mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4));
-                    else attn_cap(s[blk], blk, half, mask_caps[t & 1]);
+                    const uint32_t bits = mask_bits[t & 1][wave * 32 + col][blk];
+                    if (__builtin_amdgcn_ballot_w64(bits != ~0u)) attn_cap(s[blk], bits >> (half * 4));
                 }
             }
             float m = s[0][0];
@@ -170,8 +166,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
         if (ARRIVES) wait_vmcnt<0>();
         if (t + 1 < t_end) {
             ks.place(lds + ((t + 1) & 1) * kTileBytes, a.dim, (t + 1) * kAttnTile, range.len, tid, wave, lane, nullptr);
-            if (each) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
-            else if (masked && tid < kAttnTile) mask_caps[(t + 1) & 1][tid] = ms.byte ? __builtin_inff() : -__builtin_inff();
+            if (masked) mask_bits[(t + 1) & 1][tid >> 1][tid & 1] = ms.bits(mask, (t + 1) * kAttnTile + (tid & 1) * 32, a.length);
         }
         if (t >= t_begin) {
             int8_t* const tile = lds + (2 + (t & 1)) * kTileBytes;
@@ -255,10 +250,10 @@ template <int NT, bool BIAS, bool MASK, int LAY>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
     return a.lse ? attn_launch<NT, BIAS, MASK, LAY, true>(a, grid, st) : attn_launch<NT, BIAS, MASK, LAY, false>(a, grid, st);
 }
-// (a mask is looked for in a call's arguments where tiles come through registers: a branch a tile, 15 % of the time where they do not)
+// (a mask is looked for in a call's arguments where tiles come through registers: a branch a tile, 15 % of the time where they do not.  Of a mask the others read 32 keys at a time.)
 template <int NT, bool BIAS>
 static int attn_launch(const Attention& a, unsigned grid, hipStream_t st) {
-    const int lay = attn_layout(a.k, a.v, a.dim, a.length);
+    const int lay = a.mask && a.length < 32 ? kAnyLayout : attn_layout(a.k, a.v, a.dim, a.length);
     if (lay == kDirect) return a.mask ? attn_launch<NT, BIAS, true, kDirect>(a, grid, st) : attn_launch<NT, BIAS, false, kDirect>(a, grid, st);
     if (lay == kTurned) return a.mask ? attn_launch<NT, BIAS, true, kTurned>(a, grid, st) : attn_launch<NT, BIAS, false, kTurned>(a, grid, st);
     return lay == kColumns ? attn_launch<NT, BIAS, true, kColumns>(a, grid, st) : attn_launch<NT, BIAS, true, kAnyLayout>(a, grid, st);

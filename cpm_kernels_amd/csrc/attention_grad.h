@@ -44,7 +44,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];        // two buffers of keys and values; biases; sums of ds by distance, of each wave
     __shared__ uint32_t bad[3][2];              // tokens of a tile whose keys (and, masked, values) are no finite numbers; those of tile t in t % 3
     __shared__ uint32_t mask_bits[2][kGradRows][2];
-    __shared__ __attribute__((aligned(16))) float mask_caps[2][kAttnTile];
     __shared__ float tops[4];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -67,8 +66,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     const int32_t keys_seen = a.causal ? max(0, min(range.len, range.pos + q_last_of_all + 1)) : range.len;
     const int32_t tiles = (keys_seen + kAttnTile - 1) / kAttnTile;
     constexpr bool BY_UNIT = kByUnit<LAY>, ARRIVES = LAY == kDirect || LAY == kTurned;
-    const bool masked = MASK && a.mask != nullptr, table_wanted = BIAS && a.table_parts != nullptr;
-    const bool each = masked && a.mask_token != 0;          // a row of the mask for each query, or one for all
+    const bool masked = MASK && (ARRIVES || a.mask != nullptr), table_wanted = BIAS && a.table_parts != nullptr;
     const float scale = a.scale == 0.0f ? 1.0f : a.scale;
     const uint8_t* const mask = masked ? a.mask + b * a.mask_batch + min(qt * kGradRows + (tid >> 1), a.tokens - 1) * a.mask_token : nullptr;
     const half_t *const keys = a.k.at(b, kvh), *const values = a.v.at(b, kvh);
@@ -77,15 +75,14 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
     AttnTiles<D, LAY> ks, vs;
     ks.init(keys, a.k, a.length, a.dim, tid, wave, lane);
     vs.init(values, a.v, a.length, a.dim, tid, wave, lane);
-    AttnMaskShare ms;
+    AttnMaskShare<ARRIVES> ms;
     const auto guarded = [&](int32_t t) { return masked || (t + 1) * kAttnTile > every_sees; };       // (a key that is no finite number must not reach the queries that do not see it)
     auto fetch = [&](int32_t t) __attribute__((always_inline)) {
+        if (masked) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
         if (t >= tiles) return;
         int8_t* const buffer = lds + (t & 1) * 2 * kTileBytes;
         ks.fetch(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane);
         vs.fetch(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane);
-        if (each) ms.load(mask, t * kAttnTile + (tid & 1) * 32, a.length);
-        else if (masked && tid < kAttnTile) ms.byte = mask[min(t * kAttnTile + tid, a.length - 1)];
     };
     auto place = [&](int32_t t) __attribute__((always_inline)) {
         if (t >= tiles) return;
@@ -93,8 +90,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         if (ARRIVES) wait_vmcnt<0>();
         ks.place(buffer, a.dim, t * kAttnTile, range.len, tid, wave, lane, guarded(t) ? bad[(uint32_t)t % 3] : nullptr);
         vs.place(buffer + kTileBytes, a.dim, t * kAttnTile, range.len, tid, wave, lane, masked ? bad[(uint32_t)t % 3] : nullptr);        // (0 times no number is none)
-        if (each) mask_bits[t & 1][tid >> 1][tid & 1] = ms.bits(mask, t * kAttnTile + (tid & 1) * 32, a.length);
-        else if (masked && tid < kAttnTile) mask_caps[t & 1][tid] = ms.byte ? __builtin_inff() : -__builtin_inff();
+        if (masked) mask_bits[t & 1][tid >> 1][tid & 1] = ms.bits(mask, t * kAttnTile + (tid & 1) * 32, a.length);
         if (tid < 2) bad[(uint32_t)(t + 1) % 3][tid] = 0;
     };
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
@@ -217,8 +213,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], scale, minus_lse);
         if (masked) {
-            if (each) attn_cap_each(s, mask_bits[t & 1][wave * 32 + col][blk] >> (half * 4));
-            else attn_cap(s, blk, half, mask_caps[t & 1]);
+            const uint32_t bits = mask_bits[t & 1][wave * 32 + col][blk];
+            if (__builtin_amdgcn_ballot_w64(bits != ~0u)) attn_cap(s, bits >> (half * 4));
         }
         const uint32_t spoilt = bad[(uint32_t)t % 3][blk];
         if (k0 + 32 > all_see || spoilt) {
@@ -358,6 +354,8 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     const int32_t k_first_of_all = kt * kGradRows, k_first = k_first_of_all + wave * 32, key = k_first + col;
     constexpr bool BY_UNIT = kByUnit<LAY>, ARRIVES = LAY == kDirect || LAY == kTurned;
     const bool masked = MASK && a.mask != nullptr && a.mask_token != 0;         // (by a row for each query)
+    constexpr bool kMaskAlways = MASK && ARRIVES;          // read, without a branch
+    const uint8_t* const mask = kMaskAlways || masked ? a.mask + b * a.mask_batch : nullptr;
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);         // (of keys times its sign: a score of -inf stays one)
     // tiles of queries that see any key of the workgroup
     const int32_t first_query = a.causal ? max(0, k_first_of_all - range.pos) : 0;
@@ -400,25 +398,23 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
     AttnTiles<D, LAY> qs, gs;
     qs.init(a.q.at(b, kvh * a.group), a.q, a.tokens, a.dim, tid, wave, lane);
     gs.init(a.dout.at(b, kvh * a.group), a.dout, a.tokens, a.dim, tid, wave, lane);
-    AttnMaskShare ms;
+    AttnMaskShare<ARRIVES> ms;
     float lse = 0.0f, delta = 0.0f;
     int32_t h_fetch = kvh * a.group, t_fetch = 0, t_place = 0;       // head and tile of the head to be fetched next, the tile to be placed next
     int32_t left = of_head * a.group;           // tiles still to be fetched
     uint32_t phase_place = 0;           // of `bad`
     const auto guarded = [&](int32_t q0) { return masked || q0 + kAttnTile > a.tokens || some_out || (a.causal && range.pos + q0 < min(k_first_of_all + kGradRows, range.len) - 1); };
     auto fetch = [&](int buffer) __attribute__((always_inline)) {
-        if (left == 0) return;
         const int32_t q0 = (first_tile + t_fetch) * kAttnTile;
+        if (kMaskAlways || masked) ms.load(mask + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
+        if (left == 0) return;
         int8_t* const at = lds + buffer * 2 * kTileBytes;
         qs.fetch(at, a.dim, q0, a.tokens, tid, wave, lane);
         gs.fetch(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane);
-        if (masked) ms.load(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
-        if (tid < 128) {
-            // (as they are: to look at them here would be to wait for the tile)
-            const int64_t row = (b * a.heads + h_fetch) * a.tokens + min(q0 + (tid & 63), a.tokens - 1);
-            lse = a.lse[row];
-            delta = a.delta[row];
-        }
+        // (as they are, and without a branch: to look at them here would be to wait for the tile)
+        const int64_t row = (b * a.heads + h_fetch) * a.tokens + min(q0 + (tid & 63), a.tokens - 1);
+        lse = a.lse[row];
+        delta = a.delta[row];
         if (++t_fetch == of_head) {
             t_fetch = 0, ++h_fetch;
             qs.advance(a.q.head);
@@ -433,7 +429,7 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         if (ARRIVES) wait_vmcnt<0>();
         qs.place(at, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
         gs.place(at + kTileBytes, a.dim, q0, a.tokens, tid, wave, lane, spoilt);
-        if (masked) mask_bits[buffer][tid & 3][tid >> 2] = ms.bits(a.mask + b * a.mask_batch + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
+        if (masked) mask_bits[buffer][tid & 3][tid >> 2] = ms.bits(mask + min(q0 + (tid >> 2), a.tokens - 1) * a.mask_token, k_first_of_all + (tid & 3) * 32, a.length);
         if (tid < 128) {
             // (a query whose statistics are no numbers, like one that is none itself, must not reach the keys that it does not see)
             const float none = tid < 64 ? -__builtin_inff() : 0.0f;
@@ -622,7 +618,7 @@ static int dkv_launch(const AttentionGrad& a, unsigned grid, unsigned more, hipS
 template <int NT, bool BIAS>
 static int grad_launch(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_grid, hipStream_t st) {
     if (dq_grid) {
-        const int lay = attn_layout(a.k, a.v, a.dim, a.length);
+        const int lay = a.mask && a.length < 32 ? kAnyLayout : attn_layout(a.k, a.v, a.dim, a.length);
         const int e = lay == kDirect    ? a.mask ? dq_launch<NT, BIAS, true, kDirect>(a, dq_grid, st) : dq_launch<NT, BIAS, false, kDirect>(a, dq_grid, st)
                       : lay == kTurned  ? a.mask ? dq_launch<NT, BIAS, true, kTurned>(a, dq_grid, st) : dq_launch<NT, BIAS, false, kTurned>(a, dq_grid, st)
                       : lay == kColumns ? dq_launch<NT, BIAS, true, kColumns>(a, dq_grid, st)
@@ -631,7 +627,7 @@ static int grad_launch(const AttentionGrad& a, unsigned dq_grid, unsigned dkv_gr
     }
     const unsigned more = a.dtable ? a.heads : 0;
     if (dkv_grid + more == 0) return 0;
-    const int lay = attn_layout(a.q, a.dout, a.dim, a.tokens);
+    const int lay = a.mask && a.length < 32 ? kAnyLayout : attn_layout(a.q, a.dout, a.dim, a.tokens);
     return lay == kDirect    ? a.mask ? dkv_launch<NT, BIAS, true, kDirect>(a, dkv_grid, more, st) : dkv_launch<NT, BIAS, false, kDirect>(a, dkv_grid, more, st)
            : lay == kTurned  ? a.mask ? dkv_launch<NT, BIAS, true, kTurned>(a, dkv_grid, more, st) : dkv_launch<NT, BIAS, false, kTurned>(a, dkv_grid, more, st)
            : lay == kColumns ? dkv_launch<NT, BIAS, true, kColumns>(a, dkv_grid, more, st)
