@@ -530,15 +530,6 @@ __device__ __forceinline__ void attn_keep(half8_t (&x)[KS], const AttnTensor& t,
     for (int s = 0; s < KS; ++s) x[s] = half8_fill(x[s], half8_keep(dim - s * 16 - half * 8), half8_t{0, 0, 0, 0, 0, 0, 0, 0});
 }
 
-// Four mask bytes of keys key .. key + 3 (bytes past the row's end: 0)
-__device__ __forceinline__ uint32_t attn_mask4(const uint8_t* row, int32_t key, int32_t length) {
-    if (key + 4 <= length) return reinterpret_cast<const Byte4Any*>(row + key)->x;
-    uint32_t m = 0;
-    for (int e = 0; e < 4; ++e)
-        if (key + e < length) m |= (uint32_t)row[key + e] << (8 * e);
-    return m;
-}
-
 constexpr float kRest = 2048.0f;        // fp16 has 11 bits: what a rounding leaves, times this, is as large as the number at most
 
 // A wave's results, transposed (units n * 32 + 8 c + 4 half + {0..3} in registers 4 c .., a token a lane), times the lane's f, as fp16 to the tokens first .. first + 31 below `tokens`; or,

@@ -124,7 +124,7 @@ int cpmk_attention_forward(int32_t batch, int32_t heads, int32_t kv_heads, int32
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty || tokens == 0) return 0;
     if (lse && !rest) return CPMK_EBADARG;
-    const AttnPlan plan = attn_plan(batch, heads, kv_heads, tokens, dim, length, k_unit == 1 && v_unit == 1, lse != nullptr);
+    const AttnPlan plan = attn_plan(batch, heads, kv_heads, tokens, dim, length, k_unit == 1 && v_unit == 1 && !(mask && length < 4), lse != nullptr);          // (of masks k_attn_few reads four bytes at a time)
     a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.parts = (float*)workspace;
     if (a.splits > 1 && !workspace) return CPMK_EBADARG;
     const int64_t grid = (int64_t)batch * heads * a.row_tiles * a.splits, rows = (int64_t)batch * heads * tokens;

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 8 || DS * CT <= 4 ? 2 : 1) voi
         const int32_t r = min(r_first + ct * 16 + c, of_head - 1), query = r / a.group, h = kvh * a.group + r - query * a.group;
         where[ct] = range.pos + query;
         limit[ct] = a.causal ? min(range.len, where[ct] + 1) : range.len;
-        mask[ct] = masked ? a.mask + b * a.mask_batch + query * a.mask_token : nullptr;
+        mask[ct] = masked ? a.mask + b * a.mask_batch + query * a.mask_token : reinterpret_cast<const uint8_t*>(a.k.at(b, kvh));
         in_table[ct] = (a.group <= ROWS ? h - kvh * a.group : ct * 16 + c) * (a.distances - a.first_distance) - a.first_distance;
         const half_t* const p = a.q.at(b, h) + query * a.q.token;
         if (a.q.unit == 1) {
@@ -102,8 +102,19 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 8 || DS * CT <= 4 ? 2 : 1) voi
             }
         }
     };
+    // Four keys' bytes of a mask, on their way with the tile, before it (what is asked for later comes later), and without a branch: without a mask some bytes of the keys
+    uint32_t seen[PLAIN ? 1 : CT][2];
+    const auto mask_at = [&](int32_t t, int kb) { return min(t * kFewTile + kb * 16 + quad * 4, a.length - 4); };
+    auto load_masks = [&](int32_t t) {
+        if constexpr (!PLAIN)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) seen[ct][kb] = reinterpret_cast<const Byte4Any*>(mask[ct] + (masked ? mask_at(t, kb) : 0))->x;
+    };
     const int32_t mine = t_begin + wave;
     if (mine < t_end) {
+        load_masks(mine);
         load_keys(mine);
         load_values(mine);
     }
@@ -148,6 +159,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 8 || DS * CT <= 4 ? 2 : 1) voi
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) s[ct][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kb][u], q[ct][u], s[ct][kb], 0, 0, 0);
         const int32_t next = min(t + WAVES, t_end - 1);
+        uint32_t keep[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int32_t over = k0 + kb * 16 + quad * 4 - mask_at(t, kb);
+                keep[ct][kb] = !masked ? 0x01010101u : over < 4 ? seen[PLAIN ? 0 : ct][kb] >> (8 * over) : 0u;
+            }
+        load_masks(next);
         load_keys(next);
         // values of the eight keys, turned: x[n] are units UL c + n of the block
         half8_t x[NB];
@@ -184,14 +204,12 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 8 || DS * CT <= 4 ? 2 : 1) voi
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
                     const int32_t key = k0 + kb * 16 + quad * 4;
-                    uint32_t keep = 0x01010101u;
-                    if (masked) keep = attn_mask4(mask[ct], key, a.length);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float y = s[ct][kb][i] * scale;
                         if (biased) y = __builtin_fmaf((float)biases[in_table[ct] + max(a.first_distance, min(where[ct] - key - i, a.distances - 1))], kLog2e, y);
                         if (spoilt >> (kb * 4 + i) & 1) y = __builtin_nanf("");
-                        s[ct][kb][i] = key + i < limit[ct] && (keep >> (8 * i) & 0xffu) ? y : -__builtin_inff();
+                        s[ct][kb][i] = key + i < limit[ct] && (keep[ct][kb] >> (8 * i) & 0xffu) ? y : -__builtin_inff();
                     }
                 }
             }
@@ -299,16 +317,17 @@ static int few_launch(const Attention& a, int waves, unsigned grid, hipStream_t 
 }
 
 // How rows and keys of few rows are divided: workgroups of eight waves where there are fewer than two to a compute unit and their registers allow it, of four elsewhere; parts as long
-// as all run at once.
+// as all run at once (five queries of four heads each, dim 128: one workgroup to a compute unit by its registers, 44 us in two rounds, 36 in one).
 AttnPlan attn_few_plan(int64_t batch, int64_t held, int64_t of_head, int32_t dim, int64_t length) {
     AttnPlan p;
     p.rows = of_head > 16 ? 32 : 16;
     p.row_tiles = (int)ceil_div(of_head, p.rows);
     const int64_t base = batch * held * p.row_tiles, tiles = ceil_div(length, kFewTile), units = compute_units();
-    p.waves = base < 2 * units && (dim <= 64 || (dim <= 128 && p.rows == 16)) ? 8 : 4;
+    const bool light = dim <= 64 || (dim <= 128 && p.rows == 16);         // two waves to a SIMD
+    p.waves = base < 2 * units && light ? 8 : 4;
     p.tile = kFewTile;
     p.least = p.waves;
-    p.splits = (int)std::max<int64_t>(1, std::min(8 / p.waves * units / base, tiles / p.waves));
+    p.splits = (int)std::max<int64_t>(1, std::min((light ? 8 / p.waves : 1) * units / base, tiles / p.waves));
     return p;
 }
 
