@@ -19,7 +19,7 @@ struct Attention {
     const uint8_t* mask;
     int64_t mask_batch, mask_token;
     float* lse;                     // (batch, heads, tokens): log2 of the sum of exp2(score), +inf of a query without keys; behind them (batch, held, parts): the largest magnitude
-                                    // of a part's values that any query sees; or null
+                                    // of a part's finite values, masked or not, up to the last key of any query; or null
     int64_t rows_in_all;
     half_t* rest;                   // with lse: what the rounding of `out` left, times 2^11, under the same strides
     float* parts;
@@ -167,6 +167,12 @@ __device__ __forceinline__ half8_t attn_units(const int8_t* tile, uint32_t at, i
     return attn_join(attn_read_turning(p + (at ^ (x << 4))), attn_read_turning(p + 8 * D * 2 + (at ^ ((x ^ 2) << 4))));
 }
 
+// Magnitudes, as bits, of finite numbers (the others make their queries' results no numbers whatever the gradients' factor is)
+__device__ __forceinline__ ushort8_t attn_larger(ushort8_t m, half8_t v) {
+    const ushort8_t b = __builtin_bit_cast(ushort8_t, v) & (uint16_t)0x7fff;
+    return __builtin_elementwise_max(m, b & (ushort8_t)(b < (uint16_t)0x7c00));
+}
+
 // A thread's share of a tile on its way from memory to LDS through registers.  kColumns: eight tokens of PIECES neighbouring units, turned there.  Else pieces of eight units, unit by unit
 // where they are not neighbours.  Tokens past the last one and units past the head's are zeros.
 template <int D, int LAY, int THREADS>
@@ -261,7 +267,7 @@ struct AttnShare {
     }
     __device__ __forceinline__ ushort8_t largest(ushort8_t m) const {        // of the magnitudes, as bits
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, r[i]);
+        for (int i = 0; i < PIECES; ++i) m = attn_larger(m, r[i]);
         return m;
     }
     typedef half_t run_t __attribute__((ext_vector_type(PIECES)));
@@ -319,7 +325,7 @@ struct AttnDirect {
     }
     static __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t* lds, int wave, int lane) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, *reinterpret_cast<const half8_t*>(lds + wave * 16 * D * 2 + i * 1024 + lane * 16));
+        for (int i = 0; i < PIECES; ++i) m = attn_larger(m, *reinterpret_cast<const half8_t*>(lds + wave * 16 * D * 2 + i * 1024 + lane * 16));
         return m;
     }
 };
@@ -399,7 +405,7 @@ struct AttnTiles<D, kColumns> {
     }
     __device__ __forceinline__ ushort8_t largest(ushort8_t m, const int8_t*, int32_t, int, int) const {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) m = absbits_max(m, r[i]);
+        for (int i = 0; i < PIECES; ++i) m = attn_larger(m, r[i]);
         return m;
     }
 };
@@ -442,7 +448,7 @@ struct AttnTiles<D, kTurned> {
         for (int i = 0; i < PIECES; ++i) {
             const int c = (lane & 7) ^ attn_turned(wave * (D / 4) + i * 8 + (lane >> 3));
             const half8_t x = *reinterpret_cast<const half8_t*>(lds + wave * (D / 4) * 128 + i * 1024 + lane * 16);
-            m = absbits_max(m, count < kAttnTile ? half8_fill(x, half8_keep(count - c * 8), none) : x);
+            m = attn_larger(m, count < kAttnTile ? half8_fill(x, half8_keep(count - c * 8), none) : x);
         }
         return m;
     }

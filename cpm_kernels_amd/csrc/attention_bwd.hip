@@ -53,6 +53,7 @@ int cpmk_attention_backward(int32_t batch, int32_t heads, int32_t kv_heads, int3
     bool empty;
     if (int e = attn_check(a, batch, heads, kv_heads, bidirectional, empty)) return e;
     if (empty) return 0;
+    if (tokens == 0) a.mask = nullptr;          // (it has no rows to read)
     if ((tokens > 0 && any_null(lse, rest, dout, dq)) || (length > 0 && any_null(dk, dv)) || !workspace || (dbias && !bias)) return CPMK_EBADARG;
     a.row_tiles = (int32_t)ceil_div(tokens, kGradRows), a.query_tiles = (int32_t)ceil_div(tokens, kAttnTile);
     a.splits = tokens > 0 ? attn_plan(batch, heads, kv_heads, tokens, dim, length, false, true).splits : 0;        // (the forward pass's: where it has left the values' magnitudes)

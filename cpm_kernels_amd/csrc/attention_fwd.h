@@ -198,8 +198,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn(Attention a) {
     sum += __shfl_xor(sum, 32);
     __syncthreads();            // (the tiles are done with)
     if (looks) {
-        // (numbers that are none or infinite count as the largest one: the keys past the end among them are zeros or copies)
-        const uint32_t m = wave_max_u32(min(absbits_max_of(largest), 0x7bffu));
+        const uint32_t m = wave_max_u32(absbits_max_of(largest));
         if (lane == 0) bad[0][0] = 0;
         __syncthreads();
         if (lane == 0) atomicMax(&bad[0][0], m);

@@ -164,14 +164,18 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void k_attn_dq(AttentionGrad 
         square += __shfl_xor(square, 32);
         delta += __shfl_xor(delta, 32);
         if (real && half == 0) a.delta[row] = delta;
-        const float largest = wave_max(real ? square : 0.0f);
-        if (lane == 0) tops[wave] = largest;
         const int exponent = attn_exponent(square, attn_value_norm(a, b, kvh, lane));
         dscale = ldexpf(1.0f, exponent);
         undo = ldexpf(1.0f, -exponent - (int)kProbScale);
         const float lse = real ? a.lse[row] : __builtin_inff();
+        // (of queries that see a key, with gradients that are numbers: the others' are none, or make their keys' none, whatever the factor is)
+        const float largest = wave_max(lse != __builtin_inff() && square < __builtin_inff() ? square : 0.0f);
+        if (lane == 0) tops[wave] = largest;
         minus_lse = kProbScale - lse;
         minus_delta = lse == __builtin_inff() ? 0.0f : -delta * dscale;
+        if (lse == __builtin_inff())            // (a query without keys: its result's gradients count for nothing, numbers or none)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) g[s] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
     if (a.scale == 0.0f)
 #pragma unroll
@@ -565,12 +569,11 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         const int32_t q0 = (first_tile + t) * kAttnTile;
         if (active) block(buffer, i & 3, q0, 0, lds + buffer * 2 * kTileBytes, q0);
         const int next = buffer + 1 == BUFS ? 0 : buffer + 1;
-        if (++t == of_head) {
-            t = 0, ++g;
-            if (BIAS && i + 1 < total) {
-                __syncthreads();
-                attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
-            }
+        if (++t == of_head) t = 0, ++g;
+        const bool other_head = BIAS && t == 0 && i + 1 < total;
+        if (AHEAD && other_head) {
+            __syncthreads();
+            attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
         }
         // (with three buffers the one that is fetched into was last read before this barrier; scores behind the last tile are of what the buffer held, and nobody looks at them)
         const int32_t next_q0 = (first_tile + t) * kAttnTile;
@@ -585,6 +588,10 @@ __global__ __launch_bounds__(256, NT <= 2 ? 2 : 1) void k_attn_dkv(AttentionGrad
         if (BUFS == 2) {
             if (!ARRIVES) fetch(0);
             __syncthreads();
+            if (!AHEAD && other_head) {
+                attn_biases(a, kvh * a.group + g, scale, biases, tid, 256);
+                __syncthreads();
+            }
             if (ARRIVES) fetch(buffer);
         }
         buffer = next;

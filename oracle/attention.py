@@ -32,7 +32,7 @@ def attention(q, k, v, lens, first, scale, causal, mask=None, table=None, mappin
     Without dout (out, bound); with it lists of (out, dq, dk, dv[, dtable]) and of their bounds.
 
     Roundings: scores are fp32 sums of dim products; exponents and exponentials fp32; probabilities and the scores' gradients rounded to fp16, the first beside a power of two that makes
-    their row's largest 2^7 at least, the second beside one that brings 2 |dout| max |v| to 2^15; sums fp32; results fp16, D from what their rounding left too."""
+    their row's largest 2^7 at least, the second beside one that brings 2 |dout| sqrt(dim) max |v| to 2^15; sums fp32; results fp16, D from what their rounding left too."""
     q, k, v = (np.asarray(x, f64) for x in (q, k, v))
     batch, heads, n, dim = q.shape
     length, group = k.shape[2], heads // max(k.shape[1], 1)
@@ -83,8 +83,11 @@ def attention(q, k, v, lens, first, scale, causal, mask=None, table=None, mappin
             e_D = (np.abs(G) * bD).sum(1, keepdims=True) + (np.abs(G) * np.abs(o)).sum(1, keepdims=True) * (dim + 8) * E32
             e_ds = np.where(seen, e_p * np.abs(dp - D) + p * (e_dp + e_D), 0)
             norms = np.sqrt((G ** 2).sum(1, keepdims=True))
-            vtop = np.sqrt((v[b, h // group] ** 2).sum(1)).max(initial=0) if np.isfinite(v[b, h // group]).all() else np.sqrt((Vs ** 2).sum(1)).max(initial=0)
-            own = np.where(seen, 4 * norms * vtop * 2.0 ** -40, 0)         # half a step of the smallest numbers, undone
+            # ds is taken times 2^e, with 2 |do| sqrt(dim) max |v| 2^e in [1/2, 1], over the finite values of the sequence's keys, masked or not (|v| <= sqrt(dim) max |v|), and p
+            # times 2^15: half a step of the smallest fp16 numbers, 2^-25, is 2^-25 2^-15 2^-e <= 2^-40 4 |do| sqrt(dim) max |v| of ds
+            finite = np.abs(v[b, h // group, :keys])
+            vtop = math.sqrt(dim) * np.where(np.isfinite(finite), finite, 0).max(initial=0)
+            own = np.where(seen, 4 * norms * vtop * 2.0 ** -40, 0)
             gtop = np.sqrt((dout[b, h // group * group:(h // group + 1) * group] ** 2).sum(-1)).max(initial=0)
             all_ = np.where(seen, 4 * gtop * vtop * 2.0 ** -40, 0)
             c = abs(scale)
