@@ -642,7 +642,8 @@ __device__ __forceinline__ void attn_cap(float16_tv& s, uint32_t bits) {
 
 constexpr float16_tv kZero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-// The layout by which tiles of two tensors are brought
+// The layout by which tiles of two tensors are brought: straight into LDS where every piece of 16 bytes is on its boundary, through registers elsewhere (columns, gradients of 64 heads of 64
+// units, 4 x 1024 tokens and 4 x 1025: 340 and 650 us; 32 of 128: 360 and 610)
 inline bool attn_direct(const AttnTensor& x, int32_t dim) {
     return x.unit == 1 && dim % 8 == 0 && aligned16(x.p) && x.batch % 8 == 0 && x.head % 8 == 0 && x.token % 8 == 0 && x.token >= 0 && x.token < (1 << 23);        // (64 tokens: offsets of 32 bits)
 }

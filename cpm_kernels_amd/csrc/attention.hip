@@ -9,7 +9,13 @@
 // keys of one query, and its probabilities, rounded to fp16, are the second product's operand as they are.  fp16 keeps their bits: they are at most 2^15 and their maximum is 2^7 at least
 // (the running maximum follows the true one at a distance of up to 2^8), so what falls below fp16's normal range is less than 2^-21 of the row's largest.  Sums are fp32, of the
 // unrounded probabilities.  For training (TRAIN) what their rounding leaves is multiplied by the values as well, and what the result's rounding leaves is kept: the
-// backward pass subtracts two nearly equal numbers where a query looks at one key, do_i v_j and do_i out_i, and the second has to be as exact as the first.  Where there are few rows the keys are cut into parts, which k_attn_join adds up.
+// backward pass subtracts two nearly equal numbers where a query looks at one key, do_i v_j and do_i out_i, and the second has to be as exact as the first.  Where there are few rows the
+// keys are cut into parts, which k_attn_join adds up.
+//
+// Bound by products and exponentials together: a score costs an exponential and about five vector operations beside 4 dim operations of products, so heads of 128 units come nearer to what
+// the matrix cores give than those of 64.  128 queries, so that a tile is read from memory once for all of them; tiles of 64 keys, so that two workgroups fit a compute unit and one's
+// products run beside the other's exponentials.  Measured: 2000 queries of 32 heads, 8 of keys, dim 128, 8011 keys, causal: 275 us, 0.84 PFLOP/s; 8 x 64 heads of 64, 512 tokens, biases and a
+// mask of keys: 100 us, 0.34; 64 keys more for 8 x 32 heads of 512 queries, dim 128: 4.5 us, 0.96.
 #include <algorithm>
 #include "attention_fwd.h"
 
@@ -72,10 +78,15 @@ __global__ __launch_bounds__(256) void k_attn_join(Attention a, AttnPlan plan, u
     if (a.lse && lane == 0) a.lse[(b * a.heads + h) * a.tokens + query] = total == 0.0f ? __builtin_inff() : base - kLift + __builtin_amdgcn_logf(total);
 }
 
-// Which kernel a call takes, and how it is divided.  Keys are cut into as many parts as let the device's compute units each have a workgroup, of four tiles at least.
+// Which kernel a call takes, and how it is divided.  k_attn_few, where units are neighbours, up to 32 rows of a head of keys (8 x 32 heads on 8 of 128, 4096 keys, 4 to 32 rows: 29 to 33 us
+// and k_attn 53 to 55; 32 x 16 heads of 64, 1024 keys, one head a head of keys: 23 to 26 and 23 to 24), and where four heads or more share one, up to 192 rows of up to 32 queries: k_attn goes
+// over the keys once for each head, with 128 rows for a handful (8 x 32 heads on 8 of 64, 4096 keys, 36, 64, 128 rows: 25, 26, 30 us and 45, 45, 49; 2 x 32 on 4 of 128, 16384 keys, 192 and
+// 256 rows: 43, 55 and 55, 56; two heads that share: 48 and 64 rows 18, 19 and 18, 19; of 256 units 64 rows 31 and 25).  Elsewhere keys are cut into as many parts as let the device's
+// compute units each have two workgroups, of four tiles at least.
 AttnPlan attn_plan(int64_t batch, int64_t heads, int64_t held, int64_t tokens, int32_t dim, int64_t length, bool rows_of_keys, bool train) {
     const int64_t of_head = tokens * (heads / held);
-    if (rows_of_keys && !train && of_head <= 32 && dim % 8 == 0 && length > 0) {
+    const bool shared = heads >= 4 * held && tokens <= 32 && of_head <= 192 && dim <= 128;
+    if (rows_of_keys && !train && (of_head <= 32 || shared) && dim % 8 == 0 && length > 0) {
         AttnPlan p = attn_few_plan(batch, held, of_head, dim, length);
         p.few = true;
         return p;

@@ -1,4 +1,7 @@
 // k_attn of attention.hip (the mathematics: there), compiled for each size of heads by itself.
+//
+// Loop: the values' sums of tile t and the scores of tile t + 1 are issued as one run of products, their operands read eight ahead of them; then the softmax of t + 1.  Keys and masks are
+// fetched a tile before the values, each while the tile before it is worked on.
 #pragma once
 #include "attention.h"
 

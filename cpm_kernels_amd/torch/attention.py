@@ -26,6 +26,13 @@ def _workspace(device, *sizes):         # (how keys are divided depends on the d
     return cpmk.attention_forward_workspace(*sizes)
 
 
+_backward_workspace = lru_cache(maxsize=1024)(cpmk.attention_backward_workspace)
+
+
+def _seen(mask):
+    return mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0
+
+
 def _forward(q, k, v, table, seen, rows, sizes, keep):
     """(result, what the backward pass needs besides it)"""
     out = torch.empty_like(q)
@@ -53,8 +60,16 @@ class OpAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         assert not torch.is_grad_enabled(), "the gradients have no gradients"       # (create_graph; a wrapper that refuses it costs 10 us)
-        q, k, v, bias, mapping, _, out, lse, rest, _, _ = ctx.saved_tensors
+        q, k, v, bias, mapping, mask, out, lse, rest, lens, pos = ctx.saved_tensors
         sizes, rows, table, seen = ctx.plain
+        # (addresses again: what was saved may have been packed and unpacked meanwhile)
+        rows = (None if lens is None else lens.data_ptr(), rows[1], None if pos is None else pos.data_ptr(), *rows[3:])
+        if bias is not None:
+            table = (bias.data_ptr(), mapping.data_ptr(), *table[2:])
+        if mask is not None:
+            assert mask.stride(2) == 1 or mask.size(2) <= 1
+            seen = _seen(mask)
+        assert rest.stride() == out.stride()
         batch, heads, kv_heads, tokens, dim, length = sizes
         current_device(q.device)
         assert dout.dtype == torch.float16
@@ -62,7 +77,7 @@ class OpAttention(torch.autograd.Function):
         dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
         if batch * heads * dim == 0:
             return (dq, dk, dv, None if dbias is None else dbias.zero_()) + (None,) * 8
-        size = cpmk.attention_backward_workspace(batch, heads, kv_heads, tokens, length, 0 if dbias is None else mapping.size(0), table[4])
+        size = _backward_workspace(batch, heads, kv_heads, tokens, length, 0 if dbias is None else mapping.size(0), table[4])
         space = torch.empty(max(size, 4), dtype=torch.uint8, device=q.device)
         cpmk.attention_backward(*sizes, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), *rows, *table, *seen, out.data_ptr(), *out.stride(),
                                 lse.data_ptr(), rest.data_ptr(), dout.data_ptr(), *dout.stride(), dq.data_ptr(), *dq.stride(), dk.data_ptr(), *dk.stride(), dv.data_ptr(), *dv.stride(),
@@ -101,7 +116,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens=None, scal
             mask = mask[:, None]
         assert mask.ndim == 3 and mask.shape[::2] == (batch, length) and mask.size(1) in (1, queries)
         assert mask.stride(2) == 1 or length <= 1
-        seen = (mask.data_ptr(), mask.stride(0), mask.stride(1) if mask.size(1) > 1 else 0)
+        seen = _seen(mask)
     if bias is not None:
         assert bias.dtype == torch.float16 and bias.ndim == 2 and bias.size(0) == heads and bias.size(1) > 0 and bias.is_contiguous() and bias.device == device
         assert mapping is not None and mapping.dtype == torch.int32 and mapping.ndim == 1 and mapping.is_contiguous() and mapping.device == device

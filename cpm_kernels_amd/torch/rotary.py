@@ -10,6 +10,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 from ..library import cpmk
 from ._common import cur_stream, current_device
 
@@ -127,7 +128,11 @@ class RotaryEmbedding(torch.nn.Module):
         for x in (q, k):
             assert x is None or not x.requires_grad, "in place there are no gradients"
             assert x is None or all(s != 0 or n <= 1 for s, n in zip(x.stride(), x.shape)), "elements that share memory"
+        assert k is None or k.numel() == 0 or k.data_ptr() != q.data_ptr(), "one tensor turned twice at once"
         _launch(self, (q, k), (q, k), pos, False)
+        for x in (q, k):
+            if x is not None and not x.is_inference():
+                increment_version(x)        # (a backward pass that has kept it must not run on what it has become)
 
 
 class RotaryEmbeddingTH(torch.nn.Module):

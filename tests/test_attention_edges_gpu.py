@@ -349,6 +349,14 @@ def test_long_keys(gpu, n, h, held, d, layout):
     _Case(2, h, held, n, 3000, d, layout=layout, lens=[3000, 70], pos=None, seed=19).check(True)
 
 
+@pytest.mark.parametrize("n,h,held,d", [(9, 8, 2, 64), (32, 12, 2, 128), (1, 100, 1, 64), (5, 40, 1, 96), (32, 8, 2, 40), (33, 8, 2, 64), (48, 4, 1, 128), (2, 130, 1, 64)])
+@pytest.mark.parametrize("bias,mask", [(None, None), ("both", "query"), ("one", "key")])
+def test_rows_of_many_heads(gpu, n, h, held, d, bias, mask):
+    """Heads that share keys, from a few rows to more than the kernel of few rows takes."""
+    print("many heads", n, h, held, d, bias, mask, flush=True)
+    _Case(2, h, held, n, 700, d, causal=bias != "both", bias=bias, mask=mask, lens=[700, 131], pos=None if mask else [660, 100], seed=30).check(False)
+
+
 # ---- order, streams, graphs ----
 
 def test_the_same_bits_again(gpu):
@@ -437,6 +445,29 @@ def test_a_captured_training_step(gpu):
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_saved_tensors_that_move(gpu):
+    """What the backward pass needs, packed to host memory and unpacked elsewhere, or computed again: the same gradients."""
+    print("saved tensors", flush=True)
+    from torch.utils.checkpoint import checkpoint
+    for layout in ("rows", "columns"):
+        case = _Case(2, 4, 2, 70, 150, 64, layout=layout, bias="both", causal=False, mask="query", lens=[150, 99], pos=[80, 3], seed=29)
+        want = case.run(True)
+        q, k, v, g = case.tensors()
+        table = torch.from_numpy(case.table).cuda()
+        leaves = [x.requires_grad_() for x in (q, k, v, table)]
+        with torch.autograd.graph.save_on_cpu():
+            out = ct.attention(q, k, v, bias=table, **case.arguments())
+        spoil = [torch.full((2, 70, 150), 77, dtype=torch.uint8, device="cuda") for _ in range(8)]         # (where the mask was, perhaps)
+        got = [out, *torch.autograd.grad(out, leaves, g)]
+        assert len(spoil) == 8
+        for name, x, y, e in zip(NAMES, got, *case.oracle(True)):           # (unpacked they are rows: products of columns are added up in another order)
+            _within(x, y, e, name)
+        if layout == "rows":
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+        again = checkpoint(lambda *x: ct.attention(*x[:3], bias=x[3], **case.arguments()), *leaves, use_reentrant=False)
+        assert all(torch.equal(x, y) for x, y in zip((again, *torch.autograd.grad(again, leaves, g)), want))
+
+
 # ---- refusals ----
 
 def test_refusals(gpu):
@@ -481,6 +512,15 @@ def test_gradients_of_gradients_and_tangents_are_refused(gpu):
 
 def test_results_written_over(gpu):
     """What the backward pass needs may not be changed before it."""
+    x, w = torch.randn((1, 2, 5, 64), device="cuda").half(), torch.randn(64, device="cuda").half().requires_grad_()
+    kept = (w * x).float().sum()
+    ct.RotaryEmbedding(64).inplace(x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(kept, w)
+    with pytest.raises(AssertionError, match="twice"):
+        ct.RotaryEmbedding(64).inplace(x, x)
+    with torch.inference_mode():
+        ct.RotaryEmbedding(64).inplace(torch.ones((1, 2, 5, 64), **HALF))
     q = torch.randn((1, 2, 5, 64), device="cuda").half().requires_grad_()
     out = ct.attention(q, q, q)
     out.detach().add_(1)
