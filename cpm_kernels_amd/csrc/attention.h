@@ -667,6 +667,9 @@ inline int attn_check(Attention& a, int32_t batch, int32_t heads, int32_t kv_hea
     }
     if (kv_heads == 0 || heads % kv_heads) return CPMK_EBADARG;
     if (a.dim > 256 || a.tokens > kAttnLong || a.length > kAttnLong || !grid_fits((int64_t)batch * heads)) return CPMK_ETOOBIG;
+    if (!(fabsf(a.scale) < __builtin_inff())) return CPMK_EBADARG;
+    // (products of fp16 numbers sum up to 2^40 at most: times this they are nothing beside 1, while biases over it would leave fp32)
+    if (fabsf(a.scale) < 0x1p-100f) a.scale = 0.0f;
     if (a.table && (!a.mapping || a.buckets <= 0 || a.distances <= 0)) return CPMK_EBADARG;
     if (a.table && (int64_t)a.distances * (bidirectional ? 2 : 1) > 1024) return CPMK_ETOOBIG;
     a.heads = heads, a.held = kv_heads, a.group = heads / kv_heads;

@@ -30,7 +30,7 @@ def _backward(b=1, h=2, kv=1, n=40, d=64, length=64, q=P, k=P, out=P, lens_each=
 
 def test_refusals_of_the_c_abi():
     for call in (_forward, _backward):
-        for bad in (dict(b=-1), dict(h=-2), dict(kv=-1), dict(n=-1), dict(d=-8), dict(length=-1), dict(len=-1), dict(len=65), dict(kv=0), dict(h=3, kv=2), dict(q=N), dict(k=N), dict(out=N),
+        for bad in (dict(b=-1), dict(h=-2), dict(kv=-1), dict(n=-1), dict(d=-8), dict(length=-1), dict(len=-1), dict(len=65), dict(kv=0), dict(h=3, kv=2), dict(q=N), dict(k=N), dict(out=N), dict(scale=float("nan")), dict(scale=float("-inf")),
                     dict(bias=P), dict(bias=P, mapping=P, buckets=0), dict(bias=P, mapping=P, distances=0), dict(bias=P, mapping=P, distances=-1)):
             with pytest.raises(RuntimeError, match="invalid argument"):
                 call(**bad)

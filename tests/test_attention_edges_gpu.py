@@ -94,6 +94,23 @@ def test_bucket_numbers_outside_of_the_table(gpu, n):
         _within(x, y, e, name)
 
 
+@pytest.mark.parametrize("n,d,mask", [(70, 256, "query"), (40, 256, "key"), (70, 64, None), (3, 128, "key"), (3, 256, None)])
+@pytest.mark.parametrize("bias", ["one", "both"])
+def test_largest_tables_and_far_positions(gpu, n, d, mask, bias):
+    """As many distances as there may be beside the largest heads, and positions at either end of what is told apart."""
+    print("largest tables", n, d, mask, bias, flush=True)
+    distance = 1024 if bias == "one" else 512
+    mapping = np.random.default_rng(d).integers(0, 16, distance).astype(np.int32)
+    for pos in ([0, 900], [2 ** 30 - 1, -2 ** 30]):
+        _Case(2, 2, 1, n, 330, d, causal=False, bias=bias, count=32, distance=distance, mapping=mapping, mask=mask, pos=pos, seed=31).check(True)
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_a_scale_of_nothing(gpu, train):
+    print("scale of nothing", train, flush=True)
+    _Case(1, 2, 1, 70, 90, 64, scale=2.0 ** -120, bias="one", seed=32).check(train)
+
+
 # ---- places that do not count ----
 
 BAD = [np.nan, np.inf, -np.inf, 65504.0]
