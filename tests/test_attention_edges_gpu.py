@@ -547,17 +547,17 @@ def test_results_written_over(gpu):
 
 # ---- calls on addresses ----
 
+@pytest.mark.parametrize("guard", [4096, 4100])
 @pytest.mark.parametrize("n,d", [(2, 64), (70, 64), (70, 128)])
-def test_calls_on_addresses(gpu, n, d):
-    """The kernels layer gives the module's results, and leaves what lies before and behind its outputs and workspaces alone."""
-    print("addresses", n, d, flush=True)
+def test_calls_on_addresses(gpu, n, d, guard):
+    """The kernels layer gives the module's results, and leaves what lies before and behind its outputs and workspaces alone, which begin anywhere on 4 bytes."""
+    print("addresses", n, d, guard, flush=True)
     b, h, held, length = 2, 4, 2, 1200
     case = _Case(b, h, held, n, length, d, bias="one", mask="key", seed=23)
     want, infers = case.run(True), case.run(False)[0]
     st = torch.cuda.current_stream().cuda_stream
     q, k, v, g = (x.contiguous() for x in case.tensors())
     table, mask = torch.from_numpy(case.table).cuda(), torch.from_numpy(case.mask).cuda()
-    guard = 4096
 
     def room(count, dtype):
         raw = torch.full((count * dtype.itemsize + 2 * guard,), 77, dtype=torch.uint8, device="cuda")
